@@ -819,3 +819,118 @@ int bsa_attention_dense_block_mass(const void* q, const void* k, const void* v, 
 }
 
 }  // extern "C"
+
+namespace {
+
+bool is_dtype(int32_t d) { return d == BSA_F32 || d == BSA_BF16 || d == BSA_F16; }
+int64_t dtype_size(int32_t d) { return d == BSA_F32 ? 4 : 2; }
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// The byte ranges [a, a + na) and [b, b + nb) share a byte.
+bool overlaps(const void* a, int64_t na, const void* b, int64_t nb) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return a != nullptr && b != nullptr && x < y + static_cast<uintptr_t>(nb) &&
+         y < x + static_cast<uintptr_t>(na);
+}
+
+}  // namespace
+
+extern "C" {
+
+int bsa_residual_norm(const void* x, int32_t x_dtype, int64_t x_stride, const void* y,
+                      int32_t y_dtype, int64_t y_stride, int64_t rows, int32_t width,
+                      const int32_t* row_starts, int32_t requests, const void* gate,
+                      int64_t gate_stride, const void* shift, int64_t shift_stride,
+                      const void* scale, int64_t scale_stride, int32_t mods_dtype,
+                      const void* weight, const void* bias, int32_t affine_dtype,
+                      const void* post_weight, const void* post_bias, int32_t post_dtype,
+                      int32_t norm, int32_t post_norm, float eps, void* residual, void* normed,
+                      int32_t* err_word, void* stream) {
+  if (!is_dtype(x_dtype) || !is_dtype(y_dtype) || !is_dtype(mods_dtype) ||
+      !is_dtype(affine_dtype) || !is_dtype(post_dtype))
+    return fail(BSA_ERR_INVALID_ARGUMENT, "unknown element type");
+  if (x_dtype != BSA_F32 && y_dtype != x_dtype)
+    return fail(BSA_ERR_UNSUPPORTED, "y and normed must have the type of a 16-bit x");
+  if (rows < 0 || rows > 0x7fffffff)
+    return fail(BSA_ERR_INVALID_ARGUMENT, "rows must be in [0, 2^31)");
+  if (width < 1 || width > 32768)
+    return fail(BSA_ERR_UNSUPPORTED, "width must be in [1, 32768] (got %d)", width);
+  if (norm != BSA_NORM_LAYER && norm != BSA_NORM_RMS)
+    return fail(BSA_ERR_INVALID_ARGUMENT, "norm must be layer or rms");
+  if (post_norm != BSA_NORM_NONE && post_norm != BSA_NORM_LAYER && post_norm != BSA_NORM_RMS)
+    return fail(BSA_ERR_INVALID_ARGUMENT, "post_norm must be none, layer or rms");
+  if (!(eps >= 0.f)) return fail(BSA_ERR_INVALID_ARGUMENT, "eps must be >= 0");
+  if (requests < 1 && rows > 0) return fail(BSA_ERR_INVALID_ARGUMENT, "requests must be >= 1");
+  if (row_starts == nullptr && requests != 1 && requests != rows)
+    return fail(BSA_ERR_INVALID_ARGUMENT, "without row_starts, requests must be 1 or rows");
+  if (y == nullptr && (gate != nullptr || post_norm != BSA_NORM_NONE))
+    return fail(BSA_ERR_INVALID_ARGUMENT, "gate and post_norm need y");
+  if (post_norm == BSA_NORM_NONE && (post_weight != nullptr || post_bias != nullptr))
+    return fail(BSA_ERR_INVALID_ARGUMENT, "post_weight and post_bias need post_norm");
+  if (rows == 0) return ok();
+  if (x == nullptr || normed == nullptr || err_word == nullptr ||
+      (y != nullptr && residual == nullptr))
+    return fail(BSA_ERR_INVALID_ARGUMENT, "null pointer argument");
+  const int64_t sx = dtype_size(x_dtype), sy = dtype_size(y_dtype);
+  const void* natural[] = {x, residual};
+  for (const void* p : natural)
+    if (reinterpret_cast<uintptr_t>(p) % sx)
+      return fail(BSA_ERR_INVALID_ARGUMENT, "x or residual is not aligned to its type");
+  if (reinterpret_cast<uintptr_t>(y) % sy || reinterpret_cast<uintptr_t>(normed) % sy)
+    return fail(BSA_ERR_INVALID_ARGUMENT, "y or normed is not aligned to its type");
+  if (x_stride < 0 || y_stride < 0 || gate_stride < 0 || shift_stride < 0 || scale_stride < 0)
+    return fail(BSA_ERR_INVALID_ARGUMENT, "strides must be >= 0");
+  const int64_t x_bytes = ((rows - 1) * x_stride + width) * sx;
+  const int64_t y_bytes = ((rows - 1) * y_stride + width) * sy;
+  const int64_t r_bytes = y != nullptr ? rows * width * sx : 0, n_bytes = rows * width * sy;
+  if (overlaps(normed, n_bytes, x, x_bytes) || overlaps(normed, n_bytes, y, y_bytes) ||
+      overlaps(normed, n_bytes, y != nullptr ? residual : nullptr, r_bytes) ||
+      (y != nullptr &&
+       (overlaps(residual, r_bytes, x, x_bytes) || overlaps(residual, r_bytes, y, y_bytes))))
+    return fail(BSA_ERR_INVALID_ARGUMENT, "residual and normed must not overlap x, y or each other");
+  bsa::NormArgs a{};
+  a.x = x;
+  a.y = y;
+  a.x_stride = x_stride;
+  a.y_stride = y_stride;
+  a.x_dtype = x_dtype;
+  a.y_dtype = y_dtype;
+  a.rows = rows;
+  a.width = width;
+  a.row_starts = row_starts;
+  a.requests = requests;
+  a.gate = {gate, mods_dtype};
+  a.shift = {shift, mods_dtype};
+  a.scale = {scale, mods_dtype};
+  a.gate_stride = gate_stride;
+  a.shift_stride = shift_stride;
+  a.scale_stride = scale_stride;
+  a.weight = {weight, affine_dtype};
+  a.bias = {bias, affine_dtype};
+  a.post_weight = {post_weight, post_dtype};
+  a.post_bias = {post_bias, post_dtype};
+  a.norm_kind = norm;
+  a.post_kind = post_norm;
+  a.eps = eps;
+  a.residual = residual;
+  a.normed = normed;
+  a.err_word = err_word;
+  const bsa::NormParam params[] = {a.gate, a.shift, a.scale, a.weight, a.bias, a.post_weight,
+                                   a.post_bias};
+  for (const bsa::NormParam& p : params)
+    if (reinterpret_cast<uintptr_t>(p.ptr) % dtype_size(p.dtype))
+      return fail(BSA_ERR_INVALID_ARGUMENT, "a parameter is not aligned to its type");
+  const int64_t sm = dtype_size(mods_dtype);
+  bool vec = width % 8 == 0 && aligned16(x) && aligned16(y) && aligned16(residual) &&
+             aligned16(normed) && x_stride * sx % 16 == 0 && (y == nullptr || y_stride * sy % 16 == 0) &&
+             (gate == nullptr || gate_stride * sm % 16 == 0) &&
+             (shift == nullptr || shift_stride * sm % 16 == 0) &&
+             (scale == nullptr || scale_stride * sm % 16 == 0);
+  for (const bsa::NormParam& p : params) vec = vec && aligned16(p.ptr);
+  a.vectorised = vec ? 1 : 0;
+  const cudaError_t e = bsa::launch_residual_norm(a, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "bsa_residual_norm launch");
+  return ok();
+}
+
+}  // extern "C"

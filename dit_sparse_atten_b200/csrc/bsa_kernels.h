@@ -193,4 +193,38 @@ cudaError_t launch_block_mass(const float* block_lse, const float* lse, int64_t 
                               int64_t tokens, int64_t heads, int32_t blocks, float* mass,
                               cudaStream_t stream);
 
+// ---------------------------------------------------------------------------
+// Packed batches: several requests on one row axis, request s owning rows
+// [row_starts[s], row_starts[s + 1]) (int32, device).
+// ---------------------------------------------------------------------------
+enum Dtype : int32_t { kDtypeF32 = 0, kDtypeBf16 = 1, kDtypeF16 = 2 };
+enum NormKind : int32_t { kNormNone = 0, kNormLayer = 1, kNormRms = 2 };
+
+struct NormParam {
+  const void* ptr;        // nullptr: absent
+  int32_t dtype;          // Dtype
+};
+
+struct NormArgs {
+  const void* x;          // [rows, width], row stride x_stride (elements)
+  const void* y;          // [rows, width] or nullptr (then residual is not written)
+  int64_t x_stride, y_stride;
+  int32_t x_dtype;
+  int32_t y_dtype;        // y's and normed's (x_dtype unless x is float32)
+  int64_t rows;
+  int32_t width;
+  int32_t vectorised;     // every row of every tensor starts on 16 bytes, width % 8 == 0
+  const int32_t* row_starts;  // [requests + 1], or nullptr: requests is 1 or rows
+  int32_t requests;
+  NormParam gate, shift, scale;                     // [requests, width]
+  int64_t gate_stride, shift_stride, scale_stride;  // elements between requests
+  NormParam weight, bias, post_weight, post_bias;   // [width]
+  int32_t norm_kind, post_kind;
+  float eps;
+  void* residual;         // [rows, width] contiguous, x_dtype
+  void* normed;           // [rows, width] contiguous, y_dtype
+  int* err_word;
+};
+cudaError_t launch_residual_norm(const NormArgs& args, cudaStream_t stream);
+
 }  // namespace bsa

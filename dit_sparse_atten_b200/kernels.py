@@ -657,3 +657,129 @@ def pull_rows(peer_shards: Sequence[int], peer_tokens: int, src_row_bytes: int,
     _native.call("bsa_pull_rows", arr, len(peer_shards), int(peer_tokens), int(src_row_bytes),
                  int(src_tensor_bytes), int(src_offset), _native.ptr(perm), T, row_bytes, outs,
                  _native.err_word(device).data_ptr(), _stream(device))
+
+
+# ----------------------------------------------------------------------------
+# packed batches: several requests on one row axis
+# ----------------------------------------------------------------------------
+
+_DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_NORM_KINDS = {None: 0, "layer": 1, "rms": 2}
+
+
+def _starts_i32(starts: torch.Tensor, name: str, device: torch.device) -> torch.Tensor:
+    """Request offsets as contiguous int32 on ``device`` (``[requests + 1]``)."""
+    if starts.dim() != 1 or starts.numel() < 1:
+        raise ValueError(f"{name} must be one-dimensional with requests + 1 entries")
+    if starts.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{name} must be integers")
+    return starts.to(device=device, dtype=torch.int32).contiguous()
+
+
+def _rows_2d(t: torch.Tensor) -> torch.Tensor:
+    """``[..., C]`` as ``[rows, C]`` with contiguous columns (a view where there is one)."""
+    t = t.reshape(-1, t.shape[-1]) if t.dim() != 2 else t
+    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+
+
+class NormResult(NamedTuple):
+    residual: torch.Tensor      # x + gate * post_norm(y); x itself without y
+    normed: torch.Tensor        # the modulated norm of residual
+
+
+def residual_norm(x: torch.Tensor, y: torch.Tensor | None = None, *,
+                  gate: torch.Tensor | None = None, shift: torch.Tensor | None = None,
+                  scale: torch.Tensor | None = None, weight: torch.Tensor | None = None,
+                  bias: torch.Tensor | None = None, norm: str = "layer",
+                  post_norm: str | None = None, post_weight: torch.Tensor | None = None,
+                  post_bias: torch.Tensor | None = None, eps: float = 1e-6,
+                  row_starts: torch.Tensor | None = None,
+                  normed_dtype: torch.dtype | None = None) -> NormResult:
+    """Norms before and after a block, fused with its gate and residual:
+
+    ``residual = x + gate[s] * post_norm(y)``,
+    ``normed = (norm(residual) * weight + bias) * (1 + scale[s]) + shift[s]``
+
+    in float32, for row t of request s (``bsa_residual_norm``).  ``x``, ``y``:
+    ``[..., C]``, rows may be strided; ``x`` bf16, fp16 or float32 (a float32
+    residual stream takes a ``y`` of any of the three types).  ``gate``,
+    ``shift``, ``scale``: ``[requests, C]`` of one type, a row for each request
+    of ``row_starts`` (int ``[requests + 1]``); without ``row_starts``, one row
+    or as many as ``x`` has.  ``norm``/``post_norm``: "layer" or "rms".
+    ``normed_dtype`` (default: ``y``'s, else ``x``'s): ``y``'s type, where a float32 ``x``
+    comes alone any of the three.  Modulated LayerNorm and gated residual of
+    the reference's block: ``wan_diffusers.py:75-117``.
+    """
+    device = _require_cuda(x, y, gate, shift, scale, weight, bias, post_weight, post_bias)
+    if x.dim() < 1 or x.dtype not in _DTYPE_CODES:
+        raise ValueError("x must be [..., C] of bf16, fp16 or float32")
+    if y is not None and y.shape != x.shape:
+        raise ValueError("x and y must have equal shapes")
+    if y is not None and y.dtype not in _DTYPE_CODES:
+        raise ValueError("y must be bf16, fp16 or float32")
+    if norm not in ("layer", "rms") or post_norm not in _NORM_KINDS:
+        raise ValueError('norm must be "layer" or "rms", post_norm one of them or None')
+    if y is None and (gate is not None or post_norm is not None):
+        raise ValueError("gate and post_norm need y")
+    if post_norm is None and (post_weight is not None or post_bias is not None):
+        raise ValueError("post_weight and post_bias need post_norm")
+    if normed_dtype is None:
+        normed_dtype = y.dtype if y is not None else x.dtype
+    if normed_dtype not in _DTYPE_CODES:
+        raise ValueError("normed_dtype must be bf16, fp16 or float32")
+    if y is not None and y.dtype != normed_dtype:
+        raise ValueError("normed has y's type")
+    if x.dtype != torch.float32 and normed_dtype != x.dtype:
+        raise ValueError("y and normed must have the type of a 16-bit x")
+    C = x.shape[-1]
+    xr = _rows_2d(x)
+    yr = _rows_2d(y) if y is not None else None
+    rows = xr.shape[0]
+    if row_starts is not None:
+        row_starts = _starts_i32(row_starts, "row_starts", device)
+        requests = row_starts.numel() - 1
+    else:
+        requests = next((t.shape[0] for t in (gate, shift, scale) if t is not None), 1)
+        if requests not in (1, rows):
+            raise ValueError("without row_starts, modulations have one row or x's number of rows")
+
+    def modulation(t, name):
+        if t is None:
+            return None, 0
+        if t.dim() != 2 or tuple(t.shape) != (requests, C):
+            raise ValueError(f"{name} must be [requests, C] = {(requests, C)}")
+        t = t if t.stride(1) == 1 or C == 1 else t.contiguous()
+        return t, t.stride(0)
+
+    def shared_type(tensors, what):
+        kinds = {t.dtype for t in tensors if t is not None}
+        if len(kinds) > 1 or not kinds <= _DTYPE_CODES.keys():
+            raise ValueError(f"{what} must share one type: bf16, fp16 or float32")
+        return _DTYPE_CODES[kinds.pop()] if kinds else 0
+
+    def vector(t, name):
+        if t is not None and tuple(t.shape) != (C,):
+            raise ValueError(f"{name} must be [C] = [{C}]")
+        return t.contiguous() if t is not None else None
+
+    gate, gate_stride = modulation(gate, "gate")
+    shift, shift_stride = modulation(shift, "shift")
+    scale, scale_stride = modulation(scale, "scale")
+    weight, bias = vector(weight, "weight"), vector(bias, "bias")
+    post_weight, post_bias = vector(post_weight, "post_weight"), vector(post_bias, "post_bias")
+    mods = shared_type((gate, shift, scale), "gate, shift and scale")
+    affine = shared_type((weight, bias), "weight and bias")
+    post = shared_type((post_weight, post_bias), "post_weight and post_bias")
+    residual = torch.empty(x.shape, dtype=x.dtype, device=device) if y is not None else x
+    normed = torch.empty(x.shape, dtype=normed_dtype, device=device)
+    if rows and C:
+        p = _native.ptr
+        _native.call("bsa_residual_norm", xr.data_ptr(), _DTYPE_CODES[x.dtype], xr.stride(0),
+                     p(yr), _DTYPE_CODES[normed_dtype], yr.stride(0) if yr is not None else 0,
+                     rows, C, p(row_starts), requests, p(gate), gate_stride, p(shift),
+                     shift_stride, p(scale), scale_stride, mods, p(weight), p(bias), affine,
+                     p(post_weight), p(post_bias), post, _NORM_KINDS[norm],
+                     _NORM_KINDS[post_norm], float(eps),
+                     residual.data_ptr() if y is not None else None, normed.data_ptr(),
+                     _native.err_word(device).data_ptr(), _stream(device))
+    return NormResult(residual, normed)

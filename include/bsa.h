@@ -401,6 +401,48 @@ BSA_API int bsa_attention_dense_block_mass(const void* q, const void* k, const v
                                            int64_t out_stride_h, float* lse, float* block_lse,
                                            float* mass, int32_t* err_word, void* stream);
 
+/*
+ * Packed batches.  The entry points below take several requests on one row
+ * axis: request s owns rows [row_starts[s], row_starts[s + 1]) (int32 [requests
+ * + 1] in device memory, starting at 0, never decreasing, ending at the number
+ * of rows).  Rows that the offsets do not cover are left unwritten and reported
+ * as BSA_DEVICE_BAD_ROUTE.  Element types are BSA_F32, BSA_BF16 or BSA_F16.
+ */
+#define BSA_F32 0
+#define BSA_BF16 1
+#define BSA_F16 2
+
+#define BSA_NORM_NONE 0
+#define BSA_NORM_LAYER 1 /* (v - mean) / sqrt(var + eps) */
+#define BSA_NORM_RMS 2   /* v / sqrt(mean(v^2) + eps) */
+
+/*
+ * Norms before and after a block, fused with its gate and residual.  For a row
+ * t of request s, in float32:
+ *   p = y[t], or post_norm(y[t]) * post_weight + post_bias
+ *   r = x[t] + gate[s] * p                      -> residual[t] (type of x)
+ *   h = norm(r) * weight + bias
+ *   normed[t] = h * (1 + scale[s]) + shift[s]   (type y_dtype)
+ * y NULL: r = x, residual is not written.  gate, shift, scale ([requests,
+ * width], a row stride in elements each, mods_dtype), weight, bias
+ * (affine_dtype) and post_weight, post_bias (post_dtype) may be NULL (absent).
+ * row_starts NULL: requests must be 1 or rows (a modulation row for each row).
+ * x and y have row strides in elements; residual and normed are contiguous
+ * and must not overlap an input.  x_dtype BSA_F32 goes with any y_dtype,
+ * otherwise y_dtype == x_dtype.  1 <= width <= 32768; norm is LAYER or RMS.
+ * Replaces: attention_backends/wan_diffusers.py:75-117 (the block's modulated
+ *           norms and gated residuals).
+ */
+BSA_API int bsa_residual_norm(const void* x, int32_t x_dtype, int64_t x_stride, const void* y,
+                              int32_t y_dtype, int64_t y_stride, int64_t rows, int32_t width,
+                              const int32_t* row_starts, int32_t requests, const void* gate,
+                              int64_t gate_stride, const void* shift, int64_t shift_stride,
+                              const void* scale, int64_t scale_stride, int32_t mods_dtype,
+                              const void* weight, const void* bias, int32_t affine_dtype,
+                              const void* post_weight, const void* post_bias, int32_t post_dtype,
+                              int32_t norm, int32_t post_norm, float eps, void* residual,
+                              void* normed, int32_t* err_word, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
