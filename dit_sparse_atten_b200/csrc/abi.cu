@@ -933,4 +933,71 @@ int bsa_residual_norm(const void* x, int32_t x_dtype, int64_t x_stride, const vo
   return ok();
 }
 
+int64_t bsa_lora_add_workspace_bytes(int64_t rows, int32_t requests, int32_t k, int32_t rank) {
+  if (rows <= 0 || requests <= 0 || k <= 0 || rank <= 0) return 0;
+  return bsa::lora_plan(rows, requests, k, rank, sm_count()).workspace_bytes;
+}
+
+int bsa_lora_add(const void* y, int64_t y_stride, const void* x, int64_t x_stride,
+                 const void* lora_a, const void* lora_b, const float* scales,
+                 const int32_t* row_starts, const int32_t* adapters, int64_t rows,
+                 int32_t requests, int32_t count, int32_t k, int32_t n, int32_t rank,
+                 void* workspace, int64_t workspace_bytes, void* out, int64_t out_stride,
+                 int32_t* err_word, void* stream) {
+  if (rows < 0 || rows > 0x7fffffff || requests < 0 || count < 0)
+    return fail(BSA_ERR_INVALID_ARGUMENT, "bad rows, requests or count");
+  if (rank < 8 || rank > 128 || rank % 8 != 0)
+    return fail(BSA_ERR_UNSUPPORTED, "rank must be a multiple of 8 in [8, 128] (got %d)", rank);
+  if (k < 8 || n < 8 || k % 8 != 0 || n % 8 != 0)
+    return fail(BSA_ERR_UNSUPPORTED, "k and n must be positive multiples of 8 (got %d, %d)", k, n);
+  if (n > 65535 * 256) return fail(BSA_ERR_UNSUPPORTED, "n is too large (%d)", n);
+  if (x_stride < k || y_stride < n || out_stride < n || (x_stride | y_stride | out_stride) % 8 != 0)
+    return fail(BSA_ERR_INVALID_ARGUMENT,
+                "row strides must be multiples of 8 elements and hold a row");
+  if (rows == 0) return ok();
+  if (requests < 1) return fail(BSA_ERR_INVALID_ARGUMENT, "requests must be >= 1");
+  if (y == nullptr || x == nullptr || out == nullptr || row_starts == nullptr ||
+      adapters == nullptr || err_word == nullptr || workspace == nullptr ||
+      (count > 0 && (lora_a == nullptr || lora_b == nullptr)))
+    return fail(BSA_ERR_INVALID_ARGUMENT, "null pointer argument");
+  const void* ptrs[] = {y, x, out, lora_a, lora_b, workspace};
+  for (const void* p : ptrs)
+    if (!aligned16(p)) return fail(BSA_ERR_INVALID_ARGUMENT, "tensors must be 16-byte aligned");
+  const bsa::LoraPlan plan = bsa::lora_plan(rows, requests, k, rank, sm_count());
+  if (workspace_bytes < plan.workspace_bytes)
+    return fail(BSA_ERR_INVALID_ARGUMENT, "workspace of %lld bytes needed (got %lld)",
+                static_cast<long long>(plan.workspace_bytes),
+                static_cast<long long>(workspace_bytes));
+  const int64_t out_bytes = ((rows - 1) * out_stride + n) * 2;
+  if (overlaps(out, out_bytes, x, ((rows - 1) * x_stride + k) * 2) ||
+      ((out != y || out_stride != y_stride) &&
+       overlaps(out, out_bytes, y, ((rows - 1) * y_stride + n) * 2)))
+    return fail(BSA_ERR_INVALID_ARGUMENT, "out must not overlap x, nor y unless it is y");
+  bsa::LoraArgs a{};
+  a.y = static_cast<const __nv_bfloat16*>(y);
+  a.x = static_cast<const __nv_bfloat16*>(x);
+  a.out = static_cast<__nv_bfloat16*>(out);
+  a.y_stride = y_stride;
+  a.x_stride = x_stride;
+  a.out_stride = out_stride;
+  a.lora_a = static_cast<const __nv_bfloat16*>(lora_a);
+  a.lora_b = static_cast<const __nv_bfloat16*>(lora_b);
+  a.scales = scales;
+  a.row_starts = row_starts;
+  a.adapters = adapters;
+  a.rows = rows;
+  a.requests = requests;
+  a.count = count;
+  a.k = k;
+  a.n = n;
+  a.rank = rank;
+  a.rank_pad = plan.rank_pad;
+  a.slices = plan.slices;
+  a.workspace = static_cast<float*>(workspace);
+  a.err_word = err_word;
+  const cudaError_t e = bsa::launch_lora_add(a, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "bsa_lora_add launch");
+  return ok();
+}
+
 }  // extern "C"

@@ -227,4 +227,30 @@ struct NormArgs {
 };
 cudaError_t launch_residual_norm(const NormArgs& args, cudaStream_t stream);
 
+// Low-rank adapters (lora.cu).
+struct LoraPlan {
+  int32_t rank_pad;         // columns of a workspace row
+  int32_t slices;           // partial sums over K
+  int64_t workspace_bytes;
+};
+LoraPlan lora_plan(int64_t rows, int32_t requests, int32_t k, int32_t rank, int num_sms);
+
+struct LoraArgs {
+  const __nv_bfloat16* y;       // [rows, n], row stride y_stride (elements)
+  const __nv_bfloat16* x;       // [rows, k], row stride x_stride
+  __nv_bfloat16* out;           // [rows, n], row stride out_stride
+  int64_t y_stride, x_stride, out_stride;
+  const __nv_bfloat16* lora_a;  // [count, rank, k]
+  const __nv_bfloat16* lora_b;  // [count, n, rank]
+  const float* scales;          // [count] or nullptr (1)
+  const int32_t* row_starts;    // [requests + 1]
+  const int32_t* adapters;      // [requests], -1: none
+  int64_t rows;
+  int32_t requests, count, k, n, rank;
+  int32_t rank_pad, slices;     // of lora_plan
+  float* workspace;             // [slices, rows, rank_pad]
+  int* err_word;
+};
+cudaError_t launch_lora_add(const LoraArgs& args, cudaStream_t stream);
+
 }  // namespace bsa

@@ -783,3 +783,69 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor | None = None, *,
                      residual.data_ptr() if y is not None else None, normed.data_ptr(),
                      _native.err_word(device).data_ptr(), _stream(device))
     return NormResult(residual, normed)
+
+
+def lora_add(y: torch.Tensor, x: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, *,
+             row_starts: torch.Tensor, adapters: torch.Tensor,
+             scales: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Low-rank adapters of many requests beside a shared projection:
+
+    ``out[t] = y[t] + scales[i] * (x[t] @ lora_a[i].T) @ lora_b[i].T`` for a row
+    t of request s with adapter ``i = adapters[s]``, ``out[t] = y[t]`` where it
+    is -1 (``bsa_lora_add``).  bf16 ``y [..., N]`` (the projection's output),
+    ``x [..., K]``, ``lora_a [count, R, K]``, ``lora_b [count, N, R]``; int
+    ``row_starts [requests + 1]``, ``adapters [requests]``; float32 ``scales
+    [count]`` (default 1).  K, N and R are multiples of 8, R at most 128
+    (adapters of lower rank: pad both factors with zeros).  ``out``: an output
+    to write, ``y`` itself included; by default a new tensor.
+    """
+    device = _require_cuda(y, x, lora_a, lora_b, scales, out)
+    if any(t.dtype != torch.bfloat16 for t in (y, x, lora_a, lora_b)):
+        raise ValueError("lora_add expects bf16 y, x, lora_a and lora_b")
+    if y.dim() < 1 or x.dim() < 1 or y.shape[:-1] != x.shape[:-1]:
+        raise ValueError("y and x must be [..., N] and [..., K] with the same rows")
+    N, K = y.shape[-1], x.shape[-1]
+    if lora_a.dim() != 3 or lora_a.shape[2] != K:
+        raise ValueError(f"lora_a must be [count, R, K] with K = {K}")
+    count, R = lora_a.shape[0], lora_a.shape[1]
+    if tuple(lora_b.shape) != (count, N, R):
+        raise ValueError(f"lora_b must be [count, N, R] = {(count, N, R)}")
+    row_starts = _starts_i32(row_starts, "row_starts", device)
+    requests = row_starts.numel() - 1
+    if tuple(adapters.shape) != (requests,) or adapters.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"adapters must be integers [requests] = [{requests}]")
+    adapters = adapters.to(device=device, dtype=torch.int32).contiguous()
+    if scales is not None:
+        if tuple(scales.shape) != (count,):
+            raise ValueError(f"scales must be [count] = [{count}]")
+        scales = scales.to(torch.float32).contiguous()
+
+    def rows_8(t):
+        t = _rows_2d(t)
+        ok = t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0
+        return t if ok else t.contiguous().clone() if t.data_ptr() % 16 else t.contiguous()
+
+    if out is None:
+        out = torch.empty(y.shape, dtype=y.dtype, device=device)
+        yr, o = rows_8(y), out.view(-1, N)
+    else:
+        if out.shape != y.shape or out.dtype != y.dtype:
+            raise ValueError("out must have y's shape and type")
+        if out.dim() != 2 and not out.is_contiguous():
+            raise ValueError("an out of more than two dimensions must be contiguous")
+        o = out if out.dim() == 2 else out.view(-1, N)
+        if o.stride(1) != 1:
+            raise ValueError("out must have contiguous columns")
+        yr = o if out is y else rows_8(y)
+    xr = rows_8(x)
+    rows = xr.shape[0]
+    if rows and N:
+        lora_a, lora_b = lora_a.contiguous(), lora_b.contiguous()
+        nbytes = _native.load_library().bsa_lora_add_workspace_bytes(rows, requests, K, R)
+        work = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        _native.call("bsa_lora_add", yr.data_ptr(), yr.stride(0), xr.data_ptr(), xr.stride(0),
+                     lora_a.data_ptr(), lora_b.data_ptr(), _native.ptr(scales),
+                     row_starts.data_ptr(), adapters.data_ptr(), rows, requests, count, K, N, R,
+                     work.data_ptr(), nbytes, o.data_ptr(), o.stride(0),
+                     _native.err_word(device).data_ptr(), _stream(device))
+    return out

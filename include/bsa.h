@@ -443,6 +443,30 @@ BSA_API int bsa_residual_norm(const void* x, int32_t x_dtype, int64_t x_stride, 
                               int32_t norm, int32_t post_norm, float eps, void* residual,
                               void* normed, int32_t* err_word, void* stream);
 
+/*
+ * Low-rank adapters of many requests beside a shared projection.  For a row t
+ * of request s with adapter i = adapters[s]:
+ *   out[t] = y[t] + scales[i] * (x[t] A_i^T) B_i^T
+ * and out[t] = y[t] where adapters[s] is -1.  bf16 throughout, float32 sums;
+ * the scaled x A^T is rounded to bf16 between the two products.
+ * y: [rows, n] (the shared projection's output), x: [rows, k], out: [rows, n],
+ * row strides in elements; out may be y itself (same stride).  lora_a: [count,
+ * rank, k], lora_b: [count, n, rank], scales: fp32 [count] or NULL (1),
+ * adapters: int32 [requests]; an id outside [-1, count) counts as -1 and is
+ * reported as BSA_DEVICE_BAD_ROUTE.  k, n, rank and the strides are multiples
+ * of 8, pointers 16-byte aligned, rank <= 128.  workspace: at least
+ * bsa_lora_add_workspace_bytes of the same sizes, 16-byte aligned.
+ * No reference counterpart (the reference loads no adapters).
+ */
+BSA_API int64_t bsa_lora_add_workspace_bytes(int64_t rows, int32_t requests, int32_t k,
+                                             int32_t rank);
+BSA_API int bsa_lora_add(const void* y, int64_t y_stride, const void* x, int64_t x_stride,
+                         const void* lora_a, const void* lora_b, const float* scales,
+                         const int32_t* row_starts, const int32_t* adapters, int64_t rows,
+                         int32_t requests, int32_t count, int32_t k, int32_t n, int32_t rank,
+                         void* workspace, int64_t workspace_bytes, void* out, int64_t out_stride,
+                         int32_t* err_word, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
