@@ -59,6 +59,9 @@ SIGNATURES = {
     "bsa_lora_add_workspace_bytes": ([_I64, _I32, _I32, _I32], _I64),
     "bsa_lora_add": ([_P, _I64, _P, _I64, _P, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _I32,
                       _P, _I64, _P, _I64, _P, _P], _I32),
+    "bsa_packed_attention_workspace_bytes": ([_I64, _I64, _I32, _I32, _I32], _I64),
+    "bsa_packed_attention": ([_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _I64, _I64,
+                              _I32, _I32, _I32, _I32, _I32, _F32, _P, _I64, _P, _P, _P], _I32),
 }
 
 DEVICE_ERRORS = {

@@ -1001,3 +1001,133 @@ int bsa_lora_add(const void* y, int64_t y_stride, const void* x, int64_t x_strid
 }
 
 }  // extern "C"
+
+namespace {
+
+int64_t packed_workspace(int64_t q_rows, int32_t heads, int32_t splits) {
+  return splits > 1 ? q_rows * heads * splits * (128 + 2) * 4 : 0;
+}
+
+// 3-D bf16 map over [rows, heads, 128] with element strides; box: 64 features
+// x `box_heads` heads x `box_rows` rows, 128-byte swizzle, zero fill.
+int encode_rhd(CUtensorMap* map, const void* ptr, int64_t rows, int64_t heads, int64_t stride_t,
+               int64_t stride_h, int box_heads, int box_rows, const char* name) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) return fail(BSA_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+  cuuint64_t dims[3] = {128u, static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(stride_h) * 2,
+                           static_cast<cuuint64_t>(stride_t) * 2};
+  if (heads == 1) strides[0] = 256;                       // unused; kept well-formed
+  if (rows == 1) strides[1] = strides[0] * dims[1];
+  cuuint32_t box[3] = {64u, static_cast<cuuint32_t>(box_heads), static_cast<cuuint32_t>(box_rows)};
+  cuuint32_t estr[3] = {1u, 1u, 1u};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(ptr), dims,
+                        strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(BSA_ERR_CUDA, "cuTensorMapEncodeTiled failed for %s (%d)", name, (int)r);
+  return BSA_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t bsa_packed_attention_workspace_bytes(int64_t q_rows, int64_t k_rows, int32_t requests,
+                                             int32_t heads, int32_t kv_heads) {
+  if (q_rows <= 0 || k_rows <= 0 || requests <= 0 || heads <= 0 || kv_heads <= 0 ||
+      heads % kv_heads != 0 || heads / kv_heads > 128)
+    return 0;
+  return packed_workspace(
+      q_rows, heads, bsa::packed_splits(q_rows, k_rows, requests, heads, kv_heads, sm_count()));
+}
+
+int bsa_packed_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k,
+                         int64_t k_stride_t, int64_t k_stride_h, const void* v,
+                         int64_t v_stride_t, int64_t v_stride_h, const int32_t* q_starts,
+                         const int32_t* k_starts, int64_t q_rows, int64_t k_rows,
+                         int32_t requests, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                         int32_t causal, float scale, void* workspace, int64_t workspace_bytes,
+                         void* out, int32_t* err_word, void* stream) {
+  if (head_dim != 128) return fail(BSA_ERR_UNSUPPORTED, "head_dim must be 128 (got %d)", head_dim);
+  const int64_t most = 0x7fffffff - 256;
+  if (q_rows < 0 || k_rows < 0 || q_rows > most || k_rows > most || requests < 0)
+    return fail(BSA_ERR_INVALID_ARGUMENT, "bad q_rows, k_rows or requests");
+  if (heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0)
+    return fail(BSA_ERR_INVALID_ARGUMENT, "kv_heads must divide heads (%d, %d)", heads, kv_heads);
+  if (heads / kv_heads > 128)
+    return fail(BSA_ERR_UNSUPPORTED, "at most 128 query heads to a key head (got %d)",
+                heads / kv_heads);
+  if (!(scale > 0.f) || scale > 3.0e38f)
+    return fail(BSA_ERR_INVALID_ARGUMENT, "scale must be positive and finite");
+  if (q_rows == 0) return ok();
+  if (requests < 1) return fail(BSA_ERR_INVALID_ARGUMENT, "requests must be >= 1");
+  if (q == nullptr || out == nullptr || q_starts == nullptr || k_starts == nullptr ||
+      err_word == nullptr || (k_rows > 0 && (k == nullptr || v == nullptr)))
+    return fail(BSA_ERR_INVALID_ARGUMENT, "null pointer argument");
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(workspace))
+    return fail(BSA_ERR_INVALID_ARGUMENT, "tensors must be 16-byte aligned");
+  const int64_t strides[3][3] = {{q_stride_t, q_stride_h, heads},
+                                 {k_stride_t, k_stride_h, kv_heads},
+                                 {v_stride_t, v_stride_h, kv_heads}};
+  for (const auto& s : strides)
+    if (s[0] % 8 != 0 || s[1] % 8 != 0 || s[0] < 128 || (s[2] > 1 && (s[1] < 128 || s[0] < s[1])))
+      return fail(BSA_ERR_INVALID_ARGUMENT,
+                  "strides must be multiples of 8, head stride >= 128, token stride >= head stride");
+  const int64_t out_bytes = q_rows * heads * 256;
+  if (overlaps(out, out_bytes, q, ((q_rows - 1) * q_stride_t + (heads - 1) * q_stride_h + 128) * 2) ||
+      (k_rows > 0 &&
+       (overlaps(out, out_bytes, k, ((k_rows - 1) * k_stride_t + (kv_heads - 1) * k_stride_h + 128) * 2) ||
+        overlaps(out, out_bytes, v, ((k_rows - 1) * v_stride_t + (kv_heads - 1) * v_stride_h + 128) * 2))))
+    return fail(BSA_ERR_INVALID_ARGUMENT, "out must not overlap q, k or v");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (k_rows == 0) {   // no request has a key
+    const cudaError_t e = cudaMemsetAsync(out, 0, out_bytes, s);
+    if (e != cudaSuccess) return cuda_fail(e, "bsa_packed_attention memset");
+    return ok();
+  }
+  bsa::PackedArgs a{};
+  a.q = static_cast<const __nv_bfloat16*>(q);
+  a.k = static_cast<const __nv_bfloat16*>(k);
+  a.v = static_cast<const __nv_bfloat16*>(v);
+  a.q_stride_t = q_stride_t;
+  a.q_stride_h = q_stride_h;
+  a.k_stride_t = k_stride_t;
+  a.k_stride_h = k_stride_h;
+  a.v_stride_t = v_stride_t;
+  a.v_stride_h = v_stride_h;
+  a.q_starts = q_starts;
+  a.k_starts = k_starts;
+  a.q_rows = q_rows;
+  a.k_rows = k_rows;
+  a.requests = requests;
+  a.heads = heads;
+  a.kv_heads = kv_heads;
+  a.group = heads / kv_heads;
+  a.tile_tokens = 128 / a.group;
+  a.slots = q_rows / a.tile_tokens + requests;
+  a.splits = bsa::packed_splits(q_rows, k_rows, requests, heads, kv_heads, sm_count());
+  a.causal = causal != 0;
+  a.scale = scale;
+  a.out = static_cast<__nv_bfloat16*>(out);
+  const int64_t need = packed_workspace(q_rows, heads, a.splits);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+    return fail(BSA_ERR_INVALID_ARGUMENT, "workspace of %lld bytes needed (got %lld)",
+                static_cast<long long>(need), static_cast<long long>(workspace_bytes));
+  a.part_o = static_cast<float*>(workspace);
+  a.part_ml = need > 0 ? a.part_o + q_rows * heads * a.splits * 128 : nullptr;
+  a.err_word = err_word;
+  if (a.slots * kv_heads * a.splits > 0x7fffffff)
+    return fail(BSA_ERR_UNSUPPORTED, "too many query tiles");
+  CUtensorMap tq, tk, tv;
+  int rc = encode_rhd(&tq, q, q_rows, heads, q_stride_t, q_stride_h, a.group, a.tile_tokens, "q");
+  if (rc == BSA_OK) rc = encode_rhd(&tk, k, k_rows, kv_heads, k_stride_t, k_stride_h, 1, 128, "k");
+  if (rc == BSA_OK) rc = encode_rhd(&tv, v, k_rows, kv_heads, v_stride_t, v_stride_h, 1, 128, "v");
+  if (rc != BSA_OK) return rc;
+  const cudaError_t e = bsa::launch_packed_attention(tq, tk, tv, a, s);
+  if (e != cudaSuccess) return cuda_fail(e, "bsa_packed_attention launch");
+  return ok();
+}
+
+}  // extern "C"

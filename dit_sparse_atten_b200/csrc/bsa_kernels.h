@@ -253,4 +253,31 @@ struct LoraArgs {
 };
 cudaError_t launch_lora_add(const LoraArgs& args, cudaStream_t stream);
 
+// Attention over packed sequences (packed_attention.cu).
+struct PackedArgs {
+  const __nv_bfloat16* q;       // [q_rows, heads, 128], strides below (elements)
+  const __nv_bfloat16* k;       // [k_rows, kv_heads, 128]
+  const __nv_bfloat16* v;
+  int64_t q_stride_t, q_stride_h, k_stride_t, k_stride_h, v_stride_t, v_stride_h;
+  const int32_t* q_starts;      // [requests + 1]
+  const int32_t* k_starts;      // [requests + 1]
+  int64_t q_rows, k_rows;
+  int32_t requests, heads, kv_heads;
+  int32_t group;                // heads / kv_heads <= 128
+  int32_t tile_tokens;          // 128 / group
+  int64_t slots;                // q_rows / tile_tokens + requests
+  int32_t splits;
+  bool causal;
+  float scale;
+  __nv_bfloat16* out;           // [q_rows, heads, 128] contiguous
+  float* part_o;                // [splits, q_rows, heads, 128] (splits > 1)
+  float* part_ml;               // [splits, q_rows, heads, 2]: stabiliser (log2), sum
+  int* err_word;
+};
+int32_t packed_splits(int64_t q_rows, int64_t k_rows, int32_t requests, int32_t heads,
+                      int32_t kv_heads, int num_sms);
+cudaError_t launch_packed_attention(const CUtensorMap& tm_q, const CUtensorMap& tm_k,
+                                    const CUtensorMap& tm_v, const PackedArgs& args,
+                                    cudaStream_t stream);
+
 }  // namespace bsa

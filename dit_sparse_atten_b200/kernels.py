@@ -849,3 +849,53 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, lora_a: torch.Tensor, lora_b: tor
                      work.data_ptr(), nbytes, o.data_ptr(), o.stride(0),
                      _native.err_word(device).data_ptr(), _stream(device))
     return out
+
+
+def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_starts: torch.Tensor,
+                     k_starts: torch.Tensor | None = None, *, causal: bool = False,
+                     scale: float | None = None) -> torch.Tensor:
+    """Attention over packed sequences with grouped heads (``bsa_packed_attention``).
+
+    bf16 ``q [Tq, H, 128]``, ``k, v [Tk, Hk, 128]`` (``Hk`` divides ``H``; query
+    head h uses key head ``h // (H // Hk)``); int ``q_starts``, ``k_starts
+    [requests + 1]`` (``k_starts`` defaults to ``q_starts``).  Query i of a
+    request attends to all its keys, or, ``causal``, to the first ``i + 1 +
+    k_len - q_len`` of them (one new token: all of them).  A query without a
+    key gives 0.  Returns bf16 ``[Tq, H, 128]``.
+    """
+    device = _require_cuda(q, k, v)
+    if any(t.dtype != torch.bfloat16 for t in (q, k, v)):
+        raise ValueError("packed_attention expects bf16 q, k, v")
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape:
+        raise ValueError("q must be [Tq, H, D], k and v [Tk, Hk, D] with equal shapes")
+    Tq, H, D = q.shape
+    Tk, Hk = k.shape[0], k.shape[1]
+    if D != HEAD_DIM or k.shape[2] != HEAD_DIM:
+        raise NotImplementedError(f"head_dim must be {HEAD_DIM}")
+    if Hk == 0 or H % Hk:
+        raise ValueError(f"{Hk} key heads do not divide {H} query heads")
+    if k_starts is None and Tk != Tq:
+        raise ValueError("without k_starts, q and k must have the same rows")
+    q_starts = _starts_i32(q_starts, "q_starts", device)
+    k_starts = q_starts if k_starts is None else _starts_i32(k_starts, "k_starts", device)
+    if q_starts.numel() != k_starts.numel():
+        raise ValueError("q_starts and k_starts must have equal lengths")
+
+    def strided(t):
+        st, sh, sd = t.stride()
+        ok = (sd == 1 and st % 8 == 0 and sh % 8 == 0 and t.data_ptr() % 16 == 0 and st >= D
+              and (t.shape[1] == 1 or (sh >= D and st >= sh)))
+        return t if ok else t.clone(memory_format=torch.contiguous_format)
+    q, k, v = strided(q), strided(k), strided(v)
+    out = torch.empty((Tq, H, D), dtype=q.dtype, device=device)
+    requests = q_starts.numel() - 1
+    if Tq:
+        nbytes = _native.load_library().bsa_packed_attention_workspace_bytes(Tq, Tk, requests, H, Hk)
+        work = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+        s = float(scale) if scale is not None else D ** -0.5
+        _native.call("bsa_packed_attention", q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(),
+                     k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+                     q_starts.data_ptr(), k_starts.data_ptr(), Tq, Tk, requests, H, Hk, D,
+                     1 if causal else 0, s, _native.ptr(work), nbytes, out.data_ptr(),
+                     _native.err_word(device).data_ptr(), _stream(device))
+    return out

@@ -467,6 +467,36 @@ BSA_API int bsa_lora_add(const void* y, int64_t y_stride, const void* x, int64_t
                          void* workspace, int64_t workspace_bytes, void* out, int64_t out_stride,
                          int32_t* err_word, void* stream);
 
+/*
+ * Softmax attention over packed sequences of different lengths with grouped
+ * heads.  Query i of request s (row q_starts[s] + i of q) attends to the keys
+ * of the same request (rows [k_starts[s], k_starts[s + 1]) of k and v); causal:
+ * to the first i + 1 + k_len - q_len of them, so that new tokens see their
+ * past and a single token all of it.  A query that sees no key gives 0.  Query
+ * head h uses key head h / (heads / kv_heads).  Values of k and v at keys that
+ * a query does not see never reach it, infinities and NaN included.
+ * q: bf16 [q_rows, heads, 128], k, v: bf16 [k_rows, kv_heads, 128], token and
+ * head strides in elements (multiples of 8, head stride >= 128, token stride >=
+ * head stride, or kv_heads/heads == 1), 16-byte aligned; out: bf16 [q_rows,
+ * heads, 128] contiguous, not overlapping an input.  kv_heads divides heads,
+ * at most 128 times; scale > 0; q_rows, k_rows < 2^31 - 256.  workspace: at
+ * least bsa_packed_attention_workspace_bytes of the same sizes, 16-byte aligned
+ * (0 bytes: may be NULL): few tiles split their keys over CTAs and join them.
+ * No reference counterpart (its text cross-attention and its dense fallback
+ * call library attention on one request: wan_diffusers.py:75-117, dense.py).
+ */
+BSA_API int64_t bsa_packed_attention_workspace_bytes(int64_t q_rows, int64_t k_rows,
+                                                     int32_t requests, int32_t heads,
+                                                     int32_t kv_heads);
+BSA_API int bsa_packed_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h,
+                                 const void* k, int64_t k_stride_t, int64_t k_stride_h,
+                                 const void* v, int64_t v_stride_t, int64_t v_stride_h,
+                                 const int32_t* q_starts, const int32_t* k_starts, int64_t q_rows,
+                                 int64_t k_rows, int32_t requests, int32_t heads,
+                                 int32_t kv_heads, int32_t head_dim, int32_t causal, float scale,
+                                 void* workspace, int64_t workspace_bytes, void* out,
+                                 int32_t* err_word, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
