@@ -928,7 +928,7 @@ int bsa_residual_norm(const void* x, int32_t x_dtype, int64_t x_stride, const vo
              (scale == nullptr || scale_stride * sm % 16 == 0);
   for (const bsa::NormParam& p : params) vec = vec && aligned16(p.ptr);
   a.vectorised = vec ? 1 : 0;
-  const cudaError_t e = bsa::launch_residual_norm(a, static_cast<cudaStream_t>(stream));
+  const cudaError_t e = bsa::launch_residual_norm(a, static_cast<cudaStream_t>(stream), sm_count());
   if (e != cudaSuccess) return cuda_fail(e, "bsa_residual_norm launch");
   return ok();
 }

@@ -225,7 +225,7 @@ struct NormArgs {
   void* normed;           // [rows, width] contiguous, y_dtype
   int* err_word;
 };
-cudaError_t launch_residual_norm(const NormArgs& args, cudaStream_t stream);
+cudaError_t launch_residual_norm(const NormArgs& args, cudaStream_t stream, int num_sms);
 
 // Low-rank adapters (lora.cu).
 struct LoraPlan {

@@ -120,6 +120,31 @@ def test_post_norm(post, width):
     check(call(t, keys, norm="rms", post_norm=post), t, keys, norm="rms", post_norm=post)
 
 
+@pytest.mark.parametrize("width", [8, 40, 256, 264, 512, 520, 1536, 2560, 5120, 5128, 8192, 10240])
+@pytest.mark.parametrize("dtype,ydtype,norm,post", [
+    (torch.bfloat16, torch.bfloat16, "layer", None), (torch.float16, torch.float16, "rms", "layer"),
+    (torch.float32, torch.bfloat16, "rms", None), (torch.float32, torch.float32, "layer", "rms")])
+def test_many_rows(width, dtype, ydtype, norm, post):
+    """Enough rows for the resident blocks: several a block, requests that
+    begin and end between a block's rows, some of a single row."""
+    t = make([300, 0, 1, 2, 700, 149, 1], width, dtype=dtype, ydtype=ydtype, seed=width)
+    keys = AFFINE + (("post_weight",) if post else ())
+    check(call(t, keys, norm=norm, post_norm=post), t, keys, norm=norm, post_norm=post)
+    if width == 520:
+        for keys in ((), ("y",), ("shift", "scale"), ("y", "gate", "weight")):
+            check(call(t, keys, norm=norm), t, keys, norm=norm)
+        keys = AFFINE + ("post_weight", "post_bias")
+        check(call(t, keys, norm=norm, post_norm="rms"), t, keys, norm=norm, post_norm="rms")
+        rows = t["x"].shape[0]
+        t = make([rows], width, dtype=dtype, ydtype=ydtype, seed=1, requests=rows)
+        check(call(t, ALL, row_starts=None), t, ALL, row_request=np.arange(rows))
+        bad = dict(t, starts=torch.tensor([0, 600, 900], dtype=torch.int32, device=DEV),
+                   **{k: t[k][:2] for k in ("gate", "shift", "scale")})
+        call(bad, ALL)
+        with pytest.raises(RuntimeError, match="out of range"):
+            _native.check_device_errors()
+
+
 def test_many_requests_and_per_row_modulation():
     for s in (1, 2, 31, 32, 33, 64, 65, 200, 1024, 1025, 1500):
         lengths = [(i * 7) % 3 for i in range(s)]
