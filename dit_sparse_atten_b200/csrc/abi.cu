@@ -826,6 +826,22 @@ bool is_dtype(int32_t d) { return d == BSA_F32 || d == BSA_BF16 || d == BSA_F16;
 int64_t dtype_size(int32_t d) { return d == BSA_F32 ? 4 : 2; }
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+// bf16 tensor map: dims from the innermost, byte strides of the outer ones,
+// 128-byte swizzle (inner box of 64 elements), zero fill out of bounds.
+int encode_bf16(CUtensorMap* map, const void* ptr, int rank, const cuuint64_t* dims,
+                const cuuint64_t* strides, const cuuint32_t* box, const char* name) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) return fail(BSA_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+  const cuuint32_t ones[3] = {1u, 1u, 1u};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, static_cast<cuuint32_t>(rank),
+                        const_cast<void*>(ptr), dims, strides, box, ones,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(BSA_ERR_CUDA, "cuTensorMapEncodeTiled failed for %s (%d)", name, (int)r);
+  return BSA_OK;
+}
+
 // The byte ranges [a, a + na) and [b, b + nb) share a byte.
 bool overlaps(const void* a, int64_t na, const void* b, int64_t nb) {
   const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
@@ -993,9 +1009,26 @@ int bsa_lora_add(const void* y, int64_t y_stride, const void* x, int64_t x_strid
   a.rank = rank;
   a.rank_pad = plan.rank_pad;
   a.slices = plan.slices;
-  a.workspace = static_cast<float*>(workspace);
+  a.few_rows = plan.few_rows;
+  a.workspace = static_cast<__nv_bfloat16*>(workspace);
   a.err_word = err_word;
-  const cudaError_t e = bsa::launch_lora_add(a, static_cast<cudaStream_t>(stream));
+  CUtensorMap tx{}, ta{};
+  if (!a.few_rows && count > 0) {
+    const cuuint64_t x_dims[2] = {static_cast<cuuint64_t>(k), static_cast<cuuint64_t>(rows)};
+    const cuuint64_t x_strides[1] = {static_cast<cuuint64_t>(x_stride) * 2};
+    const cuuint32_t x_box[2] = {64u, 128u};
+    int rc = encode_bf16(&tx, x, 2, x_dims, x_strides, x_box, "x");
+    if (rc != BSA_OK) return rc;
+    const cuuint64_t a_dims[3] = {static_cast<cuuint64_t>(k), static_cast<cuuint64_t>(rank),
+                                  static_cast<cuuint64_t>(count)};
+    const cuuint64_t a_strides[2] = {static_cast<cuuint64_t>(k) * 2,
+                                     static_cast<cuuint64_t>(k) * rank * 2};
+    const cuuint32_t a_box[3] = {64u, static_cast<cuuint32_t>(bsa::lora_rank_box(rank)), 1u};
+    rc = encode_bf16(&ta, lora_a, 3, a_dims, a_strides, a_box, "lora_a");
+    if (rc != BSA_OK) return rc;
+  }
+  const cudaError_t e =
+      bsa::launch_lora_add(tx, ta, a, static_cast<cudaStream_t>(stream), sm_count());
   if (e != cudaSuccess) return cuda_fail(e, "bsa_lora_add launch");
   return ok();
 }
@@ -1008,26 +1041,18 @@ int64_t packed_workspace(int64_t q_rows, int32_t heads, int32_t splits) {
   return splits > 1 ? q_rows * heads * splits * (128 + 2) * 4 : 0;
 }
 
-// 3-D bf16 map over [rows, heads, 128] with element strides; box: 64 features
-// x `box_heads` heads x `box_rows` rows, 128-byte swizzle, zero fill.
+// Map over [rows, heads, 128] with element strides; box: 64 features x
+// `box_heads` heads x `box_rows` rows.
 int encode_rhd(CUtensorMap* map, const void* ptr, int64_t rows, int64_t heads, int64_t stride_t,
                int64_t stride_h, int box_heads, int box_rows, const char* name) {
-  EncodeTiledFn fn = encode_fn();
-  if (fn == nullptr) return fail(BSA_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
-  cuuint64_t dims[3] = {128u, static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t dims[3] = {128u, static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(rows)};
   cuuint64_t strides[2] = {static_cast<cuuint64_t>(stride_h) * 2,
                            static_cast<cuuint64_t>(stride_t) * 2};
   if (heads == 1) strides[0] = 256;                       // unused; kept well-formed
   if (rows == 1) strides[1] = strides[0] * dims[1];
-  cuuint32_t box[3] = {64u, static_cast<cuuint32_t>(box_heads), static_cast<cuuint32_t>(box_rows)};
-  cuuint32_t estr[3] = {1u, 1u, 1u};
-  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(ptr), dims,
-                        strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS)
-    return fail(BSA_ERR_CUDA, "cuTensorMapEncodeTiled failed for %s (%d)", name, (int)r);
-  return BSA_OK;
+  const cuuint32_t box[3] = {64u, static_cast<cuuint32_t>(box_heads),
+                             static_cast<cuuint32_t>(box_rows)};
+  return encode_bf16(map, ptr, 3, dims, strides, box, name);
 }
 
 }  // namespace

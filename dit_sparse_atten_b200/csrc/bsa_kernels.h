@@ -230,10 +230,12 @@ cudaError_t launch_residual_norm(const NormArgs& args, cudaStream_t stream, int 
 // Low-rank adapters (lora.cu).
 struct LoraPlan {
   int32_t rank_pad;         // columns of a workspace row
-  int32_t slices;           // partial sums over K
+  int32_t slices;           // CTAs (of one cluster) that share a row tile's K
+  bool few_rows;            // tiles of 8 rows, no tensor maps
   int64_t workspace_bytes;
 };
 LoraPlan lora_plan(int64_t rows, int32_t requests, int32_t k, int32_t rank, int num_sms);
+int lora_rank_box(int32_t rank);   // ranks a box of lora_a's tensor map covers
 
 struct LoraArgs {
   const __nv_bfloat16* y;       // [rows, n], row stride y_stride (elements)
@@ -248,10 +250,15 @@ struct LoraArgs {
   int64_t rows;
   int32_t requests, count, k, n, rank;
   int32_t rank_pad, slices;     // of lora_plan
-  float* workspace;             // [slices, rows, rank_pad]
+  bool few_rows;
+  int32_t col_ctas;             // set by the launch
+  __nv_bfloat16* workspace;     // [rows, rank_pad]
   int* err_word;
 };
-cudaError_t launch_lora_add(const LoraArgs& args, cudaStream_t stream);
+// tm_x: [rows, k] in boxes of 64 columns x 128 rows; tm_a: lora_a in boxes of
+// 64 columns x lora_rank_box ranks x 1 adapter (both unused with few_rows).
+cudaError_t launch_lora_add(const CUtensorMap& tm_x, const CUtensorMap& tm_a, LoraArgs args,
+                            cudaStream_t stream, int num_sms);
 
 // Attention over packed sequences (packed_attention.cu).
 struct PackedArgs {

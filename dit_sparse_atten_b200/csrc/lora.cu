@@ -4,25 +4,36 @@
 // and out[t] = y[t] without an adapter (-1).  y is the shared projection's
 // output (a plain library product).
 //
-// Two launches: the "shrink" x A^T leaves u [rows, R] (float32 partial sums
-// over slices of K), the "expand" adds the slices, scales and multiplies by
-// B^T.  Bound: HBM (x and y read once, out written once; 2 R (K + N) flops a
-// row are far below the tensor rate for R <= 128).
+// Two launches: the "shrink" leaves u = scales[i] * x A^T as bf16 [rows, R
+// padded to 32] in the workspace, the "expand" adds u B^T to y.  Bound: HBM (x
+// and y read once, out written once; 2 R (K + N) flops a row are far below the
+// tensor rate for R <= 128).  u is rounded to bf16 as the tensor cores'
+// operand: 2^-8 of each of its entries, as the final rounding of a delta that
+// stands alone.
+//
+// K is cut into slices where the row tiles alone would leave SMs idle; the
+// slices of a tile are one thread-block cluster, whose CTAs sum each other's
+// float32 partial tiles through distributed shared memory in a fixed order.
 //
 // A row tile never spans two requests: tile slot g of M rows belongs to
 // request s = #{i >= 1: floor(starts[i] / M) + i <= g} (floor(e/M) - floor(b/M)
 // + 1 >= ceil((e - b) / M), so every request's slots hold its rows), found by
 // one warp search; no list of tiles has to be made on the host.
+#include <algorithm>
+#include <atomic>
+
 #include "bsa_kernels.h"
 #include "packed_common.cuh"
 
 namespace bsa {
 namespace {
 
-constexpr int kShrinkRows = 8;
+constexpr int kFewRows = 8;        // rows a tile, requests of few rows
+constexpr int kTileRows = 128;     // rows a tile, tensor-core shrink
 constexpr int kExpandRows = 64;
 constexpr int kExpandCols = 256;
 constexpr int kWarps = 8;
+constexpr int kMaxSlices = 8;      // portable cluster size
 
 struct Tile {
   int64_t row;      // first row
@@ -39,9 +50,9 @@ __device__ __forceinline__ Tile find_tile(const LoraArgs& a, int64_t g) {
   Tile t{0, 0, -1};
   if (s >= a.requests) return t;
   const int64_t begin = __ldg(a.row_starts + s), end = __ldg(a.row_starts + s + 1);
+  const int id = __ldg(a.adapters + s);
   const bool bad = begin < 0 || end < begin || end > a.rows ||
                    (s == 0 && begin != 0) || (s == a.requests - 1 && end != a.rows);
-  int id = __ldg(a.adapters + s);
   if ((bad || id < -1 || id >= a.count) && (threadIdx.x & 31) == 0) atomicOr(a.err_word, kErrBadRoute);
   if (begin < 0 || end > a.rows) return t;
   t.row = begin + (g - (begin / M + s)) * M;
@@ -49,6 +60,10 @@ __device__ __forceinline__ Tile find_tile(const LoraArgs& a, int64_t g) {
   t.rows = static_cast<int>(min(static_cast<int64_t>(M), end - t.row));
   t.adapter = id >= 0 && id < a.count ? id : -1;
   return t;
+}
+
+__device__ __forceinline__ float adapter_scale(const LoraArgs& a, int adapter) {
+  return a.scales != nullptr ? __ldg(a.scales + adapter) : 1.f;
 }
 
 __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
@@ -60,23 +75,66 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// u[slice][row][r] = x[row][k in slice] . A[r][k in slice] for up to 8 rows of
-// one request.  The adapter is the M operand (16 ranks), the rows the N
-// operand (8), so a few rows waste little and A is read once.  Lane (g, q) =
-// (lane / 4, lane % 4) reads 16 bytes, k = 8 q .. 8 q + 7 of each 32-column
-// step: the four words serve two k16 products, for both operands in the same
-// (permuted) order of k.
+// Cluster helpers: the K slices of a tile are the CTAs of a cluster.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
+                   : "memory");
+}
+// The float4 at `p` (this CTA's shared memory) in CTA `rank` of the cluster.
+__device__ __forceinline__ float4 peer_float4(const float* p, int rank) {
+  uint32_t addr;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(smem_u32(p)), "r"(rank));
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+
+// Joins the slices' partial tiles `part` (rows x pad floats, row-major, in the
+// shared memory of each CTA of the cluster): this CTA takes every slices-th
+// row, adds the slices in order, scales, rounds and writes u.
+__device__ __forceinline__ void join_slices(const LoraArgs& a, const Tile& t, const float* part,
+                                            int pad, float scale) {
+  if (a.slices > 1) cluster_sync(); else __syncthreads();
+  const int per_row = a.rank_pad / 4;
+  const int mine = static_cast<int>(blockIdx.y);
+  for (int i = threadIdx.x; ; i += blockDim.x) {
+    const int row = mine + i / per_row * a.slices, c = i % per_row * 4;
+    if (row >= t.rows) break;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (c < pad) {
+      for (int s = 0; s < a.slices; ++s) {
+        const float* at = part + row * pad + c;
+        const float4 p = a.slices > 1 ? peer_float4(at, s) : *reinterpret_cast<const float4*>(at);
+        v.x += p.x; v.y += p.y; v.z += p.z; v.w += p.w;
+      }
+    }
+    *reinterpret_cast<uint2*>(a.workspace + (t.row + row) * a.rank_pad + c) =
+        make_uint2(pack_bf16x2(v.x * scale, v.y * scale), pack_bf16x2(v.z * scale, v.w * scale));
+  }
+  __syncwarp();
+  if (a.slices > 1) cluster_sync();   // peers may still read this CTA's tile
+}
+
+// Shrink for requests of few rows: up to 8 rows of one request.  The adapter
+// is the M operand (16 ranks), the rows the N operand (8), so a few rows waste
+// little and A is read once.  Lane (g, q) = (lane / 4, lane % 4) reads 16
+// bytes, k = 8 q .. 8 q + 7 of each 32-column step: the four words serve two
+// k16 products, for both operands in the same (permuted) order of k.
 template <int RG>
-__global__ void __launch_bounds__(kWarps * 32) lora_shrink_kernel(const LoraArgs a) {
-  __shared__ float part[kWarps][RG * 16][kShrinkRows];
-  const Tile t = find_tile<kShrinkRows>(a, blockIdx.x);
-  if (t.rows == 0 || t.adapter < 0) return;      // uniform over the block
+__global__ void __launch_bounds__(kWarps * 32) lora_shrink_few_kernel(const LoraArgs a) {
+  constexpr int kPad = RG * 16;
+  __shared__ __align__(16) float part[kWarps][kFewRows][kPad];
+  pdl_launch_dependents();
+  const Tile t = find_tile<kFewRows>(a, blockIdx.x);
+  if (t.rows == 0 || t.adapter < 0) return;      // uniform over the cluster
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, q = lane & 3;
-  const int slice = blockIdx.y;
   const int steps = (a.k + 31) / 32;
-  const int s0 = static_cast<int>(static_cast<int64_t>(steps) * slice / a.slices);
-  const int s1 = static_cast<int>(static_cast<int64_t>(steps) * (slice + 1) / a.slices);
+  const int s0 = static_cast<int>(static_cast<int64_t>(steps) * blockIdx.y / a.slices);
+  const int s1 = static_cast<int>(static_cast<int64_t>(steps) * (blockIdx.y + 1) / a.slices);
   const __nv_bfloat16* la = a.lora_a + static_cast<int64_t>(t.adapter) * a.rank * a.k;
   const __nv_bfloat16* x = a.x + (t.row + (g < t.rows ? g : 0)) * a.x_stride;
   const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
@@ -103,142 +161,353 @@ __global__ void __launch_bounds__(kWarps * 32) lora_shrink_kernel(const LoraArgs
   }
 #pragma unroll
   for (int m = 0; m < RG; ++m) {
-    part[warp][m * 16 + g][2 * q] = d[m][0];
-    part[warp][m * 16 + g][2 * q + 1] = d[m][1];
-    part[warp][m * 16 + g + 8][2 * q] = d[m][2];
-    part[warp][m * 16 + g + 8][2 * q + 1] = d[m][3];
+    part[warp][2 * q][m * 16 + g] = d[m][0];
+    part[warp][2 * q + 1][m * 16 + g] = d[m][1];
+    part[warp][2 * q][m * 16 + g + 8] = d[m][2];
+    part[warp][2 * q + 1][m * 16 + g + 8] = d[m][3];
   }
   __syncthreads();
-  float* u = a.workspace + (static_cast<int64_t>(slice) * a.rows + t.row) * a.rank_pad;
-  for (int i = threadIdx.x; i < t.rows * a.rank_pad; i += kWarps * 32) {
-    const int row = i / a.rank_pad, r = i % a.rank_pad;
+  for (int i = threadIdx.x; i < kFewRows * kPad; i += kWarps * 32) {
     float sum = 0.f;
-    if (r < RG * 16)
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) sum += part[w][r][row];
-    u[i] = sum;
+    for (int w = 0; w < kWarps; ++w) sum += (&part[w][0][0])[i];
+    (&part[0][0][0])[i] = sum;
   }
+  join_slices(a, t, &part[0][0][0], kPad, adapter_scale(a, t.adapter));
 }
 
-// out = y + (scale * sum of u's slices) B^T: each warp owns 32 columns, holds
-// their B fragments in registers and goes down the tile's rows 16 at a time.
-// Product column n of n-tile j stands for column 8 (n / 2) + 2 j + n % 2 of
-// the 32, so that a thread's 4 x 2 results are 8 consecutive columns: y and
-// out move as 16-byte accesses without a detour through shared memory.  The
-// scaled u is rounded to bf16 (the tensor cores' operand; 2^-9 of the delta,
-// as large as the final rounding of a delta that stands alone).
-template <int KB>
-__global__ void __launch_bounds__(kWarps * 32) lora_expand_kernel(const LoraArgs a) {
-  const Tile t = find_tile<kExpandRows>(a, blockIdx.x);
+// Shrink on the tensor cores: 128 rows of one request (the box may reach into
+// the next request's rows; they fill rows of the tile that are not stored)
+// times the adapter's ranks as N, 64 of K a stage, both by TMA.
+//   warp 0   TMA producer     warp 1   TMEM owner and MMA issuer
+//   all      epilogue: a row a thread, float32 to shared memory, join_slices
+struct ShrinkBarriers {
+  uint64_t full[8];
+  uint64_t empty[8];
+  uint64_t done;
+  uint32_t tmem_base;
+  int abort;
+};
+constexpr int kShrinkThreads = 128;
+// Two CTAs an SM; also holds the 128 x 128 float32 partial tile.
+constexpr int kShrinkRing = 100 * 1024;
+constexpr int kShrinkSmem = kShrinkRing + 1024 + static_cast<int>(sizeof(ShrinkBarriers));
+
+__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, uint64_t* bar,
+                                            int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar,
+                                            int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar))
+      : "memory");
+}
+
+template <int kPad>
+__global__ void __launch_bounds__(kShrinkThreads)
+    lora_shrink_kernel(const __grid_constant__ CUtensorMap tm_x,
+                       const __grid_constant__ CUtensorMap tm_a, const LoraArgs a) {
+  constexpr int kXBytes = kTileRows * 128;
+  constexpr int kStage = kXBytes + kPad * 128;
+  constexpr int kStages = kShrinkRing / kStage < 8 ? kShrinkRing / kStage : 8;
+  constexpr int kCols = kPad < 32 ? 32 : kPad;
+  static_assert(kStages >= 3 && kTileRows * kPad * 4 <= kShrinkRing, "ring");
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  ShrinkBarriers* bar = reinterpret_cast<ShrinkBarriers*>(ring + kShrinkRing);
+  volatile int* abort_flag = &bar->abort;
+  pdl_launch_dependents();
+  const Tile t = find_tile<kTileRows>(a, blockIdx.x);
+  if (t.rows == 0 || t.adapter < 0) return;      // uniform over the cluster
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int steps = (a.k + 63) / 64;
+  const int s0 = static_cast<int>(static_cast<int64_t>(steps) * blockIdx.y / a.slices);
+  const int n = static_cast<int>(static_cast<int64_t>(steps) * (blockIdx.y + 1) / a.slices) - s0;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&bar->full[i], 1);
+      mbar_init(&bar->empty[i], 1);
+    }
+    mbar_init(&bar->done, 1);
+    bar->abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) tmem_alloc(&bar->tmem_base, kCols);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bar->tmem_base;
+  if (warp == 0) {
+    if (lane == 0) {
+      bool ok = true;
+      int i = 0;
+      for (; i < n; ++i) {
+        const int s = i % kStages;
+        ok = mbar_wait(&bar->empty[s], ((i / kStages) & 1) ^ 1, abort_flag, a.err_word);
+        if (!ok) break;
+        uint8_t* dst = ring + s * kStage;
+        mbar_arrive_expect_tx(&bar->full[s], kStage);
+        tma_load_2d(dst, &tm_x, &bar->full[s], (s0 + i) * 64, static_cast<int>(t.row));
+        tma_load_3d(dst + kXBytes, &tm_a, &bar->full[s], (s0 + i) * 64, 0, t.adapter);
+      }
+      // Never leave a copy in flight into shared memory.
+      int never = 0;
+      for (int j = i > kStages ? i - kStages : 0; j < i; ++j)
+        mbar_wait(&bar->full[j % kStages], (j / kStages) & 1, &never, a.err_word);
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint32_t idesc = idesc_bf16_f32(128, kPad, false);
+      const uint64_t x0 = sdesc_sw128(smem_u32(ring), 16, 1024);
+      for (int i = 0; i < n; ++i) {
+        const int s = i % kStages;
+        if (!mbar_wait(&bar->full[s], (i / kStages) & 1, abort_flag, a.err_word)) break;
+        tc_fence_after();
+        const uint64_t xd = x0 + static_cast<uint64_t>((s * kStage) >> 4);
+        const uint64_t ad = xd + static_cast<uint64_t>(kXBytes >> 4);
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+          umma_bf16_ss(tmem, xd + kk * 2, ad + kk * 2, idesc, (i > 0 || kk > 0) ? 1u : 0u);
+        umma_commit(&bar->empty[s]);
+      }
+      int never = 0;
+      umma_commit(&bar->done);
+      mbar_wait(&bar->done, 0, &never, a.err_word);
+    }
+  }
+  __syncthreads();
+  // A timed-out wait leaves wrong sums behind, reported in the error word; the
+  // cluster still meets at its barriers below.
+  tc_fence_after();
+  float* part = reinterpret_cast<float*>(ring);
+  const int row = threadIdx.x;
+#pragma unroll 1
+  for (int c = 0; c < kCols; c += 32) {
+    uint32_t v[32];
+    tmem_ld_32x32b_x32(tmem + (static_cast<uint32_t>(warp * 32) << 16) + c, v);
+    tmem_wait_ld();
+    reg_fence<32>(v);
+#pragma unroll
+    for (int e = 0; e < 32; e += 4)
+      if (c + e < kPad)
+        *reinterpret_cast<uint4*>(part + row * kPad + c + e) =
+            make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kCols);
+  }
+  join_slices(a, t, part, kPad, adapter_scale(a, t.adapter));
+}
+
+// out = y + u B^T: each warp owns 32 columns at a time, holds their B
+// fragments in registers and goes down the tile's rows 16 at a time.  Product
+// column n of n-tile j stands for column 8 (n / 2) + 2 j + n % 2 of the 32, so
+// that a thread's 4 x 2 results are 8 consecutive columns: y and out move as
+// 16-byte accesses without a detour through shared memory, and u's rows are
+// the A fragments as they lie (k permuted as in lora_shrink_few_kernel).
+// kAhead row tiles of y are requested before the first product.
+template <int KB, int kAhead>
+__global__ void __launch_bounds__(kWarps * 32, 2) lora_expand_kernel(const LoraArgs a) {
+  constexpr int kTiles = kExpandRows / 16;
+  const int64_t slot = blockIdx.x / a.col_ctas;
+  const Tile t = find_tile<kExpandRows>(a, slot);
   if (t.rows == 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, q = lane & 3;
-  const int c0 = blockIdx.y * kExpandCols + warp * 32;
-  if (c0 >= a.n) return;
-  const int col = c0 + 8 * q;                    // this thread's 8 columns
   const bool has = t.adapter >= 0;
   const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-  uint4 b[KB][4];
-  if (has) {
-    const __nv_bfloat16* lb = a.lora_b + static_cast<int64_t>(t.adapter) * a.n * a.rank;
+  const __nv_bfloat16* lb = a.lora_b + (has ? static_cast<int64_t>(t.adapter) * a.n * a.rank : 0);
+  bool waited = false;
+  for (int c0 = static_cast<int>(blockIdx.x % a.col_ctas) * kExpandCols + warp * 32; c0 < a.n;
+       c0 += a.col_ctas * kExpandCols) {
+    const int col = c0 + 8 * q;                  // this thread's 8 columns
+    const bool col_in = col < a.n;
+    auto load_y = [&](int tile, int half) {
+      const int row = tile * 16 + g + 8 * half;
+      return row < t.rows && col_in
+          ? *reinterpret_cast<const uint4*>(a.y + (t.row + row) * a.y_stride + col) : zero;
+    };
+    uint4 y[kAhead][2];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) y[i][0] = load_y(i, 0), y[i][1] = load_y(i, 1);
+    uint4 b[KB][4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int c = c0 + 8 * (g >> 1) + 2 * j + (g & 1);
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) {
         const int k = kb * 32 + q * 8;
-        b[kb][j] = c < a.n && k < a.rank
+        b[kb][j] = has && c < a.n && k < a.rank
             ? __ldg(reinterpret_cast<const uint4*>(lb + static_cast<int64_t>(c) * a.rank + k)) : zero;
       }
     }
-  }
-  const float scale = has ? (a.scales != nullptr ? __ldg(a.scales + t.adapter) : 1.f) : 0.f;
-  for (int r0 = 0; r0 < t.rows; r0 += 16) {
-    float d[4][4];
+    if (!waited) {
+      pdl_wait();                                // u
+      waited = true;
+    }
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int tile = 0; tile < kTiles; ++tile) {
+      if (tile * 16 >= t.rows) break;
+      float d[4][4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) d[j][e] = 0.f;
-    if (has) {
+      for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {
-        const int k = kb * 32 + q * 8;
-        uint32_t w[2][4];
+        for (int e = 0; e < 4; ++e) d[j][e] = 0.f;
+      if (has) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int row = r0 + g + 8 * half;
-          float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-          if (row < t.rows && k < a.rank) {
-            const float* u = a.workspace + (t.row + row) * a.rank_pad + k;
-            for (int s = 0; s < a.slices; ++s) {
-              const float4 p0 = __ldg(reinterpret_cast<const float4*>(u));
-              const float4 p1 = __ldg(reinterpret_cast<const float4*>(u) + 1);
-              v[0] += p0.x; v[1] += p0.y; v[2] += p0.z; v[3] += p0.w;
-              v[4] += p1.x; v[5] += p1.y; v[6] += p1.z; v[7] += p1.w;
-              u += a.rows * a.rank_pad;
-            }
+        for (int kb = 0; kb < KB; ++kb) {
+          uint4 w[2];
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const int row = tile * 16 + g + 8 * half;
+            w[half] = row < t.rows
+                ? *reinterpret_cast<const uint4*>(a.workspace + (t.row + row) * a.rank_pad + kb * 32 + q * 8)
+                : zero;
           }
 #pragma unroll
-          for (int e = 0; e < 4; ++e) w[half][e] = pack_bf16x2(v[2 * e] * scale, v[2 * e + 1] * scale);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          mma_bf16(d[j], w[0][0], w[1][0], w[0][1], w[1][1], b[kb][j].x, b[kb][j].y);
-          mma_bf16(d[j], w[0][2], w[1][2], w[0][3], w[1][3], b[kb][j].z, b[kb][j].w);
+          for (int j = 0; j < 4; ++j) {
+            mma_bf16(d[j], w[0].x, w[1].x, w[0].y, w[1].y, b[kb][j].x, b[kb][j].y);
+            mma_bf16(d[j], w[0].z, w[1].z, w[0].w, w[1].w, b[kb][j].z, b[kb][j].w);
+          }
         }
       }
-    }
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int row = r0 + g + 8 * half;
-      if (row < t.rows && col < a.n) {
-        const uint4 in = *reinterpret_cast<const uint4*>(a.y + (t.row + row) * a.y_stride + col);
-        uint32_t w[4] = {in.x, in.y, in.z, in.w};
-        if (has) {
+      for (int half = 0; half < 2; ++half) {
+        const int row = tile * 16 + g + 8 * half;
+        const uint4 in = y[tile % kAhead][half];
+        if (tile + kAhead < kTiles) y[tile % kAhead][half] = load_y(tile + kAhead, half);
+        if (row < t.rows && col_in) {
+          uint32_t w[4] = {in.x, in.y, in.z, in.w};
+          if (has) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            w[j] = pack_bf16x2(__uint_as_float(w[j] << 16) + d[j][2 * half],
-                               __uint_as_float(w[j] & 0xffff0000u) + d[j][2 * half + 1]);
+            for (int j = 0; j < 4; ++j)
+              w[j] = pack_bf16x2(__uint_as_float(w[j] << 16) + d[j][2 * half],
+                                 __uint_as_float(w[j] & 0xffff0000u) + d[j][2 * half + 1]);
+          }
+          *reinterpret_cast<uint4*>(a.out + (t.row + row) * a.out_stride + col) =
+              make_uint4(w[0], w[1], w[2], w[3]);
         }
-        *reinterpret_cast<uint4*>(a.out + (t.row + row) * a.out_stride + col) =
-            make_uint4(w[0], w[1], w[2], w[3]);
       }
     }
   }
+}
+
+// Launch with a cluster of (1, slices, 1) CTAs.
+template <typename... Params, typename... Args>
+cudaError_t launch_sliced(void (*kernel)(Params...), dim3 grid, int threads, int smem, int slices,
+                          cudaStream_t stream, Args... args) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = grid;
+  config.blockDim = dim3(static_cast<unsigned>(threads));
+  config.dynamicSmemBytes = static_cast<size_t>(smem);
+  config.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 1;
+  attr[0].val.clusterDim.y = static_cast<unsigned>(slices);
+  attr[0].val.clusterDim.z = 1;
+  config.attrs = attr;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, kernel, args...);
+}
+
+// Launch whose blocks may start while the previous kernel of the stream still
+// runs (griddepcontrol).
+template <typename... Params, typename... Args>
+cudaError_t launch_dependent(void (*kernel)(Params...), dim3 grid, int threads, cudaStream_t stream,
+                             Args... args) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = grid;
+  config.blockDim = dim3(static_cast<unsigned>(threads));
+  config.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attr;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, kernel, args...);
+}
+
+template <int kPad>
+cudaError_t launch_shrink(const CUtensorMap& tx, const CUtensorMap& ta, const LoraArgs& a, dim3 grid,
+                          cudaStream_t stream) {
+  static std::atomic<bool> ready[64] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64 || !ready[dev].load(std::memory_order_acquire)) {
+    e = cudaFuncSetAttribute(lora_shrink_kernel<kPad>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             kShrinkSmem);
+    if (e != cudaSuccess) return e;
+    if (dev >= 0 && dev < 64) ready[dev].store(true, std::memory_order_release);
+  }
+  return launch_sliced(lora_shrink_kernel<kPad>, grid, kShrinkThreads, kShrinkSmem, a.slices, stream,
+                       tx, ta, a);
 }
 
 }  // namespace
 
-// Slices of K: enough CTAs for two waves of eight a SM, at least 512 of K each.
+// The tensor-core shrink takes requests of more than 16 rows on average; fewer
+// rows would leave most of its 128-row tiles empty and go 8 to a tile.  Slices
+// of K: two CTAs an SM (eight of the small ones), at least 4 steps of 64 each.
 LoraPlan lora_plan(int64_t rows, int32_t requests, int32_t k, int32_t rank, int num_sms) {
   LoraPlan p{};
-  p.rank_pad = (rank + 15) / 16 * 16;
-  const int64_t slots = rows / kShrinkRows + requests;
-  int64_t slices = (static_cast<int64_t>(num_sms) * 8 + slots - 1) / slots;
-  const int64_t most = (k + 511) / 512;
-  p.slices = static_cast<int32_t>(slices < 1 ? 1 : slices > most ? most : slices);
-  p.workspace_bytes = rows * p.rank_pad * p.slices * 4;
+  p.rank_pad = (rank + 31) / 32 * 32;
+  p.few_rows = rows <= 16ll * requests;
+  const int64_t slots = rows / (p.few_rows ? kFewRows : kTileRows) + requests;
+  const int64_t want = static_cast<int64_t>(num_sms) * (p.few_rows ? 8 : 2) / slots;
+  const int64_t most = std::min<int64_t>(kMaxSlices, (k + 255) / 256);
+  p.slices = static_cast<int32_t>(std::max<int64_t>(1, std::min(want, most)));
+  p.workspace_bytes = rows * p.rank_pad * 2;
   return p;
 }
 
-cudaError_t launch_lora_add(const LoraArgs& a, cudaStream_t stream) {
+cudaError_t launch_lora_add(const CUtensorMap& tx, const CUtensorMap& ta, LoraArgs a,
+                            cudaStream_t stream, int num_sms) {
   if (a.rows == 0 || a.n == 0) return cudaSuccess;
   const int groups = (a.rank + 15) / 16;
-  const dim3 sg(static_cast<unsigned>(a.rows / kShrinkRows + a.requests),
-                static_cast<unsigned>(a.slices));
-  if (groups <= 1) lora_shrink_kernel<1><<<sg, kWarps * 32, 0, stream>>>(a);
-  else if (groups <= 2) lora_shrink_kernel<2><<<sg, kWarps * 32, 0, stream>>>(a);
-  else if (groups <= 4) lora_shrink_kernel<4><<<sg, kWarps * 32, 0, stream>>>(a);
-  else lora_shrink_kernel<8><<<sg, kWarps * 32, 0, stream>>>(a);
-  cudaError_t e = cudaGetLastError();
+  const dim3 grid(static_cast<unsigned>(a.rows / (a.few_rows ? kFewRows : kTileRows) + a.requests),
+                  static_cast<unsigned>(a.slices));
+  cudaError_t e;
+  if (a.few_rows) {
+    const int threads = kWarps * 32;
+    if (groups <= 1) e = launch_sliced(lora_shrink_few_kernel<1>, grid, threads, 0, a.slices, stream, a);
+    else if (groups <= 2) e = launch_sliced(lora_shrink_few_kernel<2>, grid, threads, 0, a.slices, stream, a);
+    else if (groups <= 4) e = launch_sliced(lora_shrink_few_kernel<4>, grid, threads, 0, a.slices, stream, a);
+    else e = launch_sliced(lora_shrink_few_kernel<8>, grid, threads, 0, a.slices, stream, a);
+  } else {
+    if (groups <= 1) e = launch_shrink<16>(tx, ta, a, grid, stream);
+    else if (groups <= 2) e = launch_shrink<32>(tx, ta, a, grid, stream);
+    else if (groups <= 4) e = launch_shrink<64>(tx, ta, a, grid, stream);
+    else e = launch_shrink<128>(tx, ta, a, grid, stream);
+  }
   if (e != cudaSuccess) return e;
-  const dim3 eg(static_cast<unsigned>(a.rows / kExpandRows + a.requests),
-                static_cast<unsigned>((a.n + kExpandCols - 1) / kExpandCols));
-  const int kb = (a.rank + 31) / 32;
-  if (kb <= 1) lora_expand_kernel<1><<<eg, kWarps * 32, 0, stream>>>(a);
-  else if (kb <= 2) lora_expand_kernel<2><<<eg, kWarps * 32, 0, stream>>>(a);
-  else lora_expand_kernel<4><<<eg, kWarps * 32, 0, stream>>>(a);
-  return cudaGetLastError();
+  // Column CTAs a row tile: one for each 256 columns, fewer (each going over
+  // several) once that gives eight CTAs an SM.
+  const int64_t slots = a.rows / kExpandRows + a.requests;
+  const int64_t cols = (a.n + kExpandCols - 1) / kExpandCols;
+  a.col_ctas = static_cast<int32_t>(std::min<int64_t>(cols, (8ll * num_sms + slots - 1) / slots));
+  const dim3 eg(static_cast<unsigned>(slots * a.col_ctas));
+  const int kb = a.rank_pad / 32;
+  if (kb == 1) return launch_dependent(lora_expand_kernel<1, 4>, eg, kWarps * 32, stream, a);
+  if (kb == 2) return launch_dependent(lora_expand_kernel<2, 4>, eg, kWarps * 32, stream, a);
+  if (kb == 3) return launch_dependent(lora_expand_kernel<3, 2>, eg, kWarps * 32, stream, a);
+  return launch_dependent(lora_expand_kernel<4, 2>, eg, kWarps * 32, stream, a);
 }
+
+// Tensor maps of the tensor-core shrink: x [rows, k] in boxes of 64 x 128
+// rows, lora_a [count, rank, k] in boxes of 64 x padded ranks x 1.
+int lora_rank_box(int32_t rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : rank <= 64 ? 64 : 128; }
 
 }  // namespace bsa
