@@ -1012,23 +1012,35 @@ int bsa_lora_add(const void* y, int64_t y_stride, const void* x, int64_t x_strid
   a.few_rows = plan.few_rows;
   a.workspace = static_cast<__nv_bfloat16*>(workspace);
   a.err_word = err_word;
-  CUtensorMap tx{}, ta{};
-  if (!a.few_rows && count > 0) {
-    const cuuint64_t x_dims[2] = {static_cast<cuuint64_t>(k), static_cast<cuuint64_t>(rows)};
-    const cuuint64_t x_strides[1] = {static_cast<cuuint64_t>(x_stride) * 2};
-    const cuuint32_t x_box[2] = {64u, 128u};
-    int rc = encode_bf16(&tx, x, 2, x_dims, x_strides, x_box, "x");
-    if (rc != BSA_OK) return rc;
-    const cuuint64_t a_dims[3] = {static_cast<cuuint64_t>(k), static_cast<cuuint64_t>(rank),
+  bsa::LoraMaps maps{};
+  if (!a.few_rows) {
+    auto rows_map = [&](CUtensorMap* map, const void* p, int64_t cols, int64_t stride,
+                        const char* name) {
+      const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+      const cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride) * 2};
+      const cuuint32_t box[2] = {64u, 128u};
+      return encode_bf16(map, p, 2, dims, strides, box, name);
+    };
+    auto adapter_map = [&](CUtensorMap* map, const void* p, int64_t cols, int64_t height,
+                           int box_rows, const char* name) {
+      const cuuint64_t dims[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(height),
                                   static_cast<cuuint64_t>(count)};
-    const cuuint64_t a_strides[2] = {static_cast<cuuint64_t>(k) * 2,
-                                     static_cast<cuuint64_t>(k) * rank * 2};
-    const cuuint32_t a_box[3] = {64u, static_cast<cuuint32_t>(bsa::lora_rank_box(rank)), 1u};
-    rc = encode_bf16(&ta, lora_a, 3, a_dims, a_strides, a_box, "lora_a");
+      const cuuint64_t strides[2] = {static_cast<cuuint64_t>(cols) * 2,
+                                     static_cast<cuuint64_t>(cols) * height * 2};
+      const cuuint32_t box[3] = {64u, static_cast<cuuint32_t>(box_rows), 1u};
+      return encode_bf16(map, p, 3, dims, strides, box, name);
+    };
+    int rc = rows_map(&maps.x, x, k, x_stride, "x");
+    if (rc == BSA_OK) rc = rows_map(&maps.y, y, n, y_stride, "y");
+    if (rc == BSA_OK) rc = rows_map(&maps.out, out, n, out_stride, "out");
+    if (rc == BSA_OK) rc = rows_map(&maps.u, workspace, plan.rank_pad, plan.rank_pad, "workspace");
+    if (rc == BSA_OK && count > 0)
+      rc = adapter_map(&maps.a, lora_a, k, rank, bsa::lora_rank_box(rank), "lora_a");
+    if (rc == BSA_OK && count > 0) rc = adapter_map(&maps.b, lora_b, rank, n, 128, "lora_b");
     if (rc != BSA_OK) return rc;
   }
   const cudaError_t e =
-      bsa::launch_lora_add(tx, ta, a, static_cast<cudaStream_t>(stream), sm_count());
+      bsa::launch_lora_add(maps, a, static_cast<cudaStream_t>(stream), sm_count());
   if (e != cudaSuccess) return cuda_fail(e, "bsa_lora_add launch");
   return ok();
 }

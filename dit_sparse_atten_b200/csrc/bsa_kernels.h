@@ -255,10 +255,13 @@ struct LoraArgs {
   __nv_bfloat16* workspace;     // [rows, rank_pad]
   int* err_word;
 };
-// tm_x: [rows, k] in boxes of 64 columns x 128 rows; tm_a: lora_a in boxes of
-// 64 columns x lora_rank_box ranks x 1 adapter (both unused with few_rows).
-cudaError_t launch_lora_add(const CUtensorMap& tm_x, const CUtensorMap& tm_a, LoraArgs args,
-                            cudaStream_t stream, int num_sms);
+// Tensor maps (unused with few_rows), boxes of 64 columns x 128 rows but for
+// a's lora_rank_box ranks: x [rows, k], a [count, rank, k], y and out [rows, n],
+// b [count, n, rank], u [rows, rank_pad] (the workspace).
+struct LoraMaps {
+  CUtensorMap x, a, y, out, b, u;
+};
+cudaError_t launch_lora_add(const LoraMaps& maps, LoraArgs args, cudaStream_t stream, int num_sms);
 
 // Attention over packed sequences (packed_attention.cu).
 struct PackedArgs {

@@ -403,6 +403,291 @@ __global__ void __launch_bounds__(kWarps * 32, 2) lora_expand_kernel(const LoraA
   }
 }
 
+// Expand on the tensor cores: resident CTAs take (128 rows x 128 columns)
+// tiles of out, columns first, and stream y through a ring of shared-memory
+// stages; D = u B^T goes through two TMEM buffers, and out is written over y's
+// stage and stored by TMA (a tile that ends inside 128 rows: by the threads,
+// since a box would reach into the next request).  Every copy is asynchronous,
+// so HBM stays busy while the small products and sums go on.
+//   warp 0     TMA producer: y and B of a tile; u when the row tile changes
+//   warp 1     TMEM owner and MMA issuer
+//   warps 2-5  y + D: a row a thread, 32 columns at a time
+template <int KP>   // 64-column panels of the rank
+struct ExpandLayout {
+  static constexpr int kYBytes = kTileRows * 256;
+  static constexpr int kBBytes = KP * 128 * 128;
+  static constexpr int kStage = kYBytes + kBBytes;
+  static constexpr int kStages = KP == 1 ? 4 : 3;
+  static constexpr int kUBytes = KP * kTileRows * 128;
+  static constexpr int kUBuffers = KP == 1 ? 2 : 1;
+  static constexpr int kUOff = kStages * kStage;
+  static constexpr int kBarOff = kUOff + kUBuffers * kUBytes;
+};
+struct ExpandBarriers {
+  uint64_t full[4], empty[4];
+  uint64_t u_full[2], u_empty[2];
+  uint64_t d_full[2], d_empty[2];
+  uint64_t drain;
+  uint32_t tmem_base;
+  int abort;
+};
+constexpr int kExpandThreads = 192;
+
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(c0), "r"(c1), "r"(smem_u32(src))
+               : "memory");
+}
+
+// Walks this CTA's run of tiles; each warp has its own copy.
+struct ExpandWalk {
+  int64_t slot;        // row tile of the next item
+  int col;             // its column tile
+  int64_t left;        // items left
+  int cols;            // column tiles a row tile
+  bool fresh = true;   // `slot` has not been looked up
+  Tile tile{0, 0, -1};
+  __device__ ExpandWalk(int64_t first, int64_t last, int cols_)
+      : slot(first / cols_), col(static_cast<int>(first % cols_)), left(last - first), cols(cols_) {}
+  // Column tile of the next item with rows, or -1; `changed`: another row tile.
+  __device__ __forceinline__ int next(const LoraArgs& a, bool& changed) {
+    changed = false;
+    while (left > 0) {
+      if (fresh) {
+        tile = find_tile<kTileRows>(a, slot);
+        fresh = false;
+        changed = true;
+      }
+      const int c = col;
+      const bool empty = tile.rows == 0;
+      const int step = empty ? cols - c : 1;
+      left -= step;
+      col += step;
+      if (col == cols) {
+        col = 0;
+        ++slot;
+        fresh = true;
+      }
+      if (!empty) return c;
+    }
+    return -1;
+  }
+};
+
+template <int KP>
+__global__ void __launch_bounds__(kExpandThreads, 1)
+    lora_expand_tiles_kernel(const __grid_constant__ CUtensorMap tm_y,
+                             const __grid_constant__ CUtensorMap tm_out,
+                             const __grid_constant__ CUtensorMap tm_b,
+                             const __grid_constant__ CUtensorMap tm_u, const LoraArgs a) {
+  using L = ExpandLayout<KP>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  ExpandBarriers* bar = reinterpret_cast<ExpandBarriers*>(smem + L::kBarOff);
+  volatile int* abort_flag = &bar->abort;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t slots = a.rows / kTileRows + a.requests;
+  const int cols = (a.n + 127) / 128;
+  ExpandWalk walk(slots * cols * blockIdx.x / gridDim.x, slots * cols * (blockIdx.x + 1) / gridDim.x,
+                  cols);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&bar->full[i], 1);
+      mbar_init(&bar->empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bar->u_full[i], 1);
+      mbar_init(&bar->u_empty[i], 1);
+      mbar_init(&bar->d_full[i], 1);
+      mbar_init(&bar->d_empty[i], 128);
+    }
+    mbar_init(&bar->drain, 1);
+    bar->abort = prior_timeout(a.err_word) ? 1 : 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  if (bar->abort) return;     // uniform
+  if (warp == 1) tmem_alloc(&bar->tmem_base, 256);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bar->tmem_base;
+  bool changed;
+  if (warp == 0) {
+    // -------------------------------------------------------------- producer
+    int i = 0, u = 0;           // tiles and row tiles (with an adapter) loaded
+    bool ok = true, waited = false;
+    for (int c; ok && (c = walk.next(a, changed)) >= 0; ++i) {
+      const bool has = walk.tile.adapter >= 0;
+      const int s = i % L::kStages;
+      uint8_t* dst = smem + s * L::kStage;
+      const int row = static_cast<int>(walk.tile.row);
+      if (lane == 0) {
+        ok = mbar_wait(&bar->empty[s], ((i / L::kStages) & 1) ^ 1, abort_flag, a.err_word);
+        if (ok) {
+          mbar_arrive_expect_tx(&bar->full[s], L::kYBytes + (has ? L::kBBytes : 0));
+          tma_load_2d(dst, &tm_y, &bar->full[s], c * 128, row);
+          tma_load_2d(dst + 16384, &tm_y, &bar->full[s], c * 128 + 64, row);
+          if (has)
+#pragma unroll
+            for (int p = 0; p < KP; ++p)
+              tma_load_3d(dst + L::kYBytes + p * 16384, &tm_b, &bar->full[s], p * 64, c * 128,
+                          walk.tile.adapter);
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      if (ok && changed && has) {
+        if (!waited) pdl_wait();               // u comes from the shrink
+        waited = true;
+        const int ub = u % L::kUBuffers;
+        if (lane == 0) {
+          ok = mbar_wait(&bar->u_empty[ub], ((u / L::kUBuffers) & 1) ^ 1, abort_flag, a.err_word);
+          if (ok) {
+            mbar_arrive_expect_tx(&bar->u_full[ub], L::kUBytes);
+#pragma unroll
+            for (int p = 0; p < KP; ++p)
+              tma_load_2d(smem + L::kUOff + ub * L::kUBytes + p * 16384, &tm_u, &bar->u_full[ub], p * 64, row);
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        if (ok) ++u;
+      }
+      if (!ok) ++i;
+    }
+    if (!waited) pdl_wait();    // never end before the shrink has
+    // Never leave a copy in flight into shared memory (loads whose stage was
+    // not armed have a completed phase of this parity, or run out).
+    if (lane == 0 && *abort_flag) {
+      int never = 0;
+      for (int j = i > L::kStages ? i - L::kStages : 0; j < i; ++j)
+        mbar_wait(&bar->full[j % L::kStages], (j / L::kStages) & 1, &never, a.err_word);
+      for (int j = u > L::kUBuffers ? u - L::kUBuffers : 0; j < u; ++j)
+        mbar_wait(&bar->u_full[j % L::kUBuffers], (j / L::kUBuffers) & 1, &never, a.err_word);
+    }
+  } else if (warp == 1) {
+    // -------------------------------------------------------------- MMA issuer
+    const uint32_t idesc = idesc_bf16_f32(128, 128, false);
+    const int ksteps = (a.rank + 15) / 16;
+    int i = 0, d = 0, u = 0;
+    bool ok = true, open = false;              // open: a row tile's u is in use
+    for (int c; ok && (c = walk.next(a, changed)) >= 0; ++i) {
+      const bool has = walk.tile.adapter >= 0;
+      if (lane == 0) {
+        if (changed && open) umma_commit(&bar->u_empty[(u - 1) % L::kUBuffers]);
+        if (has) {
+          const int s = i % L::kStages, db = d & 1;
+          if (changed) {
+            ok = mbar_wait(&bar->u_full[u % L::kUBuffers], (u / L::kUBuffers) & 1, abort_flag, a.err_word);
+            ++u;
+          }
+          const int ub = (u - 1) % L::kUBuffers;
+          if (ok) ok = mbar_wait(&bar->full[s], (i / L::kStages) & 1, abort_flag, a.err_word);
+          if (ok) ok = mbar_wait(&bar->d_empty[db], ((d >> 1) & 1) ^ 1, abort_flag, a.err_word);
+          if (ok) {
+            tc_fence_after();
+            const uint64_t ud = sdesc_sw128(smem_u32(smem + L::kUOff + ub * L::kUBytes), 16, 1024);
+            const uint64_t bd = sdesc_sw128(smem_u32(smem + s * L::kStage + L::kYBytes), 16, 1024);
+            for (int kk = 0; kk < ksteps; ++kk) {
+              const uint64_t off = static_cast<uint64_t>(((kk >> 2) * 16384 + (kk & 3) * 32) >> 4);
+              umma_bf16_ss(tmem + db * 128, ud + off, bd + off, idesc, kk > 0 ? 1u : 0u);
+            }
+            umma_commit(&bar->d_full[db]);
+            ++d;
+          }
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      if (changed) open = has;
+    }
+    if (lane == 0) {
+      int never = 0;
+      umma_commit(&bar->drain);
+      mbar_wait(&bar->drain, 0, &never, a.err_word);
+    }
+  } else {
+    // -------------------------------------------------------------- epilogue
+    const int wq = warp & 3;                   // TMEM lanes 32 wq ..
+    const int row = wq * 32 + lane;
+    const uint32_t lane_addr = static_cast<uint32_t>(wq * 32) << 16;
+    const bool leader = warp == 2 && lane == 0;
+    int i = 0, d = 0, pending = -1;            // pending: stage that a store still reads
+    bool ok = true;
+    for (int c; (c = walk.next(a, changed)) >= 0; ++i) {
+      const bool has = walk.tile.adapter >= 0;
+      const int s = i % L::kStages, db = d & 1;
+      ok = mbar_wait(&bar->full[s], (i / L::kStages) & 1, abort_flag, a.err_word);
+      if (ok && has) ok = mbar_wait(&bar->d_full[db], (d >> 1) & 1, abort_flag, a.err_word);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      uint8_t* y = smem + s * L::kStage;
+      const bool whole = walk.tile.rows == kTileRows;
+      __nv_bfloat16* out = a.out + (walk.tile.row + row) * a.out_stride + c * 128;
+#pragma unroll
+      for (int cc = 0; cc < 4; ++cc) {
+        uint32_t v[32];
+        if (has) {
+          tmem_ld_32x32b_x32(tmem + lane_addr + db * 128 + cc * 32, v);
+          tmem_wait_ld();
+          reg_fence<32>(v);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] = 0u;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint4* at = reinterpret_cast<uint4*>(y + (cc >> 1) * 16384 + sw128_offset(row, (cc & 1) * 4 + j));
+          const uint4 in = *at;
+          uint32_t w[4] = {in.x, in.y, in.z, in.w};
+          if (has) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              w[e] = pack_bf16x2(__uint_as_float(w[e] << 16) + __uint_as_float(v[8 * j + 2 * e]),
+                                 __uint_as_float(w[e] & 0xffff0000u) + __uint_as_float(v[8 * j + 2 * e + 1]));
+          }
+          const uint4 res = make_uint4(w[0], w[1], w[2], w[3]);
+          if (whole)
+            *at = res;
+          else if (row < walk.tile.rows && c * 128 + cc * 32 + j * 8 < a.n)
+            *reinterpret_cast<uint4*>(out + cc * 32 + j * 8) = res;
+        }
+      }
+      if (has) {
+        tc_fence_before();
+        mbar_arrive(&bar->d_empty[db]);
+        ++d;
+      }
+      if (whole) fence_proxy_async_smem();
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      if (leader) {
+        if (whole) {
+          tma_store_2d(&tm_out, y, c * 128, static_cast<int>(walk.tile.row));
+          if (c * 128 + 64 < a.n)
+            tma_store_2d(&tm_out, y + 16384, c * 128 + 64, static_cast<int>(walk.tile.row));
+          asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+          if (pending >= 0) mbar_arrive(&bar->empty[pending]);
+          pending = s;
+        } else {
+          asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+          if (pending >= 0) mbar_arrive(&bar->empty[pending]);
+          mbar_arrive(&bar->empty[s]);
+          pending = -1;
+        }
+      }
+    }
+    if (leader) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 256);
+  }
+}
+
 // Launch with a cluster of (1, slices, 1) CTAs.
 template <typename... Params, typename... Args>
 cudaError_t launch_sliced(void (*kernel)(Params...), dim3 grid, int threads, int smem, int slices,
@@ -425,11 +710,12 @@ cudaError_t launch_sliced(void (*kernel)(Params...), dim3 grid, int threads, int
 // Launch whose blocks may start while the previous kernel of the stream still
 // runs (griddepcontrol).
 template <typename... Params, typename... Args>
-cudaError_t launch_dependent(void (*kernel)(Params...), dim3 grid, int threads, cudaStream_t stream,
-                             Args... args) {
+cudaError_t launch_dependent(void (*kernel)(Params...), dim3 grid, int threads, int smem,
+                             cudaStream_t stream, Args... args) {
   cudaLaunchConfig_t config = {};
   config.gridDim = grid;
   config.blockDim = dim3(static_cast<unsigned>(threads));
+  config.dynamicSmemBytes = static_cast<size_t>(smem);
   config.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -439,21 +725,38 @@ cudaError_t launch_dependent(void (*kernel)(Params...), dim3 grid, int threads, 
   return cudaLaunchKernelEx(&config, kernel, args...);
 }
 
+// Raises a kernel's dynamic shared memory limit, once a device.
+template <typename Kernel>
+cudaError_t allow_smem(Kernel kernel, int bytes, std::atomic<bool> (&ready)[64]) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev >= 0 && dev < 64 && ready[dev].load(std::memory_order_acquire)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev >= 0 && dev < 64) ready[dev].store(true, std::memory_order_release);
+  return e;
+}
+
 template <int kPad>
 cudaError_t launch_shrink(const CUtensorMap& tx, const CUtensorMap& ta, const LoraArgs& a, dim3 grid,
                           cudaStream_t stream) {
   static std::atomic<bool> ready[64] = {};
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
+  const cudaError_t e = allow_smem(lora_shrink_kernel<kPad>, kShrinkSmem, ready);
   if (e != cudaSuccess) return e;
-  if (dev < 0 || dev >= 64 || !ready[dev].load(std::memory_order_acquire)) {
-    e = cudaFuncSetAttribute(lora_shrink_kernel<kPad>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             kShrinkSmem);
-    if (e != cudaSuccess) return e;
-    if (dev >= 0 && dev < 64) ready[dev].store(true, std::memory_order_release);
-  }
   return launch_sliced(lora_shrink_kernel<kPad>, grid, kShrinkThreads, kShrinkSmem, a.slices, stream,
                        tx, ta, a);
+}
+
+template <int KP>
+cudaError_t launch_tiles(const LoraMaps& m, const LoraArgs& a, cudaStream_t stream, int num_sms) {
+  static std::atomic<bool> ready[64] = {};
+  const int smem = ExpandLayout<KP>::kBarOff + static_cast<int>(sizeof(ExpandBarriers)) + 1024;
+  const cudaError_t e = allow_smem(lora_expand_tiles_kernel<KP>, smem, ready);
+  if (e != cudaSuccess) return e;
+  const int64_t items = (a.rows / kTileRows + a.requests) * ((a.n + 127) / 128);
+  return launch_dependent(lora_expand_tiles_kernel<KP>,
+                          dim3(static_cast<unsigned>(std::min<int64_t>(items, num_sms))),
+                          kExpandThreads, smem, stream, m.y, m.out, m.b, m.u, a);
 }
 
 }  // namespace
@@ -473,8 +776,7 @@ LoraPlan lora_plan(int64_t rows, int32_t requests, int32_t k, int32_t rank, int 
   return p;
 }
 
-cudaError_t launch_lora_add(const CUtensorMap& tx, const CUtensorMap& ta, LoraArgs a,
-                            cudaStream_t stream, int num_sms) {
+cudaError_t launch_lora_add(const LoraMaps& maps, LoraArgs a, cudaStream_t stream, int num_sms) {
   if (a.rows == 0 || a.n == 0) return cudaSuccess;
   const int groups = (a.rank + 15) / 16;
   const dim3 grid(static_cast<unsigned>(a.rows / (a.few_rows ? kFewRows : kTileRows) + a.requests),
@@ -486,28 +788,29 @@ cudaError_t launch_lora_add(const CUtensorMap& tx, const CUtensorMap& ta, LoraAr
     else if (groups <= 2) e = launch_sliced(lora_shrink_few_kernel<2>, grid, threads, 0, a.slices, stream, a);
     else if (groups <= 4) e = launch_sliced(lora_shrink_few_kernel<4>, grid, threads, 0, a.slices, stream, a);
     else e = launch_sliced(lora_shrink_few_kernel<8>, grid, threads, 0, a.slices, stream, a);
-  } else {
-    if (groups <= 1) e = launch_shrink<16>(tx, ta, a, grid, stream);
-    else if (groups <= 2) e = launch_shrink<32>(tx, ta, a, grid, stream);
-    else if (groups <= 4) e = launch_shrink<64>(tx, ta, a, grid, stream);
-    else e = launch_shrink<128>(tx, ta, a, grid, stream);
+    if (e != cudaSuccess) return e;
+    // Column CTAs a row tile: one for each 256 columns, fewer (each going over
+    // several) once that gives eight CTAs an SM.
+    const int64_t slots = a.rows / kExpandRows + a.requests;
+    const int64_t cols = (a.n + kExpandCols - 1) / kExpandCols;
+    a.col_ctas = static_cast<int32_t>(std::min<int64_t>(cols, (8ll * num_sms + slots - 1) / slots));
+    const dim3 eg(static_cast<unsigned>(slots * a.col_ctas));
+    const int kb = a.rank_pad / 32;
+    if (kb == 1) return launch_dependent(lora_expand_kernel<1, 4>, eg, threads, 0, stream, a);
+    if (kb == 2) return launch_dependent(lora_expand_kernel<2, 4>, eg, threads, 0, stream, a);
+    if (kb == 3) return launch_dependent(lora_expand_kernel<3, 2>, eg, threads, 0, stream, a);
+    return launch_dependent(lora_expand_kernel<4, 2>, eg, threads, 0, stream, a);
   }
+  if (groups <= 1) e = launch_shrink<16>(maps.x, maps.a, a, grid, stream);
+  else if (groups <= 2) e = launch_shrink<32>(maps.x, maps.a, a, grid, stream);
+  else if (groups <= 4) e = launch_shrink<64>(maps.x, maps.a, a, grid, stream);
+  else e = launch_shrink<128>(maps.x, maps.a, a, grid, stream);
   if (e != cudaSuccess) return e;
-  // Column CTAs a row tile: one for each 256 columns, fewer (each going over
-  // several) once that gives eight CTAs an SM.
-  const int64_t slots = a.rows / kExpandRows + a.requests;
-  const int64_t cols = (a.n + kExpandCols - 1) / kExpandCols;
-  a.col_ctas = static_cast<int32_t>(std::min<int64_t>(cols, (8ll * num_sms + slots - 1) / slots));
-  const dim3 eg(static_cast<unsigned>(slots * a.col_ctas));
-  const int kb = a.rank_pad / 32;
-  if (kb == 1) return launch_dependent(lora_expand_kernel<1, 4>, eg, kWarps * 32, stream, a);
-  if (kb == 2) return launch_dependent(lora_expand_kernel<2, 4>, eg, kWarps * 32, stream, a);
-  if (kb == 3) return launch_dependent(lora_expand_kernel<3, 2>, eg, kWarps * 32, stream, a);
-  return launch_dependent(lora_expand_kernel<4, 2>, eg, kWarps * 32, stream, a);
+  return a.rank <= 64 ? launch_tiles<1>(maps, a, stream, num_sms)
+                      : launch_tiles<2>(maps, a, stream, num_sms);
 }
 
-// Tensor maps of the tensor-core shrink: x [rows, k] in boxes of 64 x 128
-// rows, lora_a [count, rank, k] in boxes of 64 x padded ranks x 1.
+// Ranks that a box of lora_a's tensor map covers.
 int lora_rank_box(int32_t rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : rank <= 64 ? 64 : 128; }
 
 }  // namespace bsa

@@ -69,6 +69,19 @@ def test_sizes(k, n):
     check(call(t), t)
 
 
+@pytest.mark.parametrize("rank", [16, 64, 72, 128])
+def test_many_tiles(rank):
+    """Several tiles a CTA, requests with and without adapters between them,
+    whole and partial row tiles, a last column tile of 8 columns."""
+    t = make([700, 0, 128, 1, 515, 256, 40, 384], 192, 2056, rank, 3, [0, 1, 2, -1, 1, -1, 0, 2],
+             seed=rank)
+    want = call(t)
+    check(want, t)
+    y = t["y"].clone()
+    assert torch.equal(call(dict(t, y=y), out=y), want)
+    assert all(torch.equal(call(t), want) for _ in range(5))
+
+
 def test_single_rows_and_many_requests():
     for s in (1, 31, 33, 200, 1030):
         t = make([1] * s, 256, 320, 16, 5, [(3 * i) % 6 - 1 for i in range(s)], seed=s)
