@@ -251,7 +251,7 @@ struct LoraArgs {
   int32_t requests, count, k, n, rank;
   int32_t rank_pad, slices;     // of lora_plan
   bool few_rows;
-  int32_t col_ctas;             // set by the launch
+  int32_t col_ctas, run;        // set by the launch
   __nv_bfloat16* workspace;     // [rows, rank_pad]
   int* err_word;
 };

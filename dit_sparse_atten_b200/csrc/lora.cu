@@ -92,11 +92,11 @@ __device__ __forceinline__ float4 peer_float4(const float* p, int rank) {
   return v;
 }
 
-// Joins the slices' partial tiles `part` (rows x pad floats, row-major, in the
-// shared memory of each CTA of the cluster): this CTA takes every slices-th
+// Joins the slices' partial tiles `part` (rows of pad floats, `stride` apart, in
+// the shared memory of each CTA of the cluster): this CTA takes every slices-th
 // row, adds the slices in order, scales, rounds and writes u.
 __device__ __forceinline__ void join_slices(const LoraArgs& a, const Tile& t, const float* part,
-                                            int pad, float scale) {
+                                            int pad, int stride, float scale) {
   if (a.slices > 1) cluster_sync(); else __syncthreads();
   const int per_row = a.rank_pad / 4;
   const int mine = static_cast<int>(blockIdx.y);
@@ -106,7 +106,7 @@ __device__ __forceinline__ void join_slices(const LoraArgs& a, const Tile& t, co
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     if (c < pad) {
       for (int s = 0; s < a.slices; ++s) {
-        const float* at = part + row * pad + c;
+        const float* at = part + row * stride + c;
         const float4 p = a.slices > 1 ? peer_float4(at, s) : *reinterpret_cast<const float4*>(at);
         v.x += p.x; v.y += p.y; v.z += p.z; v.w += p.w;
       }
@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(kWarps * 32) lora_shrink_few_kernel(const Lora
     for (int w = 0; w < kWarps; ++w) sum += (&part[w][0][0])[i];
     (&part[0][0][0])[i] = sum;
   }
-  join_slices(a, t, &part[0][0][0], kPad, adapter_scale(a, t.adapter));
+  join_slices(a, t, &part[0][0][0], kPad, kPad, adapter_scale(a, t.adapter));
 }
 
 // Shrink on the tensor cores: 128 rows of one request (the box may reach into
@@ -218,7 +218,8 @@ __global__ void __launch_bounds__(kShrinkThreads)
   constexpr int kStage = kXBytes + kPad * 128;
   constexpr int kStages = kShrinkRing / kStage < 8 ? kShrinkRing / kStage : 8;
   constexpr int kCols = kPad < 32 ? 32 : kPad;
-  static_assert(kStages >= 3 && kTileRows * kPad * 4 <= kShrinkRing, "ring");
+  constexpr int kPartStride = kPad + 4;   // a thread writes a row: 16 bytes off the bank period
+  static_assert(kStages >= 3 && kTileRows * kPartStride * 4 <= kShrinkRing, "ring");
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -298,7 +299,7 @@ __global__ void __launch_bounds__(kShrinkThreads)
 #pragma unroll
     for (int e = 0; e < 32; e += 4)
       if (c + e < kPad)
-        *reinterpret_cast<uint4*>(part + row * kPad + c + e) =
+        *reinterpret_cast<uint4*>(part + row * kPartStride + c + e) =
             make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
   }
   tc_fence_before();
@@ -307,7 +308,7 @@ __global__ void __launch_bounds__(kShrinkThreads)
     tc_fence_after();
     tmem_dealloc(tmem, kCols);
   }
-  join_slices(a, t, part, kPad, adapter_scale(a, t.adapter));
+  join_slices(a, t, part, kPad, kPartStride, adapter_scale(a, t.adapter));
 }
 
 // out = y + u B^T: each warp owns 32 columns at a time, holds their B
@@ -411,7 +412,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) lora_expand_kernel(const LoraA
 // so HBM stays busy while the small products and sums go on.
 //   warp 0     TMA producer: y and B of a tile; u when the row tile changes
 //   warp 1     TMEM owner and MMA issuer
-//   warps 2-5  y + D: a row a thread, 32 columns at a time
+//   warps 2-9  y + D: two groups of four warps take alternate tiles (and TMEM
+//              buffers), a row a thread, 32 columns at a time
 template <int KP>   // 64-column panels of the rank
 struct ExpandLayout {
   static constexpr int kYBytes = kTileRows * 256;
@@ -431,7 +433,7 @@ struct ExpandBarriers {
   uint32_t tmem_base;
   int abort;
 };
-constexpr int kExpandThreads = 192;
+constexpr int kExpandThreads = 320;
 
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int c0, int c1) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
@@ -440,36 +442,46 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void*
                : "memory");
 }
 
-// Walks this CTA's run of tiles; each warp has its own copy.
+// Walks this CTA's tiles; each warp has its own copy.  Items are runs of
+// `run` column tiles of one row tile; CTA b takes runs b, b + grid, ...
 struct ExpandWalk {
-  int64_t slot;        // row tile of the next item
-  int col;             // its column tile
-  int64_t left;        // items left
-  int cols;            // column tiles a row tile
+  int64_t slot;        // row tile of the run
+  int part;            // run within the row tile
+  int col, end;        // next column tile of the run, and its end
+  int cols, run, parts;
+  int step_slots, step_parts;
+  int64_t slots;
   bool fresh = true;   // `slot` has not been looked up
   Tile tile{0, 0, -1};
-  __device__ ExpandWalk(int64_t first, int64_t last, int cols_)
-      : slot(first / cols_), col(static_cast<int>(first % cols_)), left(last - first), cols(cols_) {}
+  __device__ ExpandWalk(int64_t slots_, int cols_, int run_)
+      : cols(cols_), run(run_), parts((cols_ + run_ - 1) / run_), slots(slots_) {
+    slot = blockIdx.x / parts;
+    part = static_cast<int>(blockIdx.x % parts);
+    step_slots = static_cast<int>(gridDim.x / parts);
+    step_parts = static_cast<int>(gridDim.x % parts);
+    col = part * run;
+    end = min(col + run, cols);
+  }
   // Column tile of the next item with rows, or -1; `changed`: another row tile.
   __device__ __forceinline__ int next(const LoraArgs& a, bool& changed) {
     changed = false;
-    while (left > 0) {
+    while (slot < slots) {
       if (fresh) {
         tile = find_tile<kTileRows>(a, slot);
         fresh = false;
         changed = true;
       }
-      const int c = col;
-      const bool empty = tile.rows == 0;
-      const int step = empty ? cols - c : 1;
-      left -= step;
-      col += step;
-      if (col == cols) {
-        col = 0;
+      if (tile.rows > 0 && col < end) return col++;
+      const int64_t before = slot;
+      slot += step_slots;
+      part += step_parts;
+      if (part >= parts) {
+        part -= parts;
         ++slot;
-        fresh = true;
       }
-      if (!empty) return c;
+      fresh = slot != before;
+      col = part * run;
+      end = min(col + run, cols);
     }
     return -1;
   }
@@ -490,8 +502,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t slots = a.rows / kTileRows + a.requests;
   const int cols = (a.n + 127) / 128;
-  ExpandWalk walk(slots * cols * blockIdx.x / gridDim.x, slots * cols * (blockIdx.x + 1) / gridDim.x,
-                  cols);
+  ExpandWalk walk(slots, cols, a.run);
   if (threadIdx.x == 0) {
     for (int i = 0; i < 4; ++i) {
       mbar_init(&bar->full[i], 1);
@@ -570,21 +581,22 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
     // -------------------------------------------------------------- MMA issuer
     const uint32_t idesc = idesc_bf16_f32(128, 128, false);
     const int ksteps = (a.rank + 15) / 16;
-    int i = 0, d = 0, u = 0;
+    int i = 0, u = 0, uses[2] = {0, 0};        // uses of each TMEM buffer
     bool ok = true, open = false;              // open: a row tile's u is in use
     for (int c; ok && (c = walk.next(a, changed)) >= 0; ++i) {
       const bool has = walk.tile.adapter >= 0;
       if (lane == 0) {
         if (changed && open) umma_commit(&bar->u_empty[(u - 1) % L::kUBuffers]);
         if (has) {
-          const int s = i % L::kStages, db = d & 1;
+          const int s = i % L::kStages, db = i & 1;
+          const int use = db ? uses[1]++ : uses[0]++;
           if (changed) {
             ok = mbar_wait(&bar->u_full[u % L::kUBuffers], (u / L::kUBuffers) & 1, abort_flag, a.err_word);
             ++u;
           }
           const int ub = (u - 1) % L::kUBuffers;
           if (ok) ok = mbar_wait(&bar->full[s], (i / L::kStages) & 1, abort_flag, a.err_word);
-          if (ok) ok = mbar_wait(&bar->d_empty[db], ((d >> 1) & 1) ^ 1, abort_flag, a.err_word);
+          if (ok) ok = mbar_wait(&bar->d_empty[db], (use & 1) ^ 1, abort_flag, a.err_word);
           if (ok) {
             tc_fence_after();
             const uint64_t ud = sdesc_sw128(smem_u32(smem + L::kUOff + ub * L::kUBytes), 16, 1024);
@@ -594,7 +606,6 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
               umma_bf16_ss(tmem + db * 128, ud + off, bd + off, idesc, kk > 0 ? 1u : 0u);
             }
             umma_commit(&bar->d_full[db]);
-            ++d;
           }
         }
       }
@@ -611,14 +622,16 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
     const int wq = warp & 3;                   // TMEM lanes 32 wq ..
     const int row = wq * 32 + lane;
     const uint32_t lane_addr = static_cast<uint32_t>(wq * 32) << 16;
-    const bool leader = warp == 2 && lane == 0;
-    int i = 0, d = 0, pending = -1;            // pending: stage that a store still reads
+    const int db = (warp - 2) >> 2;            // this group's TMEM buffer and tile parity
+    const bool leader = ((warp - 2) & 3) == 0 && lane == 0;
+    int i = 0, use = 0;
     bool ok = true;
     for (int c; (c = walk.next(a, changed)) >= 0; ++i) {
+      if ((i & 1) != db) continue;
       const bool has = walk.tile.adapter >= 0;
-      const int s = i % L::kStages, db = d & 1;
+      const int s = i % L::kStages;
       ok = mbar_wait(&bar->full[s], (i / L::kStages) & 1, abort_flag, a.err_word);
-      if (ok && has) ok = mbar_wait(&bar->d_full[db], (d >> 1) & 1, abort_flag, a.err_word);
+      if (ok && has) ok = mbar_wait(&bar->d_full[db], use & 1, abort_flag, a.err_word);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
@@ -657,25 +670,19 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
       if (has) {
         tc_fence_before();
         mbar_arrive(&bar->d_empty[db]);
-        ++d;
+        ++use;
       }
       if (whole) fence_proxy_async_smem();
-      asm volatile("bar.sync 1, 128;" ::: "memory");
+      asm volatile("bar.sync %0, 128;" ::"r"(1 + db) : "memory");
       if (leader) {
         if (whole) {
           tma_store_2d(&tm_out, y, c * 128, static_cast<int>(walk.tile.row));
           if (c * 128 + 64 < a.n)
             tma_store_2d(&tm_out, y + 16384, c * 128 + 64, static_cast<int>(walk.tile.row));
           asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-          asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-          if (pending >= 0) mbar_arrive(&bar->empty[pending]);
-          pending = s;
-        } else {
           asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-          if (pending >= 0) mbar_arrive(&bar->empty[pending]);
-          mbar_arrive(&bar->empty[s]);
-          pending = -1;
         }
+        mbar_arrive(&bar->empty[s]);
       }
     }
     if (leader) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
@@ -748,12 +755,17 @@ cudaError_t launch_shrink(const CUtensorMap& tx, const CUtensorMap& ta, const Lo
 }
 
 template <int KP>
-cudaError_t launch_tiles(const LoraMaps& m, const LoraArgs& a, cudaStream_t stream, int num_sms) {
+cudaError_t launch_tiles(const LoraMaps& m, LoraArgs a, cudaStream_t stream, int num_sms) {
+  // Two column tiles of a row tile in a row share its u; longer runs move a
+  // CTA's rows apart from its neighbours' in DRAM (57,600 x 5,120, rank 32:
+  // 235 us for runs of 1, 217 of 2, 233 of 4, 246 and more of whole rows).
+  a.run = 2;
   static std::atomic<bool> ready[64] = {};
   const int smem = ExpandLayout<KP>::kBarOff + static_cast<int>(sizeof(ExpandBarriers)) + 1024;
   const cudaError_t e = allow_smem(lora_expand_tiles_kernel<KP>, smem, ready);
   if (e != cudaSuccess) return e;
-  const int64_t items = (a.rows / kTileRows + a.requests) * ((a.n + 127) / 128);
+  const int64_t cols = (a.n + 127) / 128;
+  const int64_t items = (a.rows / kTileRows + a.requests) * ((cols + a.run - 1) / a.run);
   return launch_dependent(lora_expand_tiles_kernel<KP>,
                           dim3(static_cast<unsigned>(std::min<int64_t>(items, num_sms))),
                           kExpandThreads, smem, stream, m.y, m.out, m.b, m.u, a);
