@@ -1,58 +1,41 @@
-// Softmax attention over packed sequences of different lengths, grouped heads,
-// causal or full, for sm_100a:
-//   out[i, h] = sum_j softmax_j(scale * q[i, h] . k[j, h / G]) v[j, h / G]
-// over the keys j of query i's own request (causal: the first
-// i + 1 + k_len - q_len of them, i counted within the request), in float32
-// from bf16 inputs; a query that sees no key gives 0.
+// Attention over packed sequences where the query tiles alone leave SMs idle
+// (a few new tokens over long keys): the keys of a tile are split over CTAs and
+// joined.  The operator's definition and the larger form are in
+// packed_attention_tiles.cu.
 //
-// One CTA takes the 128 / G tokens x G heads of one key head as the 128 rows
-// of the MMA (row = token * G + head in group), so all query heads that share
-// a key head share its K and V loads, and a single new token still fills G
-// rows.  Tiles are found on the device: slot g belongs to request
-// s = #{i >= 1: floor(q_starts[i] / tokens) + i <= g} (packed_common.cuh).
-// Tiles late in their request see the most keys under the causal mask, so
-// slots run from the last to the first; a key head's tiles run next to each
-// other so that its K and V stay in L2.
+// One CTA takes one part of the key blocks of the 128 / G tokens x G heads of
+// one key head, as the 128 rows of the MMA (row = token * G + head in group):
+// all query heads that share a key head share its K and V loads, and a single
+// new token still fills G rows.  Bound: HBM, K and V read once.
 //   warp 8      TMA producer: K/V blocks of 128 keys into a ring of 32 KB
 //               slots (K0, K1, V0, K2, V1, ...)
 //   warp 9      TMEM owner; one thread loads Q and issues S_j = Q K_j^T
 //   warp 10     one thread issues O += P_j V_j (P from tensor memory)
-//   warp 11     V of the masked blocks (the last one or two): rows past the
-//               request's end are zeroed, since 0 * (whatever another request
-//               holds there, NaN included) would reach O
+//   warp 11     cleans V of the masked blocks (clean_masked_values)
 //   warps 0-7   softmax, two groups that take alternate key blocks, one row a
 //               thread, log2 domain, a stabiliser that moves only past 2^8
 // TMEM: three S (and P) buffers at [0, 384), O at [384, 512).
-//
-// A value of V that is not finite at a key which part of the tile must not see
-// (causal) cannot be kept out of those rows by P = 0; warp 11 looks for one
-// and, if there is, the tile's rows are computed again key by key in float32.
-//
 // Every mbarrier wait is bounded (bsa::mbar_wait); on a timeout the CTA sets
 // kErrWaitTimeout, drains its copies and MMAs, frees TMEM and exits.
+#include <algorithm>
 #include <atomic>
 
-#include "attention_softmax.cuh"
-#include "bsa_kernels.h"
-#include "packed_common.cuh"
+#include "packed_attention.cuh"
 
 namespace bsa {
 namespace {
 
 using namespace attn;
+using namespace packed;
 
 constexpr int kThreads = 384;
 constexpr int kProducerWarp = 8;
 constexpr int kMmaWarp = 9;
 constexpr int kPvWarp = 10;
 constexpr int kCheckWarp = 11;
-constexpr int kHeadDim = 128;
-constexpr int kBlock = 128;             // keys a block
 constexpr int kSBuffers = 3;
 constexpr uint32_t kTmemO = 384;
 constexpr int kSlots = 6;
-constexpr int kPanel = kBlock * 128;    // 64 columns x 128 rows, bf16
-constexpr int kSlotBytes = 2 * kPanel;
 constexpr int kQOff = 0;
 constexpr int kRingOff = kQOff + 128 * 256;
 constexpr int kXOff = kRingOff + kSlots * kSlotBytes;
@@ -74,98 +57,10 @@ struct Barriers {
 };
 constexpr int kUsed = kBarOff + static_cast<int>(sizeof(Barriers));
 
-__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar,
-                                            int c0, int c1, int c2) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar))
-      : "memory");
-}
-
-// What a CTA works on (uniform over the CTA).
-struct Work {
-  int64_t q0;          // first query row
-  int64_t k0;          // first key row of the request
-  int tokens;          // queries of the tile (0: nothing to do)
-  int first_limit;     // keys that the tile's first query sees, before clamping to [0, keys]
-  int keys;            // keys of the request
-  int block0, blocks;  // key blocks [block0, block0 + blocks)
-};
-
-// Query row `token` of the tile sees keys [0, limit).
-__device__ __forceinline__ int row_limit(const Work& w, int token, bool causal) {
-  if (token >= w.tokens) return 0;
-  return causal ? max(0, min(w.keys, w.first_limit + token)) : w.keys;
-}
-
-__device__ __forceinline__ Work find_work(const PackedArgs& a, int64_t slot, int split) {
-  Work w{};
-  const int tt = a.tile_tokens;
-  const int s = warp_count_le(a.requests, slot, [&](int i) {
-    return static_cast<int64_t>(__ldg(a.q_starts + i)) / tt + i;
-  });
-  if (s >= a.requests) return w;
-  const int64_t qb = __ldg(a.q_starts + s), qe = __ldg(a.q_starts + s + 1);
-  const int64_t kb = __ldg(a.k_starts + s), ke = __ldg(a.k_starts + s + 1);
-  const bool bad = qb < 0 || qe < qb || qe > a.q_rows || kb < 0 || ke < kb || ke > a.k_rows ||
-                   (s == 0 && qb != 0) || (s == a.requests - 1 && qe != a.q_rows);
-  if (bad && threadIdx.x == 0) atomicOr(a.err_word, kErrBadRoute);
-  if (qb < 0 || qe > a.q_rows || kb < 0 || ke < kb || ke > a.k_rows) return w;
-  w.q0 = qb + (slot - (qb / tt + s)) * tt;
-  if (w.q0 < qb || w.q0 >= qe) return w;
-  w.k0 = kb;
-  w.tokens = static_cast<int>(min(static_cast<int64_t>(tt), qe - w.q0));
-  w.keys = static_cast<int>(ke - kb);
-  // int: |q_rows|, |k_rows| < 2^31 - 256
-  w.first_limit = a.causal ? static_cast<int>(w.q0 - qb + 1 + (ke - kb) - (qe - qb)) : w.keys;
-  const int visible = row_limit(w, w.tokens - 1, a.causal);
-  const int n = (visible + kBlock - 1) / kBlock;
-  w.block0 = static_cast<int>(static_cast<int64_t>(n) * split / a.splits);
-  w.blocks = static_cast<int>(static_cast<int64_t>(n) * (split + 1) / a.splits) - w.block0;
-  return w;
-}
-
-// One query row key by key in float32 (a warp; lane owns 4 features): the way
-// out when V holds non-finite values at masked keys.  Returns the row's
-// stabiliser (log2 domain) and sum; o is relative to the stabiliser.
-__device__ __noinline__ float2 exact_row(const PackedArgs& a, const __nv_bfloat16* q,
-                                         int64_t k0, int head, int begin, int end, float c,
-                                         float4& o) {
-  const int lane = threadIdx.x & 31;
-  float qf[4], m = -INFINITY, l = 0.f;
-  o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-  for (int e = 0; e < 4; ++e) qf[e] = __bfloat162float(q[lane * 4 + e]);
-  for (int j = begin; j < end; ++j) {
-    const int64_t row = k0 + j;
-    const __nv_bfloat16* k = a.k + row * a.k_stride_t + head * a.k_stride_h + lane * 4;
-    const __nv_bfloat16* v = a.v + row * a.v_stride_t + head * a.v_stride_h + lane * 4;
-    float s = 0.f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) s = fmaf(qf[e], __bfloat162float(k[e]), s);
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-    s *= c;
-    const float m_new = fmaxf(m, s);
-    const float keep = m == -INFINITY ? 0.f : ex2_approx(m - m_new);
-    const float p = m_new == -INFINITY ? 0.f : ex2_approx(s - m_new);
-    l = l * keep + p;
-    o.x = fmaf(p, __bfloat162float(v[0]), m == -INFINITY ? 0.f : o.x * keep);
-    o.y = fmaf(p, __bfloat162float(v[1]), m == -INFINITY ? 0.f : o.y * keep);
-    o.z = fmaf(p, __bfloat162float(v[2]), m == -INFINITY ? 0.f : o.z * keep);
-    o.w = fmaf(p, __bfloat162float(v[3]), m == -INFINITY ? 0.f : o.w * keep);
-    m = m_new;
-  }
-  return make_float2(m, l);
-}
-
-// kSplit: this CTA takes one of a.splits parts of the tile's key blocks and
-// leaves O (relative to its stabiliser), the stabiliser and the sum in the
-// workspace for combine_kernel.
-template <bool kSplit>
+// Leaves O (relative to its stabiliser), the stabiliser and the sum of part
+// `split` in the workspace for combine_kernel.
 __global__ void __launch_bounds__(kThreads, 1)
-    packed_attention_kernel(const __grid_constant__ CUtensorMap tm_q,
+    packed_attention_split_kernel(const __grid_constant__ CUtensorMap tm_q,
                             const __grid_constant__ CUtensorMap tm_k,
                             const __grid_constant__ CUtensorMap tm_v, const PackedArgs a) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -181,13 +76,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int lane = threadIdx.x & 31;
   const int64_t slot = a.slots - 1 - blockIdx.x % a.slots;
   const int hk = static_cast<int>((blockIdx.x / a.slots) % a.kv_heads);
-  const int split = kSplit ? static_cast<int>(blockIdx.x / (a.slots * a.kv_heads)) : 0;
-  const Work w = find_work(a, slot, split);
+  const int split = static_cast<int>(blockIdx.x / (a.slots * a.kv_heads));
+  const Work w = find_work(a, slot, a.tile_tokens);
   if (w.tokens == 0) return;
   const int G = a.group;
-  const int n = w.blocks;
+  const int all = (row_limit(w, w.tokens - 1, a.causal) + kBlock - 1) / kBlock;
+  const int block0 = static_cast<int>(static_cast<int64_t>(all) * split / a.splits);
+  const int n = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / a.splits) - block0;
   // The first block of this CTA that some row of the tile does not see whole.
-  const int masked_from = max(0, min(n, max(0, row_limit(w, 0, a.causal)) / kBlock - w.block0));
+  const int masked_from = max(0, min(n, max(0, row_limit(w, 0, a.causal)) / kBlock - block0));
 
   if (threadIdx.x == 0) {
     uint32_t dyn_bytes;
@@ -245,7 +142,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           armed |= 1u << s;
           armed_phase = (armed_phase & ~(1u << s)) | (ph << s);
         }
-        const int row = static_cast<int>(w.k0 + static_cast<int64_t>(w.block0 + j) * kBlock);
+        const int row = static_cast<int>(w.k0 + static_cast<int64_t>(block0 + j) * kBlock);
         mbar_arrive_expect_tx(full, kSlotBytes);
         tma_load_3d(dst, tm, full, 0, hk, row);
         tma_load_3d(dst + kPanel, tm, full, 64, hk, row);
@@ -332,30 +229,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool ok = mbar_wait(&bar->masked_full[j - masked_from], 0, abort_flag, a.err_word);
       if (!__all_sync(0xffffffffu, ok)) break;
       const int s = seq_v(j) % kSlots;
-      uint8_t* tile = sRing + s * kSlotBytes;
-      const int key0 = (w.block0 + j) * kBlock;
-      const int real = min(kBlock, w.keys - key0);                    // rows of this request
-      const int open = max(0, row_limit(w, 0, a.causal) - key0);      // rows that every query sees
-      for (int i = lane + real * 8; i < kBlock * 8; i += 32) {
-        // a row is 8 chunks of 16 bytes in each panel; which of them is which
-        // (the swizzle) does not matter for zeroing or scanning a whole row
-        *reinterpret_cast<uint4*>(tile + i * 16) = make_uint4(0u, 0u, 0u, 0u);
-        *reinterpret_cast<uint4*>(tile + kPanel + i * 16) = make_uint4(0u, 0u, 0u, 0u);
-      }
-      bool found = false;
-      for (int i = lane + open * 8; i < real * 8; i += 32) {
-#pragma unroll
-        for (int panel = 0; panel < 2; ++panel) {
-          const uint4 x = *reinterpret_cast<const uint4*>(tile + panel * kPanel + i * 16);
-          const uint32_t e = 0x7f807f80u, words[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-          for (int p = 0; p < 4; ++p)
-            found |= (words[p] & e & 0xffffu) == (e & 0xffffu) || (words[p] & e) >> 16 == e >> 16;
-        }
-      }
-      if (__any_sync(0xffffffffu, found) && lane == 0)
+      const int key0 = (block0 + j) * kBlock;
+      if (clean_masked_values(sRing + s * kSlotBytes, max(0, row_limit(w, 0, a.causal) - key0),
+                              min(kBlock, w.keys - key0)) &&
+          lane == 0)
         *reinterpret_cast<volatile int*>(&bar->exact_rows) = 1;
-      fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar->slot_full[s]);
     }
@@ -384,7 +262,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
       const uint32_t sbuf = tmem + lane_addr + sb * 128;
       const bool partial = j >= masked_from;
-      const int64_t valid = limit - (w.block0 + j) * kBlock;
+      const int64_t valid = limit - (block0 + j) * kBlock;
       uint32_t keep[kKeptChunks<128>][32];
       const float mrow = warp_active ? row_max<128>(sbuf, partial, valid, keep) * c : -INFINITY;
       float m_prev = -INFINITY;
@@ -450,25 +328,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (ok && n > 0 && *reinterpret_cast<volatile int*>(&bar->exact_rows)) {
       for (int r = warp; r < w.tokens * G; r += 8) {
         const int t = r / G, h = head0 + r % G;
-        const int end = min(row_limit(w, t, a.causal), (w.block0 + n) * kBlock);
+        const int end = min(row_limit(w, t, a.causal), (block0 + n) * kBlock);
         float4 o;
         const float2 ml = exact_row(a, a.q + (w.q0 + t) * a.q_stride_t + h * a.q_stride_h, w.k0,
-                                    hk, w.block0 * kBlock, end, c, o);
-        const int64_t at = (w.q0 + t) * a.heads + h;
-        if constexpr (kSplit) {
-          const int64_t p = split * a.q_rows * a.heads + at;
-          *reinterpret_cast<float4*>(a.part_o + p * kHeadDim + lane * 4) = o;
-          if (lane == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * p) = ml;
-        } else {
-          const float inv = ml.y != 0.f ? 1.f / ml.y : 0.f;
-          *reinterpret_cast<uint2*>(a.out + at * kHeadDim + lane * 4) =
-              make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
-        }
+                                    hk, block0 * kBlock, end, c, o);
+        const int64_t p = (split * a.q_rows + w.q0 + t) * a.heads + h;
+        *reinterpret_cast<float4*>(a.part_o + p * kHeadDim + lane * 4) = o;
+        if (lane == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * p) = ml;
       }
     } else if (warp_active) {
-      const int64_t at = (w.q0 + token) * a.heads + head0 + (row - token * G);
-      const int64_t p = split * a.q_rows * a.heads + at;
-      const float inv_l = kSplit ? 1.f : l_row != 0.f ? 1.f / l_row : 0.f;
+      const int64_t p = (split * a.q_rows + w.q0 + token) * a.heads + head0 + (row - token * G);
 #pragma unroll 1
       for (int cc = 0; cc < 2; ++cc) {
         uint32_t o[32];
@@ -481,27 +350,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int x = 0; x < 32; ++x) o[x] = 0u;
         }
         if (!row_valid) continue;
-        if constexpr (kSplit) {
-          float4* dst = reinterpret_cast<float4*>(a.part_o + p * kHeadDim + grp * 64 + cc * 32);
+        float4* dst = reinterpret_cast<float4*>(a.part_o + p * kHeadDim + grp * 64 + cc * 32);
 #pragma unroll
-          for (int x = 0; x < 8; ++x)
-            dst[x] = make_float4(__uint_as_float(o[4 * x]), __uint_as_float(o[4 * x + 1]),
-                                 __uint_as_float(o[4 * x + 2]), __uint_as_float(o[4 * x + 3]));
-        } else {
-          uint4* dst = reinterpret_cast<uint4*>(a.out + at * kHeadDim + grp * 64 + cc * 32);
-#pragma unroll
-          for (int x = 0; x < 4; ++x)
-            dst[x] = make_uint4(
-                pack_bf16x2(__uint_as_float(o[8 * x]) * inv_l, __uint_as_float(o[8 * x + 1]) * inv_l),
-                pack_bf16x2(__uint_as_float(o[8 * x + 2]) * inv_l, __uint_as_float(o[8 * x + 3]) * inv_l),
-                pack_bf16x2(__uint_as_float(o[8 * x + 4]) * inv_l, __uint_as_float(o[8 * x + 5]) * inv_l),
-                pack_bf16x2(__uint_as_float(o[8 * x + 6]) * inv_l, __uint_as_float(o[8 * x + 7]) * inv_l));
-        }
+        for (int x = 0; x < 8; ++x)
+          dst[x] = make_float4(__uint_as_float(o[4 * x]), __uint_as_float(o[4 * x + 1]),
+                               __uint_as_float(o[4 * x + 2]), __uint_as_float(o[4 * x + 3]));
       }
-      if constexpr (kSplit) {
-        if (row_valid && grp == 0)
-          *reinterpret_cast<float2*>(a.part_ml + 2 * p) = make_float2(m_fin, l_row);
-      }
+      if (row_valid && grp == 0)
+        *reinterpret_cast<float2*>(a.part_ml + 2 * p) = make_float2(m_fin, l_row);
     }
   }
   tc_fence_before();
@@ -542,9 +398,8 @@ __global__ void __launch_bounds__(256) combine_kernel(const PackedArgs a) {
       make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
 }
 
-template <bool kSplit>
-cudaError_t launch_main(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
-                        const PackedArgs& a, cudaStream_t stream) {
+cudaError_t launch_parts(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
+                         const PackedArgs& a, cudaStream_t stream) {
   static std::atomic<int> smem_bytes[64] = {};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -556,13 +411,13 @@ cudaError_t launch_main(const CUtensorMap& tq, const CUtensorMap& tk, const CUte
     if (e != cudaSuccess) return e;
     bytes = optin < kUsed + 1024 ? optin : kUsed + 1024;
     if (bytes < kUsed) return cudaErrorInvalidConfiguration;
-    e = cudaFuncSetAttribute(packed_attention_kernel<kSplit>,
+    e = cudaFuncSetAttribute(packed_attention_split_kernel,
                              cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64) smem_bytes[dev].store(bytes, std::memory_order_release);
   }
   const int64_t grid = a.slots * a.kv_heads * a.splits;
-  packed_attention_kernel<kSplit><<<static_cast<unsigned>(grid), kThreads, bytes, stream>>>(tq, tk, tv, a);
+  packed_attention_split_kernel<<<static_cast<unsigned>(grid), kThreads, bytes, stream>>>(tq, tk, tv, a);
   return cudaGetLastError();
 }
 
@@ -574,17 +429,15 @@ int32_t packed_splits(int64_t q_rows, int64_t k_rows, int32_t requests, int32_t 
                       int32_t kv_heads, int num_sms) {
   const int64_t ctas = (q_rows / (128 / (heads / kv_heads)) + requests) * kv_heads;
   if (ctas >= 2 * num_sms) return 1;
-  int64_t splits = (4 * num_sms + ctas - 1) / ctas;
-  const int64_t most = k_rows / requests / 512;
-  splits = splits < most ? splits : most;
-  return static_cast<int32_t>(splits < 1 ? 1 : splits);
+  const int64_t splits = std::min((4 * num_sms + ctas - 1) / ctas, k_rows / requests / 512);
+  return static_cast<int32_t>(std::max<int64_t>(1, splits));
 }
 
 cudaError_t launch_packed_attention(const CUtensorMap& tq, const CUtensorMap& tk,
                                     const CUtensorMap& tv, const PackedArgs& a,
                                     cudaStream_t stream) {
-  if (a.splits == 1) return launch_main<false>(tq, tk, tv, a, stream);
-  const cudaError_t e = launch_main<true>(tq, tk, tv, a, stream);
+  if (a.splits == 1) return launch_packed_tiles(tq, tk, tv, a, stream);
+  const cudaError_t e = launch_parts(tq, tk, tv, a, stream);
   if (e != cudaSuccess) return e;
   const int64_t rows = a.q_rows * a.heads;
   combine_kernel<<<static_cast<unsigned>((rows + 7) / 8), 256, 0, stream>>>(a);

@@ -1,0 +1,581 @@
+// Softmax attention over packed sequences of different lengths, grouped heads,
+// causal or full, for sm_100a:
+//   out[i, h] = sum_j softmax_j(scale * q[i, h] . k[j, h / G]) v[j, h / G]
+// over the keys j of query i's own request (causal: the first
+// i + 1 + k_len - q_len of them, i counted within the request), in float32
+// from bf16 inputs; a query that sees no key gives 0.
+//
+// An item is 2 x (128 / G tokens) x G heads of one key head: two MMA tiles of
+// 128 rows (row = token * G + head in group), so that all query heads of a key
+// head, and both tiles, share its K and V loads.  While one tile's softmax
+// runs, the tensor pipe works for the other.  CTAs are resident and take their
+// next item from the grid's CTAs that have not started (cluster launch
+// control), so an item's first loads and S run under the last softmax and the
+// store of the item before.  Items are found on the device (packed_common.cuh),
+// those late in their request first: under the causal mask they see the most
+// keys.
+//   warp 8      TMA producer: Q; K/V blocks of 128 keys into a ring of 32 KB
+//               slots (K0, K1, V0, K2, V1, ...)
+//   warp 9      TMEM owner; one thread issues every MMA: for each block j and
+//               tile t, O_t += P_t V_j, then S_t = Q_t K_{j+1}^T
+//   warp 10     scheduler: cancels a pending CTA, looks its item up, publishes
+//   warp 11     cleans V of the masked blocks (clean_masked_values)
+//   warps 0-3, 4-7   softmax of tile 0, 1: one row a thread, log2 domain, a
+//               stabiliser that moves only past 2^8 (then O_t is rescaled in
+//               TMEM), P_t as bf16 into the first 64 columns of S_t
+// TMEM: S_0 [0, 128), S_1 [128, 256), O_0 [256, 384), O_1 [384, 512).  S_t(j+1)
+// follows O_t += P_t V_j in the issue order of one thread, which is what lets
+// P_t live in S_t's columns and makes s_full mean that PV is complete.
+//
+// A value of V that is not finite at a key which part of the item must not see
+// (causal) cannot be kept out of those rows by P = 0; warp 11 looks for one
+// and, if there is, the item's rows are computed again key by key in float32.
+//
+// Every mbarrier wait is bounded (bsa::mbar_wait); on a timeout the CTA sets
+// kErrWaitTimeout, drains its copies and MMAs, frees TMEM and exits.
+#include <atomic>
+
+#include "packed_attention.cuh"
+
+namespace bsa {
+namespace {
+
+using namespace attn;
+using namespace packed;
+
+constexpr int kThreads = 384;
+constexpr int kProducerWarp = 8;
+constexpr int kMmaWarp = 9;
+constexpr int kSchedWarp = 10;
+constexpr int kCheckWarp = 11;
+constexpr int kSlots = 5;
+constexpr int kMaskedRing = 4;          // masked V blocks between the producer and warp 11
+#ifndef BSA_PACKED_EMULATED
+#define BSA_PACKED_EMULATED 0
+#endif
+constexpr int kEmulated = BSA_PACKED_EMULATED;
+constexpr int kWorkRing = 2;            // an item at work and the next
+constexpr int kWorkReaders = 11;        // warps 0-7, producer, MMA, check
+constexpr int kQOff = 0;
+constexpr int kRingOff = 2 * kSlotBytes;
+constexpr int kBarOff = kRingOff + kSlots * kSlotBytes;
+
+// An item as the scheduler publishes it.
+struct Item {
+  Work w;              // w.tokens < 0: no more items
+  int hk;              // key head
+  int n[2];            // key blocks of each tile
+  int exact;           // set by warp 11
+};
+
+struct Barriers {
+  uint64_t q_full, q_empty;
+  uint64_t s_full[2];
+  uint64_t p_half[2], p_full[2];
+  uint64_t o_full[2], o_empty[2];
+  uint64_t slot_full[kSlots], slot_empty[kSlots];
+  uint64_t masked_full[kMaskedRing];    // V of a masked block, before warp 11
+  uint64_t work_full[kWorkRing], work_empty[kWorkRing];
+  uint64_t next_full;                   // answer of the cluster launch control
+  uint64_t drain;
+  uint32_t tmem_base;
+  int abort;
+  Item item[kWorkRing];
+  uint4 next __attribute__((aligned(16)));
+};
+constexpr int kUsed = kBarOff + static_cast<int>(sizeof(Barriers));
+
+// Cluster launch control: ask for a CTA of this grid that has not started to
+// be cancelled, its index to be taken over by the caller.
+__device__ __forceinline__ void request_next(uint4* answer, uint64_t* bar) {
+  asm volatile(
+      "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+          smem_u32(answer)),
+      "r"(smem_u32(bar))
+      : "memory");
+}
+// blockIdx.x of the cancelled CTA, or -1 (all have started).
+__device__ __forceinline__ int64_t answered_next(const uint4* answer) {
+  uint32_t ok, x;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b128 r;\n\t"
+      "ld.shared.b128 r, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "mov.u32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n\t}"
+      : "=r"(ok), "=r"(x)
+      : "r"(smem_u32(answer))
+      : "memory");
+  return ok ? static_cast<int64_t>(x) : -1;
+}
+
+__global__ void __launch_bounds__(kThreads, 1)
+    packed_attention_tiles_kernel(const __grid_constant__ CUtensorMap tm_q,
+                                  const __grid_constant__ CUtensorMap tm_k,
+                                  const __grid_constant__ CUtensorMap tm_v, const PackedArgs a) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* sQ = smem + kQOff;
+  uint8_t* sRing = smem + kRingOff;
+  Barriers* bar = reinterpret_cast<Barriers*>(smem + kBarOff);
+  volatile int* abort_flag = &bar->abort;
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int G = a.group;
+  const int tt = a.tile_tokens;
+
+  if (threadIdx.x == 0) {
+    uint32_t dyn_bytes;
+    asm("mov.u32 %0, %%dynamic_smem_size;" : "=r"(dyn_bytes));
+    const bool fits = (smem - smem_raw) + kUsed <= static_cast<int>(dyn_bytes);
+    bar->abort = (prior_timeout(a.err_word) || !fits) ? 1 : 0;
+    if (!fits) atomicOr(a.err_word, kErrSmemLayout);
+    mbar_init(&bar->q_full, 1);
+    mbar_init(&bar->q_empty, 1);
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&bar->s_full[t], 1);
+      mbar_init(&bar->p_half[t], 128);
+      mbar_init(&bar->p_full[t], 128);
+      mbar_init(&bar->o_full[t], 1);
+      mbar_init(&bar->o_empty[t], 128);
+    }
+    for (int s = 0; s < kSlots; ++s) {
+      mbar_init(&bar->slot_full[s], 1);
+      mbar_init(&bar->slot_empty[s], 1);
+    }
+    for (int i = 0; i < kMaskedRing; ++i) mbar_init(&bar->masked_full[i], 1);
+    for (int i = 0; i < kWorkRing; ++i) {
+      mbar_init(&bar->work_full[i], 1);
+      mbar_init(&bar->work_empty[i], kWorkReaders);
+    }
+    mbar_init(&bar->next_full, 1);
+    mbar_init(&bar->drain, 1);
+    fence_mbar_init();
+  }
+  __syncthreads();
+  if (bar->abort) return;  // uniform: set before the barrier, read after it
+  if (warp == kMmaWarp) tmem_alloc(&bar->tmem_base, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bar->tmem_base;
+
+  // Item number i of this CTA, or null (no more, or aborting).
+  auto item_at = [&](int i) -> Item* {
+    const int r = i % kWorkRing;
+    if (!mbar_wait(&bar->work_full[r], (i / kWorkRing) & 1, abort_flag, a.err_word)) return nullptr;
+    Item* it = &bar->item[r];
+    return it->w.tokens < 0 ? nullptr : it;
+  };
+  auto done_with = [&](int i) { mbar_arrive(&bar->work_empty[i % kWorkRing]); };
+  // First block of the item that some row of tile t does not see whole.
+  auto masked_from = [&](const Work& w, int t) { return row_limit(w, t * tt, a.causal) / kBlock; };
+
+  if (warp == kSchedWarp) {
+    // ------------------------------------------------------------ scheduler
+    int64_t cta = blockIdx.x;
+    uint32_t answers = 0;
+    for (int i = 0;;) {
+      Item it{};
+      it.w.tokens = -1;
+      if (cta >= 0) {
+        // late slots first; a key head's items next to each other
+        it.hk = static_cast<int>(cta % a.kv_heads);
+        it.w = find_work(a, a.slots - 1 - cta / a.kv_heads, 2 * tt);
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&bar->next_full, 16);
+          request_next(&bar->next, &bar->next_full);
+        }
+      }
+      if (it.w.tokens != 0) {
+        for (int t = 0; t < 2; ++t) {
+          const int last = min(it.w.tokens, (t + 1) * tt) - 1;
+          it.n[t] = last < t * tt ? 0 : (row_limit(it.w, last, a.causal) + kBlock - 1) / kBlock;
+        }
+        bool ok = true;
+        if (lane == 0) {
+          const int r = i % kWorkRing;
+          ok = mbar_wait(&bar->work_empty[r], ((i / kWorkRing) & 1) ^ 1, abort_flag, a.err_word);
+          if (ok) {
+            bar->item[r] = it;
+            mbar_arrive(&bar->work_full[r]);
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        ++i;
+        if (cta < 0) break;
+        if (!ok) {
+          int never = 0;   // an answer is on its way into shared memory
+          mbar_wait(&bar->next_full, answers & 1, &never, a.err_word);
+          break;
+        }
+      }
+      if (!mbar_wait(&bar->next_full, answers & 1, abort_flag, a.err_word)) {
+        int never = 0;
+        mbar_wait(&bar->next_full, answers & 1, &never, a.err_word);
+        break;
+      }
+      ++answers;
+      cta = answered_next(&bar->next);
+      fence_proxy_async_smem();   // the answer is read before the next one is asked for
+      __syncwarp();
+    }
+  } else if (warp == kProducerWarp) {
+    // ------------------------------------------------------------ producer
+    if (lane == 0) {
+      uint32_t armed = 0, armed_phase = 0;
+      int seq = 0, masked = 0, loads = 0;      // of K/V, of masked V, of Q
+      bool ok = true;
+      for (int i = 0; ok; ++i) {
+        const Item* it = item_at(i);
+        if (it == nullptr) break;
+        const Work w = it->w;
+        const int hk = it->hk;
+        const int n = max(it->n[0], it->n[1]);
+        done_with(i);
+        const int from = masked_from(w, 0);
+        auto load = [&](const CUtensorMap* tm, int j, bool is_v) {
+          const int s = seq % kSlots;
+          const uint32_t ph = (seq / kSlots) & 1;
+          if (!mbar_wait(&bar->slot_empty[s], ph ^ 1, abort_flag, a.err_word)) return false;
+          uint8_t* dst = sRing + s * kSlotBytes;
+          uint64_t* full = &bar->slot_full[s];
+          if (is_v && j >= from) {
+            full = &bar->masked_full[masked++ % kMaskedRing];
+            armed &= ~(1u << s);   // an earlier load of this slot has long been consumed
+          } else {
+            armed |= 1u << s;
+            armed_phase = (armed_phase & ~(1u << s)) | (ph << s);
+          }
+          const int row = static_cast<int>(w.k0 + static_cast<int64_t>(j) * kBlock);
+          mbar_arrive_expect_tx(full, kSlotBytes);
+          tma_load_3d(dst, tm, full, 0, hk, row);
+          tma_load_3d(dst + kPanel, tm, full, 64, hk, row);
+          ++seq;
+          return true;
+        };
+        if (n == 0) continue;
+        ok = load(&tm_k, 0, false);
+        if (ok) ok = mbar_wait(&bar->q_empty, (loads & 1) ^ 1, abort_flag, a.err_word);
+        if (!ok) break;
+        // Rows past tt * G keep whatever the shared memory held: a row of
+        // garbage reaches only its own row of S and O, which is not stored.
+        mbar_arrive_expect_tx(&bar->q_full, static_cast<uint32_t>(tt * G) * 512u);
+        for (int t = 0; t < 2; ++t)
+          for (int p = 0; p < 2; ++p)
+            tma_load_3d(sQ + t * kSlotBytes + p * kPanel, &tm_q, &bar->q_full, p * 64, hk * G,
+                        static_cast<int>(w.q0) + t * tt);
+        ++loads;
+        for (int j = 0; ok && j < n; ++j) {
+          if (j + 1 < n) ok = load(&tm_k, j + 1, false);
+          if (ok) ok = load(&tm_v, j, true);
+        }
+      }
+      // Never leave a copy in flight into shared memory.
+      int never = 0;
+#pragma unroll
+      for (int s = 0; s < kSlots; ++s)
+        if (armed & (1u << s))
+          mbar_wait(&bar->slot_full[s], (armed_phase >> s) & 1u, &never, a.err_word);
+      for (int j = max(0, masked - kMaskedRing); j < masked; ++j)
+        mbar_wait(&bar->masked_full[j % kMaskedRing], (j / kMaskedRing) & 1, &never, a.err_word);
+      if (loads) mbar_wait(&bar->q_full, (loads - 1) & 1, &never, a.err_word);
+    }
+  } else if (warp == kMmaWarp) {
+    // ------------------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      const uint32_t idesc_s = idesc_bf16_f32(128, kBlock, false);
+      const uint32_t idesc_o = idesc_bf16_f32(128, kHeadDim, true);
+      const uint64_t kdesc0 = sdesc_sw128(smem_u32(sRing), 16, 1024);
+      const uint64_t vdesc0 = sdesc_sw128(smem_u32(sRing), kPanel, 1024);
+      const uint64_t qdesc0 = sdesc_sw128(smem_u32(sQ), 16, 1024);
+      int seq = 0, loads = 0;
+      int blocks[2] = {0, 0}, outs[2] = {0, 0};   // P consumed, O finished, of each tile
+      bool ok = true;
+      auto wait = [&](uint64_t* b, uint32_t parity) {
+        ok = ok && mbar_wait(b, parity, abort_flag, a.err_word);
+        return ok;
+      };
+      for (int i = 0; ok; ++i) {
+        const Item* it = item_at(i);
+        if (it == nullptr) break;
+        const int nt[2] = {it->n[0], it->n[1]};
+        done_with(i);
+        const int n = max(nt[0], nt[1]);
+        if (n == 0) continue;
+        auto issue_s = [&](int t, int s) {
+          const uint64_t kd = kdesc0 + static_cast<uint64_t>((s * kSlotBytes) >> 4);
+          const uint64_t qd = qdesc0 + static_cast<uint64_t>((t * kSlotBytes) >> 4);
+#pragma unroll
+          for (int kk = 0; kk < kHeadDim / 16; ++kk) {
+            const uint64_t off = static_cast<uint64_t>(((kk >> 2) * kPanel + (kk & 3) * 32) >> 4);
+            umma_bf16_ss(tmem + t * 128, qd + off, kd + off, idesc_s, kk > 0 ? 1u : 0u);
+          }
+          umma_commit(&bar->s_full[t]);
+        };
+        int sk = seq % kSlots;
+        wait(&bar->slot_full[sk], (seq / kSlots) & 1);
+        ++seq;
+        wait(&bar->q_full, loads & 1);
+        ++loads;
+        if (!ok) break;
+        tc_fence_after();
+        for (int t = 0; t < 2; ++t)
+          if (nt[t] > 0) issue_s(t, sk);
+        umma_commit(&bar->slot_empty[sk]);
+        if (n == 1) umma_commit(&bar->q_empty);
+        for (int j = 0; ok && j < n; ++j) {
+          // slots in load order: K_{j+1}, V_j
+          int sk1 = 0;
+          if (j + 1 < n) {
+            sk1 = seq % kSlots;
+            if (!wait(&bar->slot_full[sk1], (seq / kSlots) & 1)) break;
+            ++seq;
+          }
+          const int sv = seq % kSlots;
+          if (!wait(&bar->slot_full[sv], (seq / kSlots) & 1)) break;
+          ++seq;
+          const uint64_t vd = vdesc0 + static_cast<uint64_t>((sv * kSlotBytes) >> 4);
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (j >= nt[t] || !ok) continue;
+            // the first PV of an item overwrites the O that its softmax group stores
+            if (j == 0) wait(&bar->o_empty[t], (outs[t] & 1) ^ 1);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              if (!wait(half ? &bar->p_full[t] : &bar->p_half[t], blocks[t] & 1)) break;
+              tc_fence_after();
+#pragma unroll
+              for (int kk = half * 4; kk < half * 4 + 4; ++kk)
+                umma_bf16_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8,
+                             vd + static_cast<uint64_t>((kk * 16 * 128) >> 4), idesc_o,
+                             (j > 0 || kk > 0) ? 1u : 0u);
+            }
+            if (!ok) continue;
+            ++blocks[t];
+            if (j + 1 < nt[t]) {
+              issue_s(t, sk1);
+            } else {
+              umma_commit(&bar->o_full[t]);
+              ++outs[t];
+            }
+          }
+          if (!ok) break;
+          umma_commit(&bar->slot_empty[sv]);
+          if (j + 1 < n) umma_commit(&bar->slot_empty[sk1]);
+          if (j + 2 == n) umma_commit(&bar->q_empty);
+        }
+      }
+      int never = 0;
+      umma_commit(&bar->drain);
+      mbar_wait(&bar->drain, 0, &never, a.err_word);
+    }
+  } else if (warp == kCheckWarp) {
+    // ------------------------------------------------------ masked V blocks
+    int seq = 0, masked = 0;
+    for (int i = 0;; ++i) {
+      Item* it = item_at(i);
+      if (!__all_sync(0xffffffffu, it != nullptr)) break;
+      const Work w = it->w;
+      const int n = max(it->n[0], it->n[1]);
+      bool ok = true;
+      for (int j = masked_from(w, 0); ok && j < n; ++j) {
+        ok = mbar_wait(&bar->masked_full[masked % kMaskedRing], (masked / kMaskedRing) & 1, abort_flag,
+                       a.err_word);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        ++masked;
+        const int s = (seq + (j + 1 < n ? 2 * j + 2 : 2 * j + 1)) % kSlots;
+        const int key0 = j * kBlock;
+        if (clean_masked_values(sRing + s * kSlotBytes, max(0, row_limit(w, 0, a.causal) - key0),
+                                min(kBlock, w.keys - key0)) &&
+            lane == 0)
+          *reinterpret_cast<volatile int*>(&it->exact) = 1;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar->slot_full[s]);
+      }
+      if (!ok) break;
+      seq += 2 * n;
+      __syncwarp();
+      if (lane == 0) done_with(i);
+    }
+  } else {
+    // ------------------------------------------------------------ softmax
+    const int t = warp >> 2;                   // this group's tile
+    const int wq = warp & 3;
+    const int row = wq * 32 + lane;
+    const uint32_t lane_addr = static_cast<uint32_t>(wq * 32) << 16;
+    const uint32_t sbuf = tmem + lane_addr + t * 128;
+    const uint32_t obuf = tmem + lane_addr + 256 + t * 128;
+    const int token = t * tt + row / G;        // in the item
+    const int head_in_group = row - row / G * G;
+    const float c = a.scale * kLog2e;
+    const float2 c2 = make_float2(c, c);
+    int blocks = 0, outs = 0;
+    bool ok = true;
+    for (int i = 0; ok; ++i) {
+      Item* it = item_at(i);
+      if (!__all_sync(0xffffffffu, it != nullptr)) break;
+      const Work w = it->w;
+      const int n = t ? it->n[1] : it->n[0];
+      const int head = it->hk * G + head_in_group;
+      const int from = masked_from(w, t);
+      // rows past the tile's tokens x heads (row / G >= tt) belong to no query
+      const int limit = row < tt * G ? row_limit(w, token, a.causal) : 0;
+      const bool row_valid = row < tt * G && token < w.tokens;
+      const bool warp_active = wq * 32 < min(tt, w.tokens - t * tt) * G;
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < n; ++j) {
+        ok = mbar_wait(&bar->s_full[t], blocks & 1, abort_flag, a.err_word);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        ++blocks;
+        tc_fence_after();
+        if (warp_active) {
+          const bool partial = j >= from;
+          const int64_t valid = limit - j * kBlock;
+          uint32_t keep[2][32];
+          const float mrow = row_max<128, 2>(sbuf, partial, valid, keep) * c;
+          const bool need = mrow > m + kRescaleThreshold;
+          const float m_used = need ? mrow : m;
+          // O_t holds the blocks before j relative to m; PV(j - 1) is complete.
+          if (j > 0 && __any_sync(0xffffffffu, need)) {
+            const float f = need ? ex2_approx(m - m_used) : 1.f;
+            l *= f;
+#pragma unroll 1
+            for (int cc = 0; cc < kHeadDim / 32; ++cc) {
+              uint32_t o[32];
+              tmem_ld_32x32b_x32(obuf + cc * 32, o);
+              tmem_wait_ld();
+              reg_fence<32>(o);
+#pragma unroll
+              for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+              tmem_st_32x32b_x32(obuf + cc * 32, o);
+            }
+          }
+          m = m_used;
+          // -inf stands for "no key yet": the exponents (all -inf) are taken against 0.
+          const float neg = m == -INFINITY ? 0.f : -m;
+          const float2 neg_m = make_float2(neg, neg);
+          float2 acc[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f),
+                           make_float2(0.f, 0.f)};
+          uint32_t r[2][32];
+          tmem_ld_32x32b_x32(sbuf, r[0]);
+          tmem_wait_ld();
+          reg_fence<32>(r[0]);
+          tmem_ld_32x32b_x32(sbuf + 32, r[1]);
+          if (partial) mask_chunk(r[0], 0, valid);
+          exp_chunk<kEmulated>(r[0], c2, neg_m, acc, sbuf);
+          tmem_wait_ld();
+          reg_fence<32>(r[1]);
+          if (partial) mask_chunk(r[1], 32, valid);
+          exp_chunk<kEmulated>(r[1], c2, neg_m, acc, sbuf + 16);
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(&bar->p_half[t]);
+          exp_chunk<kEmulated>(keep[0], c2, neg_m, acc, sbuf + 32);
+          exp_chunk<kEmulated>(keep[1], c2, neg_m, acc, sbuf + 48);
+          const float2 sum = __fadd2_rn(__fadd2_rn(acc[0], acc[1]), __fadd2_rn(acc[2], acc[3]));
+          l += sum.x + sum.y;
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(&bar->p_full[t]);
+        } else {
+          mbar_arrive(&bar->p_half[t]);
+          mbar_arrive(&bar->p_full[t]);
+        }
+      }
+      if (!ok) break;
+      // ---------------------------------------------------------- epilogue
+      if (n > 0) {
+        ok = mbar_wait(&bar->o_full[t], outs & 1, abort_flag, a.err_word);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        ++outs;
+        tc_fence_after();
+      }
+      if (n > 0 && *reinterpret_cast<volatile int*>(&it->exact)) {
+        const int rows = min(tt, w.tokens - t * tt) * G;
+        for (int r = wq; r < rows; r += 4) {
+          const int64_t q_row = w.q0 + t * tt + r / G;
+          const int h = it->hk * G + r % G;
+          float4 o;
+          const float2 ml = exact_row(a, a.q + q_row * a.q_stride_t + h * a.q_stride_h, w.k0, it->hk, 0,
+                                      row_limit(w, t * tt + r / G, a.causal), c, o);
+          const float inv = ml.y != 0.f ? 1.f / ml.y : 0.f;
+          *reinterpret_cast<uint2*>(a.out + (q_row * a.heads + h) * kHeadDim + lane * 4) =
+              make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+        }
+        mbar_arrive(&bar->o_empty[t]);
+      } else {
+        const float inv_l = l != 0.f ? 1.f / l : 0.f;
+        __nv_bfloat16* out = a.out + ((w.q0 + token) * a.heads + head) * kHeadDim;
+#pragma unroll
+        for (int cc = 0; cc < kHeadDim / 32; ++cc) {
+          uint32_t o[32];
+          if (n > 0 && warp_active) {
+            tmem_ld_32x32b_x32(obuf + cc * 32, o);
+            tmem_wait_ld();
+            reg_fence<32>(o);
+          } else {
+#pragma unroll
+            for (int x = 0; x < 32; ++x) o[x] = 0u;
+          }
+          if (cc == kHeadDim / 32 - 1 && n > 0) {
+            tc_fence_before();
+            mbar_arrive(&bar->o_empty[t]);     // O_t is in registers: its buffer is free
+          }
+          if (row_valid) {
+            uint4* dst = reinterpret_cast<uint4*>(out + cc * 32);
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              dst[x] = make_uint4(
+                  pack_bf16x2(__uint_as_float(o[8 * x]) * inv_l, __uint_as_float(o[8 * x + 1]) * inv_l),
+                  pack_bf16x2(__uint_as_float(o[8 * x + 2]) * inv_l, __uint_as_float(o[8 * x + 3]) * inv_l),
+                  pack_bf16x2(__uint_as_float(o[8 * x + 4]) * inv_l, __uint_as_float(o[8 * x + 5]) * inv_l),
+                  pack_bf16x2(__uint_as_float(o[8 * x + 6]) * inv_l, __uint_as_float(o[8 * x + 7]) * inv_l));
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) done_with(i);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+}  // namespace
+
+cudaError_t launch_packed_tiles(const CUtensorMap& tq, const CUtensorMap& tk,
+                                const CUtensorMap& tv, const PackedArgs& args,
+                                cudaStream_t stream) {
+  static std::atomic<int> smem_bytes[64] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  int bytes = (dev >= 0 && dev < 64) ? smem_bytes[dev].load(std::memory_order_acquire) : 0;
+  if (bytes == 0) {
+    int optin = 0;
+    e = cudaDeviceGetAttribute(&optin, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev);
+    if (e != cudaSuccess) return e;
+    bytes = optin < kUsed + 1024 ? optin : kUsed + 1024;
+    if (bytes < kUsed) return cudaErrorInvalidConfiguration;
+    e = cudaFuncSetAttribute(packed_attention_tiles_kernel,
+                             cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return e;
+    if (dev >= 0 && dev < 64) smem_bytes[dev].store(bytes, std::memory_order_release);
+  }
+  PackedArgs a = args;
+  a.slots = a.q_rows / (2 * a.tile_tokens) + a.requests;
+  packed_attention_tiles_kernel<<<static_cast<unsigned>(a.slots * a.kv_heads), kThreads, bytes,
+                                  stream>>>(tq, tk, tv, a);
+  return cudaGetLastError();
+}
+
+}  // namespace bsa

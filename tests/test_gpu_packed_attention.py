@@ -91,6 +91,47 @@ def test_different_lengths(q_lengths, k_lengths, causal, heads, kv_heads):
     check(call(t, causal=causal), t, causal)
 
 
+def reference64(t, causal):
+    """The definition in float64 torch on the GPU (larger cases), and with |v|."""
+    q, k, v = (t[x].double() for x in "qkv")
+    group = q.shape[1] // k.shape[1]
+    k, v = k.repeat_interleave(group, 1), v.repeat_interleave(group, 1)
+    qs, ks = t["qs"].tolist(), t["ks"].tolist()
+    ref, mag = torch.zeros_like(q), torch.zeros_like(q)
+    for s in range(len(qs) - 1):
+        a, b = slice(qs[s], qs[s + 1]), slice(ks[s], ks[s + 1])
+        n, m = a.stop - a.start, b.stop - b.start
+        if not n or not m:
+            continue
+        w = torch.einsum("ihd,jhd->hij", q[a], k[b]) * 128 ** -0.5
+        if causal:
+            hidden = (torch.arange(m, device=DEV)[None]
+                      > torch.arange(n, device=DEV)[:, None] + (m - n))
+            w = w.masked_fill(hidden, float("-inf"))
+        w = torch.softmax(w, -1).nan_to_num(0.0)
+        ref[a] = torch.einsum("hij,jhd->ihd", w, v[b])
+        mag[a] = torch.einsum("hij,jhd->ihd", w, v[b].abs())
+    return ref, mag
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("heads,kv_heads", [(16, 16), (16, 4), (40, 8), (12, 4), (24, 3)])
+def test_many_items(heads, kv_heads, causal):
+    """Several items a CTA: requests of very different lengths, among them
+    empty ones and ones without keys, blocks of every kind next to each other."""
+    q_lengths = [700, 1, 0, 333, 1500, 64, 129, 9, 256, 40, 2, 511]
+    k_lengths = [700, 1, 5, 333, 900, 2000, 129, 0, 512, 39, 300, 511]
+    t = make(q_lengths, k_lengths, heads, kv_heads, seed=heads + causal)
+    out = call(t, causal=causal)
+    ref, mag = reference64(t, causal)
+    big = 128 ** -0.5 * t["q"].double().abs().sum(-1).max() * t["k"].double().abs().max()
+    top = 128 ** -0.5 * (t["q"].double().pow(2).sum(-1).max() * t["k"].double().pow(2).sum(-1).max()).sqrt()
+    share = 1.01 * U16 + 2 * (136 * U32 * big + 4 * 2.0 ** -22 * (1 + top)) + 2004 * U32
+    tol = 1.01 * U16 * ref.abs() + share * mag + 1e-30
+    assert ((out.double() - ref).abs() <= tol).all()
+    assert all(torch.equal(call(t, causal=causal), out) for _ in range(5))
+
+
 def test_long_single_tokens_split():
     """Few rows over long keys: the keys are split over CTAs and joined."""
     k_lengths = [5000, 1, 2048, 0, 777]
