@@ -14,15 +14,18 @@
 // store of the item before.  Items are found on the device (packed_common.cuh),
 // those late in their request first: under the causal mask they see the most
 // keys.
-//   warp 8      TMA producer: Q; K/V blocks of 128 keys into a ring of 32 KB
+//   warps 0-3, 4-7   softmax of tile 0, 1: one row a thread, all 128 scores in
+//               registers, log2 domain, a stabiliser that moves only past 2^8
+//               (then O_t is rescaled in TMEM), P_t as bf16 into the first 64
+//               columns of S_t
+//   warps 8, 9  MMA issuers, one thread for each tile t: for each block j,
+//               O_t += P_t V_j (each half of the keys as soon as its P is
+//               there), then S_t = Q_t K_{j+1}^T; warp 8 owns TMEM.  A tile has
+//               its own issuer so that it never waits for the other's softmax.
+//   warp 10     TMA producer: Q; K/V blocks of 128 keys into a ring of 32 KB
 //               slots (K0, K1, V0, K2, V1, ...)
-//   warp 9      TMEM owner; one thread issues every MMA: for each block j and
-//               tile t, O_t += P_t V_j, then S_t = Q_t K_{j+1}^T
-//   warp 10     scheduler: cancels a pending CTA, looks its item up, publishes
-//   warp 11     cleans V of the masked blocks (clean_masked_values)
-//   warps 0-3, 4-7   softmax of tile 0, 1: one row a thread, log2 domain, a
-//               stabiliser that moves only past 2^8 (then O_t is rescaled in
-//               TMEM), P_t as bf16 into the first 64 columns of S_t
+//   warp 11     scheduler: cancels a pending CTA, looks its item up, publishes
+//   warp 12     cleans V of the masked blocks (clean_masked_values)
 // TMEM: S_0 [0, 128), S_1 [128, 256), O_0 [256, 384), O_1 [384, 512).  S_t(j+1)
 // follows O_t += P_t V_j in the issue order of one thread, which is what lets
 // P_t live in S_t's columns and makes s_full mean that PV is complete.
@@ -43,22 +46,32 @@ namespace {
 using namespace attn;
 using namespace packed;
 
-constexpr int kThreads = 384;
-constexpr int kProducerWarp = 8;
-constexpr int kMmaWarp = 9;
-constexpr int kSchedWarp = 10;
-constexpr int kCheckWarp = 11;
-constexpr int kSlots = 5;
+constexpr int kSoftWarps = 8;
+constexpr int kThreads = 512;
+constexpr int kMmaWarp = 8;             // and 9
+constexpr int kProducerWarp = 10;
+constexpr int kSchedWarp = 11;
+constexpr int kCheckWarp = 12;
+// The two control warpgroups give registers to the two softmax warpgroups,
+// within the launch's total.
+constexpr uint32_t kLaunchRegs = 128;
+constexpr uint32_t kSoftRegs = 200;
+constexpr uint32_t kControlRegs = 56;
+static_assert(256 * kSoftRegs + 256 * kControlRegs <= kThreads * kLaunchRegs,
+              "register split must stay within the launch total");
+constexpr int kSlots = 4;
 constexpr int kMaskedRing = 4;          // masked V blocks between the producer and warp 11
 #ifndef BSA_PACKED_EMULATED
 #define BSA_PACKED_EMULATED 0
 #endif
 constexpr int kEmulated = BSA_PACKED_EMULATED;
 constexpr int kWorkRing = 2;            // an item at work and the next
-constexpr int kWorkReaders = 11;        // warps 0-7, producer, MMA, check
+constexpr int kWorkReaders = kSoftWarps + 4;   // and both issuers, producer, check
 constexpr int kQOff = 0;
 constexpr int kRingOff = 2 * kSlotBytes;
-constexpr int kBarOff = kRingOff + kSlots * kSlotBytes;
+constexpr int kStageOff = kRingOff + kSlots * kSlotBytes;
+constexpr int kStageBytes = 32 * 128;   // of each softmax warp: 64 features of its 32 rows
+constexpr int kBarOff = kStageOff + kSoftWarps * kStageBytes;
 
 // An item as the scheduler publishes it.
 struct Item {
@@ -76,8 +89,9 @@ struct Barriers {
   uint64_t slot_full[kSlots], slot_empty[kSlots];
   uint64_t masked_full[kMaskedRing];    // V of a masked block, before warp 11
   uint64_t work_full[kWorkRing], work_empty[kWorkRing];
+  uint64_t turn[2];                     // the other tile's exponentials are done
   uint64_t next_full;                   // answer of the cluster launch control
-  uint64_t drain;
+  uint64_t drain[2];
   uint32_t tmem_base;
   int abort;
   Item item[kWorkRing];
@@ -134,17 +148,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     bar->abort = (prior_timeout(a.err_word) || !fits) ? 1 : 0;
     if (!fits) atomicOr(a.err_word, kErrSmemLayout);
     mbar_init(&bar->q_full, 1);
-    mbar_init(&bar->q_empty, 1);
+    mbar_init(&bar->q_empty, 2);
     for (int t = 0; t < 2; ++t) {
       mbar_init(&bar->s_full[t], 1);
       mbar_init(&bar->p_half[t], 128);
       mbar_init(&bar->p_full[t], 128);
       mbar_init(&bar->o_full[t], 1);
       mbar_init(&bar->o_empty[t], 128);
+      mbar_init(&bar->turn[t], 4);
     }
     for (int s = 0; s < kSlots; ++s) {
       mbar_init(&bar->slot_full[s], 1);
-      mbar_init(&bar->slot_empty[s], 1);
+      mbar_init(&bar->slot_empty[s], 2);
     }
     for (int i = 0; i < kMaskedRing; ++i) mbar_init(&bar->masked_full[i], 1);
     for (int i = 0; i < kWorkRing; ++i) {
@@ -152,7 +167,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&bar->work_empty[i], kWorkReaders);
     }
     mbar_init(&bar->next_full, 1);
-    mbar_init(&bar->drain, 1);
+    for (int t = 0; t < 2; ++t) mbar_init(&bar->drain[t], 1);
     fence_mbar_init();
   }
   __syncthreads();
@@ -174,7 +189,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   // First block of the item that some row of tile t does not see whole.
   auto masked_from = [&](const Work& w, int t) { return row_limit(w, t * tt, a.causal) / kBlock; };
 
-  if (warp == kSchedWarp) {
+  // The register split sits at the top of the two role branches (not before a
+  // join), so each branch is compiled against its own budget.
+  if (warp >= kSoftWarps) {
+   setmaxnreg_dec<kControlRegs>();
+   if (warp == kSchedWarp) {
     // ------------------------------------------------------------ scheduler
     int64_t cta = blockIdx.x;
     uint32_t answers = 0;
@@ -223,7 +242,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       fence_proxy_async_smem();   // the answer is read before the next one is asked for
       __syncwarp();
     }
-  } else if (warp == kProducerWarp) {
+   } else if (warp == kProducerWarp) {
     // ------------------------------------------------------------ producer
     if (lane == 0) {
       uint32_t armed = 0, armed_phase = 0;
@@ -284,96 +303,100 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_wait(&bar->masked_full[j % kMaskedRing], (j / kMaskedRing) & 1, &never, a.err_word);
       if (loads) mbar_wait(&bar->q_full, (loads - 1) & 1, &never, a.err_word);
     }
-  } else if (warp == kMmaWarp) {
-    // ------------------------------------------------------------ MMA issuer
+   } else if (warp == kMmaWarp || warp == kMmaWarp + 1) {
+    // ------------------------------------------------------------ MMA issuers
     if (lane == 0) {
+      const int t = warp - kMmaWarp;
       const uint32_t idesc_s = idesc_bf16_f32(128, kBlock, false);
       const uint32_t idesc_o = idesc_bf16_f32(128, kHeadDim, true);
       const uint64_t kdesc0 = sdesc_sw128(smem_u32(sRing), 16, 1024);
       const uint64_t vdesc0 = sdesc_sw128(smem_u32(sRing), kPanel, 1024);
-      const uint64_t qdesc0 = sdesc_sw128(smem_u32(sQ), 16, 1024);
-      int seq = 0, loads = 0;
-      int blocks[2] = {0, 0}, outs[2] = {0, 0};   // P consumed, O finished, of each tile
+      const uint64_t qdesc = sdesc_sw128(smem_u32(sQ + t * kSlotBytes), 16, 1024);
+      const uint32_t s_tmem = tmem + t * 128, o_tmem = tmem + 256 + t * 128;
+      int slot = 0, loads = 0;
+      uint32_t ring_phase = 0;
+      int blocks = 0, outs = 0;                // P consumed, O finished
       bool ok = true;
       auto wait = [&](uint64_t* b, uint32_t parity) {
-        ok = ok && mbar_wait(b, parity, abort_flag, a.err_word);
-        return ok;
+        return mbar_wait(b, parity, abort_flag, a.err_word);
+      };
+      // Next slot of the ring, once it is full.
+      auto next_slot = [&]() -> int {
+        const int s = slot;
+        ok = wait(&bar->slot_full[s], ring_phase);
+        if (++slot == kSlots) slot = 0, ring_phase ^= 1;
+        return s;
+      };
+      auto issue_s = [&](int s) {
+        const uint64_t kd = kdesc0 + static_cast<uint64_t>((s * kSlotBytes) >> 4);
+#pragma unroll
+        for (int kk = 0; kk < kHeadDim / 16; ++kk) {
+          const uint64_t off = static_cast<uint64_t>(((kk >> 2) * kPanel + (kk & 3) * 32) >> 4);
+          umma_bf16_ss(s_tmem, qdesc + off, kd + off, idesc_s, kk > 0 ? 1u : 0u);
+        }
+        umma_commit(&bar->s_full[t]);
+        umma_commit(&bar->slot_empty[s]);
       };
       for (int i = 0; ok; ++i) {
         const Item* it = item_at(i);
         if (it == nullptr) break;
-        const int nt[2] = {it->n[0], it->n[1]};
+        const int mine = it->n[t];
+        const int n = max(it->n[0], it->n[1]);
         done_with(i);
-        const int n = max(nt[0], nt[1]);
         if (n == 0) continue;
-        auto issue_s = [&](int t, int s) {
-          const uint64_t kd = kdesc0 + static_cast<uint64_t>((s * kSlotBytes) >> 4);
-          const uint64_t qd = qdesc0 + static_cast<uint64_t>((t * kSlotBytes) >> 4);
-#pragma unroll
-          for (int kk = 0; kk < kHeadDim / 16; ++kk) {
-            const uint64_t off = static_cast<uint64_t>(((kk >> 2) * kPanel + (kk & 3) * 32) >> 4);
-            umma_bf16_ss(tmem + t * 128, qd + off, kd + off, idesc_s, kk > 0 ? 1u : 0u);
-          }
-          umma_commit(&bar->s_full[t]);
-        };
-        int sk = seq % kSlots;
-        wait(&bar->slot_full[sk], (seq / kSlots) & 1);
-        ++seq;
-        wait(&bar->q_full, loads & 1);
+        // Blocks past this tile's last are only passed on (the other tile reads
+        // them): the slot is given back once it is full.
+        const int s0 = next_slot();
+        if (!ok || !(ok = wait(&bar->q_full, loads & 1))) break;
         ++loads;
-        if (!ok) break;
         tc_fence_after();
-        for (int t = 0; t < 2; ++t)
-          if (nt[t] > 0) issue_s(t, sk);
-        umma_commit(&bar->slot_empty[sk]);
-        if (n == 1) umma_commit(&bar->q_empty);
-        for (int j = 0; ok && j < n; ++j) {
-          // slots in load order: K_{j+1}, V_j
-          int sk1 = 0;
+        if (mine > 0) issue_s(s0); else mbar_arrive(&bar->slot_empty[s0]);
+        if (mine <= 1) umma_commit(&bar->q_empty);
+        for (int j = 0; j < n; ++j) {
+          int sk = 0;
           if (j + 1 < n) {
-            sk1 = seq % kSlots;
-            if (!wait(&bar->slot_full[sk1], (seq / kSlots) & 1)) break;
-            ++seq;
+            sk = next_slot();
+            if (!ok) break;
           }
-          const int sv = seq % kSlots;
-          if (!wait(&bar->slot_full[sv], (seq / kSlots) & 1)) break;
-          ++seq;
-          const uint64_t vd = vdesc0 + static_cast<uint64_t>((sv * kSlotBytes) >> 4);
-#pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            if (j >= nt[t] || !ok) continue;
-            // the first PV of an item overwrites the O that its softmax group stores
-            if (j == 0) wait(&bar->o_empty[t], (outs[t] & 1) ^ 1);
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              if (!wait(half ? &bar->p_full[t] : &bar->p_half[t], blocks[t] & 1)) break;
-              tc_fence_after();
-#pragma unroll
-              for (int kk = half * 4; kk < half * 4 + 4; ++kk)
-                umma_bf16_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8,
-                             vd + static_cast<uint64_t>((kk * 16 * 128) >> 4), idesc_o,
-                             (j > 0 || kk > 0) ? 1u : 0u);
-            }
-            if (!ok) continue;
-            ++blocks[t];
-            if (j + 1 < nt[t]) {
-              issue_s(t, sk1);
-            } else {
-              umma_commit(&bar->o_full[t]);
-              ++outs[t];
-            }
-          }
+          const int sv = next_slot();
           if (!ok) break;
+          if (j >= mine) {
+            if (j + 1 < n) mbar_arrive(&bar->slot_empty[sk]);
+            mbar_arrive(&bar->slot_empty[sv]);
+            continue;
+          }
+          // the first PV of an item overwrites the O that the softmax group stores
+          if (j == 0 && !(ok = wait(&bar->o_empty[t], (outs & 1) ^ 1))) break;
+          const uint64_t vd = vdesc0 + static_cast<uint64_t>((sv * kSlotBytes) >> 4);
+          if (!(ok = wait(&bar->p_half[t], blocks & 1))) break;
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            umma_bf16_ts(o_tmem, s_tmem + kk * 8, vd + static_cast<uint64_t>((kk * 16 * 128) >> 4),
+                         idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
+          if (!(ok = wait(&bar->p_full[t], blocks & 1))) break;
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 4; kk < 8; ++kk)
+            umma_bf16_ts(o_tmem, s_tmem + kk * 8, vd + static_cast<uint64_t>((kk * 16 * 128) >> 4),
+                         idesc_o, 1u);
+          ++blocks;
+          if (j + 1 < mine) {
+            issue_s(sk);
+            if (j + 2 == mine) umma_commit(&bar->q_empty);
+          } else {
+            umma_commit(&bar->o_full[t]);
+            ++outs;
+            if (j + 1 < n) mbar_arrive(&bar->slot_empty[sk]);
+          }
           umma_commit(&bar->slot_empty[sv]);
-          if (j + 1 < n) umma_commit(&bar->slot_empty[sk1]);
-          if (j + 2 == n) umma_commit(&bar->q_empty);
         }
       }
       int never = 0;
-      umma_commit(&bar->drain);
-      mbar_wait(&bar->drain, 0, &never, a.err_word);
+      umma_commit(&bar->drain[t]);
+      mbar_wait(&bar->drain[t], 0, &never, a.err_word);
     }
-  } else if (warp == kCheckWarp) {
+   } else if (warp == kCheckWarp) {
     // ------------------------------------------------------ masked V blocks
     int seq = 0, masked = 0;
     for (int i = 0;; ++i) {
@@ -402,7 +425,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) done_with(i);
     }
+   }
   } else {
+    setmaxnreg_inc<kSoftRegs>();
     // ------------------------------------------------------------ softmax
     const int t = warp >> 2;                   // this group's tile
     const int wq = warp & 3;
@@ -416,16 +441,29 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float2 c2 = make_float2(c, c);
     int blocks = 0, outs = 0;
     bool ok = true;
+    // The tiles take turns at the exponentials, tile 0 first: MUFU is the
+    // softmax's bound, and two tiles at it together would then also wait for
+    // the tensor pipe together.
+    uint32_t turn_phase = t ^ 1;
+    auto take_turn = [&]() -> bool {
+      const bool mine = mbar_wait(&bar->turn[t], turn_phase, abort_flag, a.err_word);
+      turn_phase ^= 1;
+      return __all_sync(0xffffffffu, mine);
+    };
+    auto pass_turn = [&]() {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar->turn[t ^ 1]);
+    };
     for (int i = 0; ok; ++i) {
       Item* it = item_at(i);
       if (!__all_sync(0xffffffffu, it != nullptr)) break;
       const Work w = it->w;
       const int n = t ? it->n[1] : it->n[0];
+      const int turns = max(it->n[0], it->n[1]);
       const int head = it->hk * G + head_in_group;
       const int from = masked_from(w, t);
       // rows past the tile's tokens x heads (row / G >= tt) belong to no query
       const int limit = row < tt * G ? row_limit(w, token, a.causal) : 0;
-      const bool row_valid = row < tt * G && token < w.tokens;
       const bool warp_active = wq * 32 < min(tt, w.tokens - t * tt) * G;
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < n; ++j) {
@@ -434,10 +472,24 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++blocks;
         tc_fence_after();
         if (warp_active) {
-          const bool partial = j >= from;
-          const int64_t valid = limit - j * kBlock;
-          uint32_t keep[2][32];
-          const float mrow = row_max<128, 2>(sbuf, partial, valid, keep) * c;
+          uint32_t r[4][32];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) tmem_ld_32x32b_x32(sbuf + k * 32, r[k]);
+          tmem_wait_ld();
+#pragma unroll
+          for (int k = 0; k < 4; ++k) reg_fence<32>(r[k]);
+          if (j >= from) {
+            const int64_t valid = limit - j * kBlock;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) mask_chunk(r[k], k * 32, valid);
+          }
+          float m8[8];
+#pragma unroll
+          for (int q = 0; q < 8; ++q) m8[q] = -INFINITY;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) max_chunk(m8, r[k]);
+          const float mrow = fmax3(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], m8[5]),
+                                   fmaxf(m8[6], m8[7])) * c;
           const bool need = mrow > m + kRescaleThreshold;
           const float m_used = need ? mrow : m;
           // O_t holds the blocks before j relative to m; PV(j - 1) is complete.
@@ -445,14 +497,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float f = need ? ex2_approx(m - m_used) : 1.f;
             l *= f;
 #pragma unroll 1
-            for (int cc = 0; cc < kHeadDim / 32; ++cc) {
-              uint32_t o[32];
-              tmem_ld_32x32b_x32(obuf + cc * 32, o);
+            for (int cc = 0; cc < kHeadDim / 16; ++cc) {
+              uint32_t o[16];
+              tmem_ld_32x32b_x16(obuf + cc * 16, o);
               tmem_wait_ld();
-              reg_fence<32>(o);
+              reg_fence<16>(o);
 #pragma unroll
-              for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
-              tmem_st_32x32b_x32(obuf + cc * 32, o);
+              for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+              tmem_st_32x32b_x16(obuf + cc * 16, o);
             }
           }
           m = m_used;
@@ -461,31 +513,31 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float2 neg_m = make_float2(neg, neg);
           float2 acc[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f),
                            make_float2(0.f, 0.f)};
-          uint32_t r[2][32];
-          tmem_ld_32x32b_x32(sbuf, r[0]);
-          tmem_wait_ld();
-          reg_fence<32>(r[0]);
-          tmem_ld_32x32b_x32(sbuf + 32, r[1]);
-          if (partial) mask_chunk(r[0], 0, valid);
+          if (!(ok = take_turn())) break;
           exp_chunk<kEmulated>(r[0], c2, neg_m, acc, sbuf);
-          tmem_wait_ld();
-          reg_fence<32>(r[1]);
-          if (partial) mask_chunk(r[1], 32, valid);
           exp_chunk<kEmulated>(r[1], c2, neg_m, acc, sbuf + 16);
           tmem_wait_st();
           tc_fence_before();
           mbar_arrive(&bar->p_half[t]);
-          exp_chunk<kEmulated>(keep[0], c2, neg_m, acc, sbuf + 32);
-          exp_chunk<kEmulated>(keep[1], c2, neg_m, acc, sbuf + 48);
+          exp_chunk<kEmulated>(r[2], c2, neg_m, acc, sbuf + 32);
+          exp_chunk<kEmulated>(r[3], c2, neg_m, acc, sbuf + 48);
+          pass_turn();
           const float2 sum = __fadd2_rn(__fadd2_rn(acc[0], acc[1]), __fadd2_rn(acc[2], acc[3]));
           l += sum.x + sum.y;
           tmem_wait_st();
           tc_fence_before();
           mbar_arrive(&bar->p_full[t]);
         } else {
+          if (!(ok = take_turn())) break;
+          pass_turn();
           mbar_arrive(&bar->p_half[t]);
           mbar_arrive(&bar->p_full[t]);
         }
+      }
+      // the turns of blocks that only the other tile sees
+      for (int j = n; ok && j < turns; ++j) {
+        ok = take_turn();
+        if (ok) pass_turn();
       }
       if (!ok) break;
       // ---------------------------------------------------------- epilogue
@@ -509,33 +561,49 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         mbar_arrive(&bar->o_empty[t]);
       } else {
+        // O goes out through shared memory: a thread owns a row, whose 16-byte
+        // pieces would each be a store of their own; staged, 8 lanes write 128
+        // bytes of a row.  (16 16-byte stores a thread took 9,000 cycles an item.)
         const float inv_l = l != 0.f ? 1.f / l : 0.f;
-        __nv_bfloat16* out = a.out + ((w.q0 + token) * a.heads + head) * kHeadDim;
+        const int64_t at = ((w.q0 + token) * a.heads + head) * kHeadDim;
+        const int rows = min(tt, w.tokens - t * tt) * G - wq * 32;   // of this warp
+        uint8_t* stage = smem + kStageOff + warp * kStageBytes;
 #pragma unroll
-        for (int cc = 0; cc < kHeadDim / 32; ++cc) {
-          uint32_t o[32];
+        for (int half = 0; half < 2; ++half) {
+          uint32_t o[2][32];
           if (n > 0 && warp_active) {
-            tmem_ld_32x32b_x32(obuf + cc * 32, o);
+            tmem_ld_32x32b_x32(obuf + half * 64, o[0]);
+            tmem_ld_32x32b_x32(obuf + half * 64 + 32, o[1]);
             tmem_wait_ld();
-            reg_fence<32>(o);
+            reg_fence<32>(o[0]);
+            reg_fence<32>(o[1]);
           } else {
 #pragma unroll
-            for (int x = 0; x < 32; ++x) o[x] = 0u;
+            for (int x = 0; x < 32; ++x) o[0][x] = o[1][x] = 0u;
           }
-          if (cc == kHeadDim / 32 - 1 && n > 0) {
+          if (half == 1 && n > 0) {
             tc_fence_before();
             mbar_arrive(&bar->o_empty[t]);     // O_t is in registers: its buffer is free
           }
-          if (row_valid) {
-            uint4* dst = reinterpret_cast<uint4*>(out + cc * 32);
 #pragma unroll
-            for (int x = 0; x < 4; ++x)
-              dst[x] = make_uint4(
-                  pack_bf16x2(__uint_as_float(o[8 * x]) * inv_l, __uint_as_float(o[8 * x + 1]) * inv_l),
-                  pack_bf16x2(__uint_as_float(o[8 * x + 2]) * inv_l, __uint_as_float(o[8 * x + 3]) * inv_l),
-                  pack_bf16x2(__uint_as_float(o[8 * x + 4]) * inv_l, __uint_as_float(o[8 * x + 5]) * inv_l),
-                  pack_bf16x2(__uint_as_float(o[8 * x + 6]) * inv_l, __uint_as_float(o[8 * x + 7]) * inv_l));
+          for (int x = 0; x < 8; ++x) {
+            const uint32_t* v = &o[x >> 2][(x & 3) * 8];
+            *reinterpret_cast<uint4*>(stage + sw128_offset(lane, x)) = make_uint4(
+                pack_bf16x2(__uint_as_float(v[0]) * inv_l, __uint_as_float(v[1]) * inv_l),
+                pack_bf16x2(__uint_as_float(v[2]) * inv_l, __uint_as_float(v[3]) * inv_l),
+                pack_bf16x2(__uint_as_float(v[4]) * inv_l, __uint_as_float(v[5]) * inv_l),
+                pack_bf16x2(__uint_as_float(v[6]) * inv_l, __uint_as_float(v[7]) * inv_l));
           }
+          __syncwarp();
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            const int r = x * 4 + (lane >> 3);
+            const int64_t dst = __shfl_sync(0xffffffffu, at, r);
+            if (r < rows)
+              *reinterpret_cast<uint4*>(a.out + dst + half * 64 + (lane & 7) * 8) =
+                  *reinterpret_cast<const uint4*>(stage + sw128_offset(r, lane & 7));
+          }
+          __syncwarp();
         }
       }
       __syncwarp();
@@ -566,6 +634,11 @@ cudaError_t launch_packed_tiles(const CUtensorMap& tq, const CUtensorMap& tk,
     if (e != cudaSuccess) return e;
     bytes = optin < kUsed + 1024 ? optin : kUsed + 1024;
     if (bytes < kUsed) return cudaErrorInvalidConfiguration;
+    // The register split assumes exactly kLaunchRegs a thread at launch.
+    cudaFuncAttributes attr{};
+    e = cudaFuncGetAttributes(&attr, packed_attention_tiles_kernel);
+    if (e != cudaSuccess) return e;
+    if (attr.numRegs != static_cast<int>(kLaunchRegs)) return cudaErrorInvalidConfiguration;
     e = cudaFuncSetAttribute(packed_attention_tiles_kernel,
                              cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) return e;
