@@ -14,21 +14,23 @@
 // store of the item before.  Items are found on the device (packed_common.cuh),
 // those late in their request first: under the causal mask they see the most
 // keys.
-//   warps 0-3, 4-7   softmax of tile 0, 1: one row a thread, all 128 scores in
-//               registers, log2 domain, a stabiliser that moves only past 2^8
-//               (then O_t is rescaled in TMEM), P_t as bf16 into the first 64
-//               columns of S_t
-//   warps 8, 9  MMA issuers, one thread for each tile t: for each block j,
-//               O_t += P_t V_j (each half of the keys as soon as its P is
-//               there), then S_t = Q_t K_{j+1}^T; warp 8 owns TMEM.  A tile has
-//               its own issuer so that it never waits for the other's softmax.
+//   warps 0-3, 4-7   softmax of tile 0, 1: 64 keys at a time, one row a thread,
+//               log2 domain, a stabiliser that moves only past 2^8 (then O_t is
+//               rescaled in TMEM), P as bf16 into the first half of S's columns
+//   warps 8, 9  MMA issuers, one thread for each tile t: for each 64 keys u,
+//               O_t += P_t(u) V(u), then S_t(u + 2) = Q_t K(u + 2)^T; warp 8
+//               owns TMEM.  A tile has its own issuer so that it never waits
+//               for the other's softmax.
 //   warp 10     TMA producer: Q; K/V blocks of 128 keys into a ring of 32 KB
 //               slots (K0, K1, V0, K2, V1, ...)
 //   warp 11     scheduler: cancels a pending CTA, looks its item up, publishes
 //   warp 12     cleans V of the masked blocks (clean_masked_values)
-// TMEM: S_0 [0, 128), S_1 [128, 256), O_0 [256, 384), O_1 [384, 512).  S_t(j+1)
-// follows O_t += P_t V_j in the issue order of one thread, which is what lets
-// P_t live in S_t's columns and makes s_full mean that PV is complete.
+// TMEM: tile t's two S buffers of 64 columns at 128 t, O_t at 256 + 128 t.
+// Two buffers of 64 keys, not one of 128: P lives in S's columns, so S of the
+// next keys waits for PV, and with one buffer the softmax waited for both (1,300
+// of 3,700 cycles a block); with two it runs while the other's PV and S do.
+// (S of 64 keys reads Q from shared memory twice as often: 1.5 times the time
+// of one product of 128, still under the softmax's.)
 //
 // A value of V that is not finite at a key which part of the item must not see
 // (causal) cannot be kept out of those rows by P = 0; warp 11 looks for one
@@ -47,18 +49,12 @@ using namespace attn;
 using namespace packed;
 
 constexpr int kSoftWarps = 8;
-constexpr int kThreads = 512;
+constexpr int kThreads = 416;
 constexpr int kMmaWarp = 8;             // and 9
 constexpr int kProducerWarp = 10;
 constexpr int kSchedWarp = 11;
 constexpr int kCheckWarp = 12;
-// The two control warpgroups give registers to the two softmax warpgroups,
-// within the launch's total.
-constexpr uint32_t kLaunchRegs = 128;
-constexpr uint32_t kSoftRegs = 200;
-constexpr uint32_t kControlRegs = 56;
-static_assert(256 * kSoftRegs + 256 * kControlRegs <= kThreads * kLaunchRegs,
-              "register split must stay within the launch total");
+constexpr int kSub = 64;                // keys of an S buffer
 constexpr int kSlots = 4;
 constexpr int kMaskedRing = 4;          // masked V blocks between the producer and warp 11
 #ifndef BSA_PACKED_EMULATED
@@ -77,19 +73,18 @@ constexpr int kBarOff = kStageOff + kSoftWarps * kStageBytes;
 struct Item {
   Work w;              // w.tokens < 0: no more items
   int hk;              // key head
-  int n[2];            // key blocks of each tile
+  int n[2];            // 64-key sub-blocks of each tile
   int exact;           // set by warp 11
 };
 
 struct Barriers {
   uint64_t q_full, q_empty;
-  uint64_t s_full[2];
-  uint64_t p_half[2], p_full[2];
+  uint64_t s_full[2][2], p_full[2][2];  // [tile][S buffer]
+  uint64_t pv_done[2];
   uint64_t o_full[2], o_empty[2];
   uint64_t slot_full[kSlots], slot_empty[kSlots];
   uint64_t masked_full[kMaskedRing];    // V of a masked block, before warp 11
   uint64_t work_full[kWorkRing], work_empty[kWorkRing];
-  uint64_t turn[2];                     // the other tile's exponentials are done
   uint64_t next_full;                   // answer of the cluster launch control
   uint64_t drain[2];
   uint32_t tmem_base;
@@ -150,12 +145,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&bar->q_full, 1);
     mbar_init(&bar->q_empty, 2);
     for (int t = 0; t < 2; ++t) {
-      mbar_init(&bar->s_full[t], 1);
-      mbar_init(&bar->p_half[t], 128);
-      mbar_init(&bar->p_full[t], 128);
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(&bar->s_full[t][b], 1);
+        mbar_init(&bar->p_full[t][b], 128);
+      }
+      mbar_init(&bar->pv_done[t], 1);
       mbar_init(&bar->o_full[t], 1);
       mbar_init(&bar->o_empty[t], 128);
-      mbar_init(&bar->turn[t], 4);
     }
     for (int s = 0; s < kSlots; ++s) {
       mbar_init(&bar->slot_full[s], 1);
@@ -189,10 +185,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   // First block of the item that some row of tile t does not see whole.
   auto masked_from = [&](const Work& w, int t) { return row_limit(w, t * tt, a.causal) / kBlock; };
 
-  // The register split sits at the top of the two role branches (not before a
-  // join), so each branch is compiled against its own budget.
+  // Blocks of 128 keys of an item: both tiles'.
+  auto item_blocks = [&](const Item* it) { return (max(it->n[0], it->n[1]) + 1) / 2; };
+
   if (warp >= kSoftWarps) {
-   setmaxnreg_dec<kControlRegs>();
    if (warp == kSchedWarp) {
     // ------------------------------------------------------------ scheduler
     int64_t cta = blockIdx.x;
@@ -212,7 +208,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (it.w.tokens != 0) {
         for (int t = 0; t < 2; ++t) {
           const int last = min(it.w.tokens, (t + 1) * tt) - 1;
-          it.n[t] = last < t * tt ? 0 : (row_limit(it.w, last, a.causal) + kBlock - 1) / kBlock;
+          it.n[t] = last < t * tt ? 0 : (row_limit(it.w, last, a.causal) + kSub - 1) / kSub;
         }
         bool ok = true;
         if (lane == 0) {
@@ -253,7 +249,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (it == nullptr) break;
         const Work w = it->w;
         const int hk = it->hk;
-        const int n = max(it->n[0], it->n[1]);
+        const int n = item_blocks(it);
         done_with(i);
         const int from = masked_from(w, 0);
         auto load = [&](const CUtensorMap* tm, int j, bool is_v) {
@@ -307,7 +303,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ------------------------------------------------------------ MMA issuers
     if (lane == 0) {
       const int t = warp - kMmaWarp;
-      const uint32_t idesc_s = idesc_bf16_f32(128, kBlock, false);
+      const uint32_t idesc_s = idesc_bf16_f32(128, kSub, false);
       const uint32_t idesc_o = idesc_bf16_f32(128, kHeadDim, true);
       const uint64_t kdesc0 = sdesc_sw128(smem_u32(sRing), 16, 1024);
       const uint64_t vdesc0 = sdesc_sw128(smem_u32(sRing), kPanel, 1024);
@@ -315,7 +311,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t s_tmem = tmem + t * 128, o_tmem = tmem + 256 + t * 128;
       int slot = 0, loads = 0;
       uint32_t ring_phase = 0;
-      int blocks = 0, outs = 0;                // P consumed, O finished
+      uint32_t scored = 0, used = 0, outs = 0;   // S issued, P consumed, O finished
       bool ok = true;
       auto wait = [&](uint64_t* b, uint32_t parity) {
         return mbar_wait(b, parity, abort_flag, a.err_word);
@@ -327,69 +323,69 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (++slot == kSlots) slot = 0, ring_phase ^= 1;
         return s;
       };
-      auto issue_s = [&](int s) {
-        const uint64_t kd = kdesc0 + static_cast<uint64_t>((s * kSlotBytes) >> 4);
+      // S of keys 64 half .. of the K block in slot s, into the next buffer.
+      auto issue_s = [&](int s, int half) {
+        const uint64_t kd = kdesc0 + static_cast<uint64_t>((s * kSlotBytes + half * kSub * 128) >> 4);
+        const uint32_t b = scored & 1;
 #pragma unroll
         for (int kk = 0; kk < kHeadDim / 16; ++kk) {
           const uint64_t off = static_cast<uint64_t>(((kk >> 2) * kPanel + (kk & 3) * 32) >> 4);
-          umma_bf16_ss(s_tmem, qdesc + off, kd + off, idesc_s, kk > 0 ? 1u : 0u);
+          umma_bf16_ss(s_tmem + b * kSub, qdesc + off, kd + off, idesc_s, kk > 0 ? 1u : 0u);
         }
-        umma_commit(&bar->s_full[t]);
-        umma_commit(&bar->slot_empty[s]);
+        umma_commit(&bar->s_full[t][b]);
+        ++scored;
       };
       for (int i = 0; ok; ++i) {
         const Item* it = item_at(i);
         if (it == nullptr) break;
-        const int mine = it->n[t];
-        const int n = max(it->n[0], it->n[1]);
+        const int mine = it->n[t];               // sub-blocks
+        const int n = item_blocks(it);
         done_with(i);
         if (n == 0) continue;
         // Blocks past this tile's last are only passed on (the other tile reads
         // them): the slot is given back once it is full.
-        const int s0 = next_slot();
+        int sk = next_slot();
         if (!ok || !(ok = wait(&bar->q_full, loads & 1))) break;
         ++loads;
         tc_fence_after();
-        if (mine > 0) issue_s(s0); else mbar_arrive(&bar->slot_empty[s0]);
-        if (mine <= 1) umma_commit(&bar->q_empty);
-        for (int j = 0; j < n; ++j) {
-          int sk = 0;
+        if (mine > 0) issue_s(sk, 0);
+        if (mine > 1) issue_s(sk, 1);
+        umma_commit(&bar->slot_empty[sk]);
+        if (mine <= 2) umma_commit(&bar->q_empty);
+        for (int j = 0; ok && j < n; ++j) {
           if (j + 1 < n) {
             sk = next_slot();
             if (!ok) break;
           }
           const int sv = next_slot();
           if (!ok) break;
-          if (j >= mine) {
-            if (j + 1 < n) mbar_arrive(&bar->slot_empty[sk]);
-            mbar_arrive(&bar->slot_empty[sv]);
-            continue;
-          }
-          // the first PV of an item overwrites the O that the softmax group stores
-          if (j == 0 && !(ok = wait(&bar->o_empty[t], (outs & 1) ^ 1))) break;
           const uint64_t vd = vdesc0 + static_cast<uint64_t>((sv * kSlotBytes) >> 4);
-          if (!(ok = wait(&bar->p_half[t], blocks & 1))) break;
-          tc_fence_after();
+#pragma unroll 1
+          for (int half = 0; half < 2; ++half) {
+            const int u = 2 * j + half;
+            if (u >= mine) break;
+            // the first PV of an item overwrites the O that the softmax group stores
+            if (u == 0 && !(ok = wait(&bar->o_empty[t], (outs & 1) ^ 1))) break;
+            const uint32_t b = used & 1;
+            if (!(ok = wait(&bar->p_full[t][b], (used >> 1) & 1))) break;
+            tc_fence_after();
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            umma_bf16_ts(o_tmem, s_tmem + kk * 8, vd + static_cast<uint64_t>((kk * 16 * 128) >> 4),
-                         idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
-          if (!(ok = wait(&bar->p_full[t], blocks & 1))) break;
-          tc_fence_after();
-#pragma unroll
-          for (int kk = 4; kk < 8; ++kk)
-            umma_bf16_ts(o_tmem, s_tmem + kk * 8, vd + static_cast<uint64_t>((kk * 16 * 128) >> 4),
-                         idesc_o, 1u);
-          ++blocks;
-          if (j + 1 < mine) {
-            issue_s(sk);
-            if (j + 2 == mine) umma_commit(&bar->q_empty);
-          } else {
-            umma_commit(&bar->o_full[t]);
-            ++outs;
-            if (j + 1 < n) mbar_arrive(&bar->slot_empty[sk]);
+            for (int kk = 0; kk < kSub / 16; ++kk)
+              umma_bf16_ts(o_tmem, s_tmem + b * kSub + kk * 8,
+                           vd + static_cast<uint64_t>(((half * kSub + kk * 16) * 128) >> 4), idesc_o,
+                           (u > 0 || kk > 0) ? 1u : 0u);
+            umma_commit(&bar->pv_done[t]);
+            ++used;
+            if (u + 1 == mine) {
+              umma_commit(&bar->o_full[t]);
+              ++outs;
+            }
+            if (u + 2 < mine) issue_s(sk, half);
+            if (u + 3 == mine) umma_commit(&bar->q_empty);
           }
+          if (!ok) break;
           umma_commit(&bar->slot_empty[sv]);
+          if (j + 1 < n) umma_commit(&bar->slot_empty[sk]);
         }
       }
       int never = 0;
@@ -403,7 +399,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       Item* it = item_at(i);
       if (!__all_sync(0xffffffffu, it != nullptr)) break;
       const Work w = it->w;
-      const int n = max(it->n[0], it->n[1]);
+      const int n = item_blocks(it);
       bool ok = true;
       for (int j = masked_from(w, 0); ok && j < n; ++j) {
         ok = mbar_wait(&bar->masked_full[masked % kMaskedRing], (masked / kMaskedRing) & 1, abort_flag,
@@ -427,7 +423,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
    }
   } else {
-    setmaxnreg_inc<kSoftRegs>();
     // ------------------------------------------------------------ softmax
     const int t = warp >> 2;                   // this group's tile
     const int wq = warp & 3;
@@ -439,62 +434,51 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int head_in_group = row - row / G * G;
     const float c = a.scale * kLog2e;
     const float2 c2 = make_float2(c, c);
-    int blocks = 0, outs = 0;
+    uint32_t seen = 0, outs = 0;               // sub-blocks, outputs
     bool ok = true;
-    // The tiles take turns at the exponentials, tile 0 first: MUFU is the
-    // softmax's bound, and two tiles at it together would then also wait for
-    // the tensor pipe together.
-    uint32_t turn_phase = t ^ 1;
-    auto take_turn = [&]() -> bool {
-      const bool mine = mbar_wait(&bar->turn[t], turn_phase, abort_flag, a.err_word);
-      turn_phase ^= 1;
-      return __all_sync(0xffffffffu, mine);
-    };
-    auto pass_turn = [&]() {
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bar->turn[t ^ 1]);
-    };
     for (int i = 0; ok; ++i) {
       Item* it = item_at(i);
       if (!__all_sync(0xffffffffu, it != nullptr)) break;
       const Work w = it->w;
       const int n = t ? it->n[1] : it->n[0];
-      const int turns = max(it->n[0], it->n[1]);
       const int head = it->hk * G + head_in_group;
-      const int from = masked_from(w, t);
+      const int from = row_limit(w, t * tt, a.causal) / kSub;   // first sub-block not seen whole
       // rows past the tile's tokens x heads (row / G >= tt) belong to no query
       const int limit = row < tt * G ? row_limit(w, token, a.causal) : 0;
       const bool warp_active = wq * 32 < min(tt, w.tokens - t * tt) * G;
       float m = -INFINITY, l = 0.f;
-      for (int j = 0; j < n; ++j) {
-        ok = mbar_wait(&bar->s_full[t], blocks & 1, abort_flag, a.err_word);
+      for (int u = 0; u < n; ++u, ++seen) {
+        const uint32_t b = seen & 1;
+        ok = mbar_wait(&bar->s_full[t][b], (seen >> 1) & 1, abort_flag, a.err_word);
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-        ++blocks;
         tc_fence_after();
         if (warp_active) {
-          uint32_t r[4][32];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) tmem_ld_32x32b_x32(sbuf + k * 32, r[k]);
+          const uint32_t buf = sbuf + b * kSub;
+          uint32_t r[2][32];
+          tmem_ld_32x32b_x32(buf, r[0]);
+          tmem_ld_32x32b_x32(buf + 32, r[1]);
           tmem_wait_ld();
-#pragma unroll
-          for (int k = 0; k < 4; ++k) reg_fence<32>(r[k]);
-          if (j >= from) {
-            const int64_t valid = limit - j * kBlock;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) mask_chunk(r[k], k * 32, valid);
+          reg_fence<32>(r[0]);
+          reg_fence<32>(r[1]);
+          if (u >= from) {
+            const int64_t valid = limit - u * kSub;
+            mask_chunk(r[0], 0, valid);
+            mask_chunk(r[1], 32, valid);
           }
           float m8[8];
 #pragma unroll
           for (int q = 0; q < 8; ++q) m8[q] = -INFINITY;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) max_chunk(m8, r[k]);
+          max_chunk(m8, r[0]);
+          max_chunk(m8, r[1]);
           const float mrow = fmax3(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], m8[5]),
                                    fmaxf(m8[6], m8[7])) * c;
           const bool need = mrow > m + kRescaleThreshold;
-          const float m_used = need ? mrow : m;
-          // O_t holds the blocks before j relative to m; PV(j - 1) is complete.
-          if (j > 0 && __any_sync(0xffffffffu, need)) {
-            const float f = need ? ex2_approx(m - m_used) : 1.f;
+          if (u > 0 && __any_sync(0xffffffffu, need)) {
+            // O_t holds the keys before these relative to m, once their PV is complete.
+            ok = mbar_wait(&bar->pv_done[t], (seen - 1) & 1, abort_flag, a.err_word);
+            if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+            tc_fence_after();
+            const float f = need ? ex2_approx(m - mrow) : 1.f;
             l *= f;
 #pragma unroll 1
             for (int cc = 0; cc < kHeadDim / 16; ++cc) {
@@ -507,37 +491,20 @@ __global__ void __launch_bounds__(kThreads, 1)
               tmem_st_32x32b_x16(obuf + cc * 16, o);
             }
           }
-          m = m_used;
+          if (need) m = mrow;
           // -inf stands for "no key yet": the exponents (all -inf) are taken against 0.
           const float neg = m == -INFINITY ? 0.f : -m;
           const float2 neg_m = make_float2(neg, neg);
           float2 acc[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f),
                            make_float2(0.f, 0.f)};
-          if (!(ok = take_turn())) break;
-          exp_chunk<kEmulated>(r[0], c2, neg_m, acc, sbuf);
-          exp_chunk<kEmulated>(r[1], c2, neg_m, acc, sbuf + 16);
-          tmem_wait_st();
-          tc_fence_before();
-          mbar_arrive(&bar->p_half[t]);
-          exp_chunk<kEmulated>(r[2], c2, neg_m, acc, sbuf + 32);
-          exp_chunk<kEmulated>(r[3], c2, neg_m, acc, sbuf + 48);
-          pass_turn();
+          exp_chunk<kEmulated>(r[0], c2, neg_m, acc, buf);
+          exp_chunk<kEmulated>(r[1], c2, neg_m, acc, buf + 16);
           const float2 sum = __fadd2_rn(__fadd2_rn(acc[0], acc[1]), __fadd2_rn(acc[2], acc[3]));
           l += sum.x + sum.y;
           tmem_wait_st();
           tc_fence_before();
-          mbar_arrive(&bar->p_full[t]);
-        } else {
-          if (!(ok = take_turn())) break;
-          pass_turn();
-          mbar_arrive(&bar->p_half[t]);
-          mbar_arrive(&bar->p_full[t]);
         }
-      }
-      // the turns of blocks that only the other tile sees
-      for (int j = n; ok && j < turns; ++j) {
-        ok = take_turn();
-        if (ok) pass_turn();
+        mbar_arrive(&bar->p_full[t][b]);
       }
       if (!ok) break;
       // ---------------------------------------------------------- epilogue
@@ -634,11 +601,6 @@ cudaError_t launch_packed_tiles(const CUtensorMap& tq, const CUtensorMap& tk,
     if (e != cudaSuccess) return e;
     bytes = optin < kUsed + 1024 ? optin : kUsed + 1024;
     if (bytes < kUsed) return cudaErrorInvalidConfiguration;
-    // The register split assumes exactly kLaunchRegs a thread at launch.
-    cudaFuncAttributes attr{};
-    e = cudaFuncGetAttributes(&attr, packed_attention_tiles_kernel);
-    if (e != cudaSuccess) return e;
-    if (attr.numRegs != static_cast<int>(kLaunchRegs)) return cudaErrorInvalidConfiguration;
     e = cudaFuncSetAttribute(packed_attention_tiles_kernel,
                              cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) return e;
