@@ -7,6 +7,7 @@ when it is missing or when a call fails; there is no CPU substitute.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 import threading
 from pathlib import Path
@@ -14,6 +15,7 @@ from pathlib import Path
 import torch
 
 LIBRARY_PATH = Path(__file__).resolve().with_name("libbsa.so")
+BINDING_PATH = LIBRARY_PATH.with_name("_binding.so")
 
 # Entry points and their C signatures (include/bsa.h).
 _I32, _I64, _F32 = ctypes.c_int32, ctypes.c_int64, ctypes.c_float
@@ -73,6 +75,7 @@ DEVICE_ERRORS = {
 
 _lock = threading.Lock()
 _lib = None
+_binding = None
 _err_words: dict = {}
 
 
@@ -102,6 +105,26 @@ def load_library(path: Path | None = None) -> ctypes.CDLL:
         return lib
 
 
+def load_binding():
+    """The compiled calls of the packed operators (``_binding.so``, csrc/binding.cpp)."""
+    global _binding
+    if _binding is None:
+        lib = load_library()
+        if not BINDING_PATH.exists():
+            raise RuntimeError(
+                f"{BINDING_PATH} is missing: build it with `python -m dit_sparse_atten_b200.csrc.build`")
+        spec = importlib.util.spec_from_file_location(__package__ + "._binding", BINDING_PATH)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        module.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
+            "bsa_last_error", "bsa_residual_norm", "bsa_lora_add_workspace_bytes", "bsa_lora_add",
+            "bsa_packed_attention_workspace_bytes", "bsa_packed_attention")))
+        for device, word in _err_words.items():
+            module.set_err_word(device, word.data_ptr())
+        _binding = module
+    return _binding
+
+
 def call(name: str, *args) -> None:
     """Call an entry point; raise ``RuntimeError`` with its message on failure."""
     lib = load_library()
@@ -127,6 +150,8 @@ def err_word(device: torch.device) -> torch.Tensor:
     if word is None:
         word = torch.zeros(1, dtype=torch.int32, device=device)
         _err_words[key] = word
+        if _binding is not None:
+            _binding.set_err_word(key, word.data_ptr())
     return word
 
 

@@ -1,8 +1,9 @@
-"""Build ``libbsa.so`` (the C ABI of include/bsa.h) for sm_100a with nvcc.
+"""Build ``libbsa.so`` (the C ABI of include/bsa.h) for sm_100a with nvcc, and
+``_binding.so`` (binding.cpp: the packed operators' calls from torch) with g++.
 
 Usage: ``python -m dit_sparse_atten_b200.csrc.build [--verbose-ptxas]``.
-The library is written next to the package (``dit_sparse_atten_b200/libbsa.so``)
-so it travels with the source tree; it is rebuilt only when a source is newer.
+Both are written next to the package (``dit_sparse_atten_b200/libbsa.so``) so
+they travel with the source tree; each is rebuilt only when a source is newer.
 """
 
 from __future__ import annotations
@@ -19,6 +20,7 @@ CSRC = Path(__file__).resolve().parent
 PACKAGE = CSRC.parent
 REPO = PACKAGE.parent
 LIBRARY = PACKAGE / "libbsa.so"
+BINDING = PACKAGE / "_binding.so"
 SOURCES = sorted(CSRC.glob("*.cu"))
 HEADERS = sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + [REPO / "include" / "bsa.h"]
 
@@ -73,13 +75,41 @@ def build(force: bool = False, verbose_ptxas: bool = False) -> Path:
     return LIBRARY
 
 
+def binding_up_to_date() -> bool:
+    sources = [CSRC / "binding.cpp", REPO / "include" / "bsa.h", Path(__file__)]
+    return BINDING.exists() and all(p.stat().st_mtime <= BINDING.stat().st_mtime for p in sources)
+
+
+def build_binding(force: bool = False) -> Path:
+    """``_binding.so``; the entry points of ``libbsa.so`` are handed to it at run time."""
+    if not force and binding_up_to_date():
+        return BINDING
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    includes = cpp_extension.include_paths("cuda") + [sysconfig.get_paths()["include"]]
+    torch_lib = str(Path(torch.__file__).resolve().parent / "lib")
+    tmp = BINDING.with_suffix(".so.tmp")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *[f"-I{p}" for p in includes], str(CSRC / "binding.cpp"), "-o", str(tmp),
+           f"-L{torch_lib}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    done = subprocess.run(cmd, capture_output=True, text=True)
+    sys.stderr.write(done.stderr)
+    done.check_returncode()
+    os.replace(tmp, BINDING)
+    return BINDING
+
+
 def main(argv=None) -> int:
     parser = argparse.ArgumentParser(description=__doc__)
     parser.add_argument("--force", action="store_true")
     parser.add_argument("--verbose-ptxas", action="store_true")
     args = parser.parse_args(argv)
-    path = build(force=args.force, verbose_ptxas=args.verbose_ptxas)
-    print(path)
+    print(build(force=args.force, verbose_ptxas=args.verbose_ptxas))
+    print(build_binding(force=args.force))
     return 0
 
 

@@ -30,8 +30,7 @@ namespace {
 
 constexpr int kFewRows = 8;        // rows a tile, requests of few rows
 constexpr int kTileRows = 128;     // rows a tile, tensor-core shrink
-constexpr int kExpandRows = 64;
-constexpr int kExpandCols = 256;
+constexpr int kExpandRows = 16;    // rows a tile, expand of requests of few rows
 constexpr int kWarps = 8;
 constexpr int kMaxSlices = 8;      // portable cluster size
 
@@ -311,16 +310,15 @@ __global__ void __launch_bounds__(kShrinkThreads)
   join_slices(a, t, part, kPad, kPartStride, adapter_scale(a, t.adapter));
 }
 
-// out = y + u B^T: each warp owns 32 columns at a time, holds their B
-// fragments in registers and goes down the tile's rows 16 at a time.  Product
-// column n of n-tile j stands for column 8 (n / 2) + 2 j + n % 2 of the 32, so
-// that a thread's 4 x 2 results are 8 consecutive columns: y and out move as
-// 16-byte accesses without a detour through shared memory, and u's rows are
-// the A fragments as they lie (k permuted as in lora_shrink_few_kernel).
-// kAhead row tiles of y are requested before the first product.
-template <int KB, int kAhead>
-__global__ void __launch_bounds__(kWarps * 32, 2) lora_expand_kernel(const LoraArgs a) {
-  constexpr int kTiles = kExpandRows / 16;
+// Expand for requests of few rows: out = y + u B^T for 16 rows of one request
+// and kGroups x 32 columns a warp.  Product column n of n-tile j stands for
+// column 8 (n / 2) + 2 j + n % 2 of the 32, so that a thread's 4 x 2 results
+// are 8 consecutive columns: y and out move as 16-byte accesses, and u's rows
+// are the A fragments as they lie (k permuted as in lora_shrink_few_kernel).
+// All loads of y and B are requested before the wait for u: a CTA lives for
+// little more than one memory latency, which is what bounds this kernel.
+template <int KB, int kGroups>
+__global__ void __launch_bounds__(kWarps * 32) lora_expand_few_kernel(const LoraArgs a) {
   const int64_t slot = blockIdx.x / a.col_ctas;
   const Tile t = find_tile<kExpandRows>(a, slot);
   if (t.rows == 0) return;
@@ -329,77 +327,66 @@ __global__ void __launch_bounds__(kWarps * 32, 2) lora_expand_kernel(const LoraA
   const bool has = t.adapter >= 0;
   const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
   const __nv_bfloat16* lb = a.lora_b + (has ? static_cast<int64_t>(t.adapter) * a.n * a.rank : 0);
-  bool waited = false;
-  for (int c0 = static_cast<int>(blockIdx.x % a.col_ctas) * kExpandCols + warp * 32; c0 < a.n;
-       c0 += a.col_ctas * kExpandCols) {
-    const int col = c0 + 8 * q;                  // this thread's 8 columns
-    const bool col_in = col < a.n;
-    auto load_y = [&](int tile, int half) {
-      const int row = tile * 16 + g + 8 * half;
-      return row < t.rows && col_in
-          ? *reinterpret_cast<const uint4*>(a.y + (t.row + row) * a.y_stride + col) : zero;
-    };
-    uint4 y[kAhead][2];
+  const int c0 = (static_cast<int>(blockIdx.x % a.col_ctas) * kWarps + warp) * 32 * kGroups;
+  uint4 y[kGroups][2], b[kGroups][KB][4];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) y[i][0] = load_y(i, 0), y[i][1] = load_y(i, 1);
-    uint4 b[KB][4];
+  for (int i = 0; i < kGroups; ++i) {
+    const int col = c0 + i * 32 + 8 * q;         // this thread's 8 columns
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int row = g + 8 * half;
+      y[i][half] = row < t.rows && col < a.n
+          ? *reinterpret_cast<const uint4*>(a.y + (t.row + row) * a.y_stride + col) : zero;
+    }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int c = c0 + 8 * (g >> 1) + 2 * j + (g & 1);
+      const int c = c0 + i * 32 + 8 * (g >> 1) + 2 * j + (g & 1);
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) {
         const int k = kb * 32 + q * 8;
-        b[kb][j] = has && c < a.n && k < a.rank
+        b[i][kb][j] = has && c < a.n && k < a.rank
             ? __ldg(reinterpret_cast<const uint4*>(lb + static_cast<int64_t>(c) * a.rank + k)) : zero;
       }
     }
-    if (!waited) {
-      pdl_wait();                                // u
-      waited = true;
+  }
+  pdl_wait();                                    // u
+  uint4 w[KB][2];
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int row = g + 8 * half;
+      w[kb][half] = has && row < t.rows
+          ? *reinterpret_cast<const uint4*>(a.workspace + (t.row + row) * a.rank_pad + kb * 32 + q * 8)
+          : zero;
     }
 #pragma unroll
-    for (int tile = 0; tile < kTiles; ++tile) {
-      if (tile * 16 >= t.rows) break;
-      float d[4][4];
+  for (int i = 0; i < kGroups; ++i) {
+    float d[4][4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < 4; ++j) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) d[j][e] = 0.f;
+      for (int e = 0; e < 4; ++e) d[j][e] = 0.f;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        mma_bf16(d[j], w[kb][0].x, w[kb][1].x, w[kb][0].y, w[kb][1].y, b[i][kb][j].x, b[i][kb][j].y);
+        mma_bf16(d[j], w[kb][0].z, w[kb][1].z, w[kb][0].w, w[kb][1].w, b[i][kb][j].z, b[i][kb][j].w);
+      }
+    }
+    const int col = c0 + i * 32 + 8 * q;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int row = g + 8 * half;
+      if (row >= t.rows || col >= a.n) continue;
+      uint32_t v[4] = {y[i][half].x, y[i][half].y, y[i][half].z, y[i][half].w};
       if (has) {
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
-          uint4 w[2];
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const int row = tile * 16 + g + 8 * half;
-            w[half] = row < t.rows
-                ? *reinterpret_cast<const uint4*>(a.workspace + (t.row + row) * a.rank_pad + kb * 32 + q * 8)
-                : zero;
-          }
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            mma_bf16(d[j], w[0].x, w[1].x, w[0].y, w[1].y, b[kb][j].x, b[kb][j].y);
-            mma_bf16(d[j], w[0].z, w[1].z, w[0].w, w[1].w, b[kb][j].z, b[kb][j].w);
-          }
-        }
+        for (int j = 0; j < 4; ++j)
+          v[j] = pack_bf16x2(__uint_as_float(v[j] << 16) + d[j][2 * half],
+                             __uint_as_float(v[j] & 0xffff0000u) + d[j][2 * half + 1]);
       }
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int row = tile * 16 + g + 8 * half;
-        const uint4 in = y[tile % kAhead][half];
-        if (tile + kAhead < kTiles) y[tile % kAhead][half] = load_y(tile + kAhead, half);
-        if (row < t.rows && col_in) {
-          uint32_t w[4] = {in.x, in.y, in.z, in.w};
-          if (has) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              w[j] = pack_bf16x2(__uint_as_float(w[j] << 16) + d[j][2 * half],
-                                 __uint_as_float(w[j] & 0xffff0000u) + d[j][2 * half + 1]);
-          }
-          *reinterpret_cast<uint4*>(a.out + (t.row + row) * a.out_stride + col) =
-              make_uint4(w[0], w[1], w[2], w[3]);
-        }
-      }
+      *reinterpret_cast<uint4*>(a.out + (t.row + row) * a.out_stride + col) =
+          make_uint4(v[0], v[1], v[2], v[3]);
     }
   }
 }
@@ -801,17 +788,16 @@ cudaError_t launch_lora_add(const LoraMaps& maps, LoraArgs a, cudaStream_t strea
     else if (groups <= 4) e = launch_sliced(lora_shrink_few_kernel<4>, grid, threads, 0, a.slices, stream, a);
     else e = launch_sliced(lora_shrink_few_kernel<8>, grid, threads, 0, a.slices, stream, a);
     if (e != cudaSuccess) return e;
-    // Column CTAs a row tile: one for each 256 columns, fewer (each going over
-    // several) once that gives eight CTAs an SM.
-    const int64_t slots = a.rows / kExpandRows + a.requests;
-    const int64_t cols = (a.n + kExpandCols - 1) / kExpandCols;
-    a.col_ctas = static_cast<int32_t>(std::min<int64_t>(cols, (8ll * num_sms + slots - 1) / slots));
-    const dim3 eg(static_cast<unsigned>(slots * a.col_ctas));
     const int kb = a.rank_pad / 32;
-    if (kb == 1) return launch_dependent(lora_expand_kernel<1, 4>, eg, threads, 0, stream, a);
-    if (kb == 2) return launch_dependent(lora_expand_kernel<2, 4>, eg, threads, 0, stream, a);
-    if (kb == 3) return launch_dependent(lora_expand_kernel<3, 2>, eg, threads, 0, stream, a);
-    return launch_dependent(lora_expand_kernel<4, 2>, eg, threads, 0, stream, a);
+    auto expand = [&](auto kernel, int columns) {
+      a.col_ctas = (a.n + kWarps * columns - 1) / (kWarps * columns);
+      const int64_t ctas = (a.rows / kExpandRows + a.requests) * a.col_ctas;
+      return launch_dependent(kernel, dim3(static_cast<unsigned>(ctas)), threads, 0, stream, a);
+    };
+    if (kb == 1) return expand(lora_expand_few_kernel<1, 4>, 128);
+    if (kb == 2) return expand(lora_expand_few_kernel<2, 2>, 64);
+    if (kb == 3) return expand(lora_expand_few_kernel<3, 1>, 32);
+    return expand(lora_expand_few_kernel<4, 1>, 32);
   }
   if (groups <= 1) e = launch_shrink<16>(maps.x, maps.a, a, grid, stream);
   else if (groups <= 2) e = launch_shrink<32>(maps.x, maps.a, a, grid, stream);

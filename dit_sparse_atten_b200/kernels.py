@@ -667,6 +667,12 @@ _DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _NORM_KINDS = {None: 0, "layer": 1, "rms": 2}
 
 
+def _call_on(device: torch.device, name: str, *args) -> None:
+    """``_native.call`` with ``device`` current (a launch goes to the current device)."""
+    with torch.cuda.device(device):
+        _native.call(name, *args, _native.err_word(device).data_ptr(), _stream(device))
+
+
 def _starts_i32(starts: torch.Tensor, name: str, device: torch.device) -> torch.Tensor:
     """Request offsets as contiguous int32 on ``device`` (``[requests + 1]``)."""
     if starts.dim() != 1 or starts.numel() < 1:
@@ -710,6 +716,13 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor | None = None, *,
     comes alone any of the three.  Modulated LayerNorm and gated residual of
     the reference's block: ``wan_diffusers.py:75-117``.
     """
+    if norm in _NORM_KINDS and post_norm in _NORM_KINDS and norm is not None:
+        done = _native.load_binding().residual_norm(
+            x, y, gate, shift, scale, weight, bias, post_weight, post_bias, row_starts,
+            _NORM_KINDS[norm], _NORM_KINDS[post_norm], eps,
+            -1 if normed_dtype is None else _DTYPE_CODES.get(normed_dtype, -2))
+        if done is not None:
+            return NormResult(*done)
     device = _require_cuda(x, y, gate, shift, scale, weight, bias, post_weight, post_bias)
     if x.dim() < 1 or x.dtype not in _DTYPE_CODES:
         raise ValueError("x must be [..., C] of bf16, fp16 or float32")
@@ -774,14 +787,13 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor | None = None, *,
     normed = torch.empty(x.shape, dtype=normed_dtype, device=device)
     if rows and C:
         p = _native.ptr
-        _native.call("bsa_residual_norm", xr.data_ptr(), _DTYPE_CODES[x.dtype], xr.stride(0),
-                     p(yr), _DTYPE_CODES[normed_dtype], yr.stride(0) if yr is not None else 0,
-                     rows, C, p(row_starts), requests, p(gate), gate_stride, p(shift),
-                     shift_stride, p(scale), scale_stride, mods, p(weight), p(bias), affine,
-                     p(post_weight), p(post_bias), post, _NORM_KINDS[norm],
-                     _NORM_KINDS[post_norm], float(eps),
-                     residual.data_ptr() if y is not None else None, normed.data_ptr(),
-                     _native.err_word(device).data_ptr(), _stream(device))
+        _call_on(device, "bsa_residual_norm", xr.data_ptr(), _DTYPE_CODES[x.dtype], xr.stride(0),
+                 p(yr), _DTYPE_CODES[normed_dtype], yr.stride(0) if yr is not None else 0,
+                 rows, C, p(row_starts), requests, p(gate), gate_stride, p(shift),
+                 shift_stride, p(scale), scale_stride, mods, p(weight), p(bias), affine,
+                 p(post_weight), p(post_bias), post, _NORM_KINDS[norm],
+                 _NORM_KINDS[post_norm], float(eps),
+                 residual.data_ptr() if y is not None else None, normed.data_ptr())
     return NormResult(residual, normed)
 
 
@@ -799,6 +811,9 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, lora_a: torch.Tensor, lora_b: tor
     (adapters of lower rank: pad both factors with zeros).  ``out``: an output
     to write, ``y`` itself included; by default a new tensor.
     """
+    done = _native.load_binding().lora_add(y, x, lora_a, lora_b, row_starts, adapters, scales, out)
+    if done is not None:
+        return done
     device = _require_cuda(y, x, lora_a, lora_b, scales, out)
     if any(t.dtype != torch.bfloat16 for t in (y, x, lora_a, lora_b)):
         raise ValueError("lora_add expects bf16 y, x, lora_a and lora_b")
@@ -843,11 +858,10 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, lora_a: torch.Tensor, lora_b: tor
         lora_a, lora_b = lora_a.contiguous(), lora_b.contiguous()
         nbytes = _native.load_library().bsa_lora_add_workspace_bytes(rows, requests, K, R)
         work = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        _native.call("bsa_lora_add", yr.data_ptr(), yr.stride(0), xr.data_ptr(), xr.stride(0),
-                     lora_a.data_ptr(), lora_b.data_ptr(), _native.ptr(scales),
-                     row_starts.data_ptr(), adapters.data_ptr(), rows, requests, count, K, N, R,
-                     work.data_ptr(), nbytes, o.data_ptr(), o.stride(0),
-                     _native.err_word(device).data_ptr(), _stream(device))
+        _call_on(device, "bsa_lora_add", yr.data_ptr(), yr.stride(0), xr.data_ptr(), xr.stride(0),
+                 lora_a.data_ptr(), lora_b.data_ptr(), _native.ptr(scales),
+                 row_starts.data_ptr(), adapters.data_ptr(), rows, requests, count, K, N, R,
+                 work.data_ptr(), nbytes, o.data_ptr(), o.stride(0))
     return out
 
 
@@ -863,6 +877,10 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_starts
     k_len - q_len`` of them (one new token: all of them).  A query without a
     key gives 0.  Returns bf16 ``[Tq, H, 128]``.
     """
+    done = _native.load_binding().packed_attention(
+        q, k, v, q_starts, k_starts, causal, HEAD_DIM ** -0.5 if scale is None else float(scale))
+    if done is not None:
+        return done
     device = _require_cuda(q, k, v)
     if any(t.dtype != torch.bfloat16 for t in (q, k, v)):
         raise ValueError("packed_attention expects bf16 q, k, v")
@@ -893,9 +911,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_starts
         nbytes = _native.load_library().bsa_packed_attention_workspace_bytes(Tq, Tk, requests, H, Hk)
         work = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
         s = float(scale) if scale is not None else D ** -0.5
-        _native.call("bsa_packed_attention", q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(),
-                     k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-                     q_starts.data_ptr(), k_starts.data_ptr(), Tq, Tk, requests, H, Hk, D,
-                     1 if causal else 0, s, _native.ptr(work), nbytes, out.data_ptr(),
-                     _native.err_word(device).data_ptr(), _stream(device))
+        _call_on(device, "bsa_packed_attention", q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(),
+                 k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+                 q_starts.data_ptr(), k_starts.data_ptr(), Tq, Tk, requests, H, Hk, D,
+                 1 if causal else 0, s, _native.ptr(work), nbytes, out.data_ptr())
     return out
