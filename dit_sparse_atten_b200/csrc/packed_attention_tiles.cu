@@ -94,6 +94,17 @@ struct Barriers {
 };
 constexpr int kUsed = kBarOff + static_cast<int>(sizeof(Barriers));
 
+// One lane of the (converged) warp, the same every time.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok));
+  return ok != 0;
+}
+
 // Cluster launch control: ask for a CTA of this grid that has not started to
 // be cancelled, its index to be taken over by the caller.
 __device__ __forceinline__ void request_next(uint4* answer, uint64_t* bar) {
@@ -131,7 +142,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   Barriers* bar = reinterpret_cast<Barriers*>(smem + kBarOff);
   volatile int* abort_flag = &bar->abort;
 
-  const int warp = threadIdx.x >> 5;
+  // shuffled, so that the compiler knows it uniform over the warp
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
   const int lane = threadIdx.x & 31;
   const int G = a.group;
   const int tt = a.tile_tokens;
@@ -301,7 +313,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
    } else if (warp == kMmaWarp || warp == kMmaWarp + 1) {
     // ------------------------------------------------------------ MMA issuers
-    if (lane == 0) {
+    {
       const int t = warp - kMmaWarp;
       const uint32_t idesc_s = idesc_bf16_f32(128, kSub, false);
       const uint32_t idesc_o = idesc_bf16_f32(128, kHeadDim, true);
@@ -313,8 +325,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t ring_phase = 0;
       uint32_t scored = 0, used = 0, outs = 0;   // S issued, P consumed, O finished
       bool ok = true;
+      // The whole warp goes through the loop, so that the descriptors stay in
+      // uniform registers; one elected lane issues.
       auto wait = [&](uint64_t* b, uint32_t parity) {
-        return mbar_wait(b, parity, abort_flag, a.err_word);
+        return __all_sync(0xffffffffu, mbar_wait(b, parity, abort_flag, a.err_word)) != 0;
+      };
+      auto commit = [&](uint64_t* b) {
+        if (elect_one()) umma_commit(b);
       };
       // Next slot of the ring, once it is full.
       auto next_slot = [&]() -> int {
@@ -327,20 +344,24 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto issue_s = [&](int s, int half) {
         const uint64_t kd = kdesc0 + static_cast<uint64_t>((s * kSlotBytes + half * kSub * 128) >> 4);
         const uint32_t b = scored & 1;
+        if (elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < kHeadDim / 16; ++kk) {
-          const uint64_t off = static_cast<uint64_t>(((kk >> 2) * kPanel + (kk & 3) * 32) >> 4);
-          umma_bf16_ss(s_tmem + b * kSub, qdesc + off, kd + off, idesc_s, kk > 0 ? 1u : 0u);
+          for (int kk = 0; kk < kHeadDim / 16; ++kk) {
+            const uint64_t off = static_cast<uint64_t>(((kk >> 2) * kPanel + (kk & 3) * 32) >> 4);
+            umma_bf16_ss(s_tmem + b * kSub, qdesc + off, kd + off, idesc_s, kk > 0 ? 1u : 0u);
+          }
+          umma_commit(&bar->s_full[t][b]);
         }
-        umma_commit(&bar->s_full[t][b]);
+        __syncwarp();
         ++scored;
       };
       for (int i = 0; ok; ++i) {
         const Item* it = item_at(i);
-        if (it == nullptr) break;
-        const int mine = it->n[t];               // sub-blocks
-        const int n = item_blocks(it);
-        done_with(i);
+        if (!__all_sync(0xffffffffu, it != nullptr)) break;
+        const int mine = __shfl_sync(0xffffffffu, it->n[t], 0);         // sub-blocks
+        const int n = __shfl_sync(0xffffffffu, item_blocks(it), 0);
+        __syncwarp();
+        if (elect_one()) done_with(i);
         if (n == 0) continue;
         // Blocks past this tile's last are only passed on (the other tile reads
         // them): the slot is given back once it is full.
@@ -350,8 +371,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
         if (mine > 0) issue_s(sk, 0);
         if (mine > 1) issue_s(sk, 1);
-        umma_commit(&bar->slot_empty[sk]);
-        if (mine <= 2) umma_commit(&bar->q_empty);
+        commit(&bar->slot_empty[sk]);
+        if (mine <= 2) commit(&bar->q_empty);
         for (int j = 0; ok && j < n; ++j) {
           if (j + 1 < n) {
             sk = next_slot();
@@ -369,27 +390,30 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t b = used & 1;
             if (!(ok = wait(&bar->p_full[t][b], (used >> 1) & 1))) break;
             tc_fence_after();
+            if (elect_one()) {
 #pragma unroll
-            for (int kk = 0; kk < kSub / 16; ++kk)
-              umma_bf16_ts(o_tmem, s_tmem + b * kSub + kk * 8,
-                           vd + static_cast<uint64_t>(((half * kSub + kk * 16) * 128) >> 4), idesc_o,
-                           (u > 0 || kk > 0) ? 1u : 0u);
-            umma_commit(&bar->pv_done[t]);
+              for (int kk = 0; kk < kSub / 16; ++kk)
+                umma_bf16_ts(o_tmem, s_tmem + b * kSub + kk * 8,
+                             vd + static_cast<uint64_t>(((half * kSub + kk * 16) * 128) >> 4), idesc_o,
+                             (u > 0 || kk > 0) ? 1u : 0u);
+              umma_commit(&bar->pv_done[t]);
+            }
+            __syncwarp();
             ++used;
             if (u + 1 == mine) {
-              umma_commit(&bar->o_full[t]);
+              commit(&bar->o_full[t]);
               ++outs;
             }
             if (u + 2 < mine) issue_s(sk, half);
-            if (u + 3 == mine) umma_commit(&bar->q_empty);
+            if (u + 3 == mine) commit(&bar->q_empty);
           }
           if (!ok) break;
-          umma_commit(&bar->slot_empty[sv]);
-          if (j + 1 < n) umma_commit(&bar->slot_empty[sk]);
+          commit(&bar->slot_empty[sv]);
+          if (j + 1 < n) commit(&bar->slot_empty[sk]);
         }
       }
       int never = 0;
-      umma_commit(&bar->drain[t]);
+      commit(&bar->drain[t]);
       mbar_wait(&bar->drain[t], 0, &never, a.err_word);
     }
    } else if (warp == kCheckWarp) {
