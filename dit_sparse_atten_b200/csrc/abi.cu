@@ -1143,7 +1143,7 @@ int bsa_packed_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h, 
   a.kv_heads = kv_heads;
   a.group = heads / kv_heads;
   a.tile_tokens = 128 / a.group;
-  a.slots = q_rows / a.tile_tokens + requests;
+  a.slots = q_rows / (2 * a.tile_tokens) + requests;
   a.splits = bsa::packed_splits(q_rows, k_rows, requests, heads, kv_heads, sm_count());
   a.causal = causal != 0;
   a.scale = scale;

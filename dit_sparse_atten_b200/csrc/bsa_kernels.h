@@ -263,7 +263,7 @@ struct LoraMaps {
 };
 cudaError_t launch_lora_add(const LoraMaps& maps, LoraArgs args, cudaStream_t stream, int num_sms);
 
-// Attention over packed sequences (packed_attention_tiles.cu, packed_attention.cu).
+// Attention over packed sequences (packed_attention.cu).
 struct PackedArgs {
   const __nv_bfloat16* q;       // [q_rows, heads, 128], strides below (elements)
   const __nv_bfloat16* k;       // [k_rows, kv_heads, 128]
@@ -275,7 +275,7 @@ struct PackedArgs {
   int32_t requests, heads, kv_heads;
   int32_t group;                // heads / kv_heads <= 128
   int32_t tile_tokens;          // 128 / group
-  int64_t slots;                // q_rows / tile_tokens + requests
+  int64_t slots;                // q_rows / (2 tile_tokens) + requests
   int32_t splits;
   bool causal;
   float scale;
@@ -286,9 +286,6 @@ struct PackedArgs {
 };
 int32_t packed_splits(int64_t q_rows, int64_t k_rows, int32_t requests, int32_t heads,
                       int32_t kv_heads, int num_sms);
-cudaError_t launch_packed_tiles(const CUtensorMap& tm_q, const CUtensorMap& tm_k,
-                                const CUtensorMap& tm_v, const PackedArgs& args,
-                                cudaStream_t stream);
 cudaError_t launch_packed_attention(const CUtensorMap& tm_q, const CUtensorMap& tm_k,
                                     const CUtensorMap& tm_v, const PackedArgs& args,
                                     cudaStream_t stream);

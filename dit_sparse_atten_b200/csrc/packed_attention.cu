@@ -1,20 +1,41 @@
-// Attention over packed sequences where the query tiles alone leave SMs idle
-// (a few new tokens over long keys): the keys of a tile are split over CTAs and
-// joined.  The operator's definition and the larger form are in
-// packed_attention_tiles.cu.
+// Softmax attention over packed sequences of different lengths, grouped heads,
+// causal or full, for sm_100a:
+//   out[i, h] = sum_j softmax_j(scale * q[i, h] . k[j, h / G]) v[j, h / G]
+// over the keys j of query i's own request (causal: the first
+// i + 1 + k_len - q_len of them, i counted within the request), in float32
+// from bf16 inputs; a query that sees no key gives 0.
 //
-// One CTA takes one part of the key blocks of the 128 / G tokens x G heads of
-// one key head, as the 128 rows of the MMA (row = token * G + head in group):
-// all query heads that share a key head share its K and V loads, and a single
-// new token still fills G rows.  Bound: HBM, K and V read once.
-//   warp 8      TMA producer: K/V blocks of 128 keys into a ring of 32 KB
+// An item is 2 x (128 / G tokens) x G heads of one key head: two MMA tiles of
+// 128 rows (row = token * G + head in group), so that all query heads of a key
+// head, and both tiles, share its K and V loads.  While one tile's softmax
+// runs, the tensor pipe works for the other.  CTAs are resident and take their
+// next item from the grid's CTAs that have not started (cluster launch
+// control), so an item's first loads and S run under the last softmax and the
+// store of the item before.  Items are found on the device (packed_common.cuh),
+// those late in their request first: under the causal mask they see the most
+// keys.
+//   warps 0-3, 4-7   softmax of tile 0, 1: 64 keys at a time, one row a thread,
+//               log2 domain, a stabiliser that moves only past 2^8 (then O_t is
+//               rescaled in TMEM), P as bf16 into the first half of S's columns
+//   warps 8, 9  MMA issuers, one thread for each tile t: for each 64 keys u,
+//               O_t += P_t(u) V(u), then S_t(u + 2) = Q_t K(u + 2)^T; warp 8
+//               owns TMEM.  A tile has its own issuer so that it never waits
+//               for the other's softmax.
+//   warp 10     TMA producer: Q; K/V blocks of 128 keys into a ring of 32 KB
 //               slots (K0, K1, V0, K2, V1, ...)
-//   warp 9      TMEM owner; one thread loads Q and issues S_j = Q K_j^T
-//   warp 10     one thread issues O += P_j V_j (P from tensor memory)
-//   warp 11     cleans V of the masked blocks (clean_masked_values)
-//   warps 0-7   softmax, two groups that take alternate key blocks, one row a
-//               thread, log2 domain, a stabiliser that moves only past 2^8
-// TMEM: three S (and P) buffers at [0, 384), O at [384, 512).
+//   warp 11     scheduler: cancels a pending CTA, looks its item up, publishes
+//   warp 12     cleans V of the masked blocks (clean_masked_values)
+// TMEM: tile t's two S buffers of 64 columns at 128 t, O_t at 256 + 128 t.
+// Two buffers of 64 keys, not one of 128: P lives in S's columns, so S of the
+// next keys waits for PV, and with one buffer the softmax waited for both (1,300
+// of 3,700 cycles a block); with two it runs while the other's PV and S do.
+// (S of 64 keys reads Q from shared memory twice as often: 1.5 times the time
+// of one product of 128, still under the softmax's.)
+//
+// A value of V that is not finite at a key which part of the item must not see
+// (causal) cannot be kept out of those rows by P = 0; warp 12 looks for one
+// and, if there is, the item's rows are computed again key by key in float32.
+//
 // Every mbarrier wait is bounded (bsa::mbar_wait); on a timeout the CTA sets
 // kErrWaitTimeout, drains its copies and MMAs, frees TMEM and exits.
 #include <algorithm>
@@ -28,86 +49,148 @@ namespace {
 using namespace attn;
 using namespace packed;
 
-constexpr int kThreads = 384;
-constexpr int kProducerWarp = 8;
-constexpr int kMmaWarp = 9;
-constexpr int kPvWarp = 10;
-constexpr int kCheckWarp = 11;
-constexpr int kSBuffers = 3;
-constexpr uint32_t kTmemO = 384;
-constexpr int kSlots = 6;
+constexpr int kSoftWarps = 8;
+constexpr int kThreads = 416;
+constexpr int kMmaWarp = 8;             // and 9
+constexpr int kProducerWarp = 10;
+constexpr int kSchedWarp = 11;
+constexpr int kCheckWarp = 12;
+constexpr int kLate = 2;                // key blocks left to load of an item when the next is asked for
+constexpr int kSub = 64;                // keys of an S buffer
+// Ring slots; parts of keys are bound by HBM and stage no output, which leaves
+// room for one more.
+constexpr int kMaxSlots = 5;
+template <bool kSplit>
+constexpr int kSlotsOf = kSplit ? 5 : 4;
+constexpr int kMaskedRing = 4;          // masked V blocks between the producer and warp 12
+#ifndef BSA_PACKED_EMULATED
+#define BSA_PACKED_EMULATED 0
+#endif
+constexpr int kEmulated = BSA_PACKED_EMULATED;
+constexpr int kWorkRing = 2;            // an item at work and the next
+constexpr int kWorkReaders = kSoftWarps + 4;   // and both issuers, producer, check
 constexpr int kQOff = 0;
-constexpr int kRingOff = kQOff + 128 * 256;
-constexpr int kXOff = kRingOff + kSlots * kSlotBytes;
-constexpr int kBarOff = kXOff + 2 * 2 * 128 * 4;
+constexpr int kRingOff = 2 * kSlotBytes;
+constexpr int kStageOff = kRingOff + kSlotsOf<false> * kSlotBytes;
+constexpr int kStageBytes = 32 * 128;   // of each softmax warp: 64 features of its 32 rows
+constexpr int kBarOff = kStageOff + kSoftWarps * kStageBytes;
+static_assert(kBarOff == kRingOff + kSlotsOf<true> * kSlotBytes, "the fifth slot takes the stage's place");
+
+// An item as the scheduler publishes it.
+struct Item {
+  Work w;              // w.tokens < 0: no more items
+  int hk;              // key head
+  int n[2];            // 64-key sub-blocks of each tile
+  int part;            // of the keys
+  int exact;           // set by warp 12
+};
 
 struct Barriers {
-  uint64_t q_full;
-  uint64_t s_full[kSBuffers];
-  uint64_t p_full[kSBuffers];
-  uint64_t m_full[2];
-  uint64_t o_done[kSBuffers];
+  uint64_t q_full, q_empty;
+  uint64_t s_full[2][2], p_full[2][2];  // [tile][S buffer]
+  uint64_t pv_done[2];
+  uint64_t o_full[2], o_empty[2];
+  uint64_t slot_full[kMaxSlots], slot_empty[kMaxSlots];
+  uint64_t masked_full[kMaskedRing];    // V of a masked block, before warp 12
+  uint64_t work_full[kWorkRing], work_empty[kWorkRing];
+  uint64_t nearly_done;                 // the producer is at an item's last blocks
+  uint64_t next_full;                   // answer of the cluster launch control
   uint64_t drain[2];
-  uint64_t masked_full[2];              // V of the masked blocks, before warp 11
-  uint64_t slot_full[kSlots];
-  uint64_t slot_empty[kSlots];
   uint32_t tmem_base;
   int abort;
-  int exact_rows;                       // warp 11: recompute the rows key by key
+  Item item[kWorkRing];
+  uint4 next __attribute__((aligned(16)));
 };
 constexpr int kUsed = kBarOff + static_cast<int>(sizeof(Barriers));
 
-// Leaves O (relative to its stabiliser), the stabiliser and the sum of part
-// `split` in the workspace for combine_kernel.
+// One lane of the (converged) warp, the same every time.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok));
+  return ok != 0;
+}
+
+// Cluster launch control: ask for a CTA of this grid that has not started to
+// be cancelled, its index to be taken over by the caller.
+__device__ __forceinline__ void request_next(uint4* answer, uint64_t* bar) {
+  asm volatile(
+      "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+          smem_u32(answer)),
+      "r"(smem_u32(bar))
+      : "memory");
+}
+// blockIdx.x of the cancelled CTA, or -1 (all have started).
+__device__ __forceinline__ int64_t answered_next(const uint4* answer) {
+  uint32_t ok, x;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b128 r;\n\t"
+      "ld.shared.b128 r, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "mov.u32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n\t}"
+      : "=r"(ok), "=r"(x)
+      : "r"(smem_u32(answer))
+      : "memory");
+  return ok ? static_cast<int64_t>(x) : -1;
+}
+
+// kSplit: items are parts of the keys (find_part); O (relative to its
+// stabiliser), the stabiliser and the sum go to the workspace for
+// combine_kernel.
+template <bool kSplit>
 __global__ void __launch_bounds__(kThreads, 1)
-    packed_attention_split_kernel(const __grid_constant__ CUtensorMap tm_q,
-                            const __grid_constant__ CUtensorMap tm_k,
-                            const __grid_constant__ CUtensorMap tm_v, const PackedArgs a) {
+    packed_attention_tiles_kernel(const __grid_constant__ CUtensorMap tm_q,
+                                  const __grid_constant__ CUtensorMap tm_k,
+                                  const __grid_constant__ CUtensorMap tm_v, const PackedArgs a) {
+  constexpr int kSlots = kSlotsOf<kSplit>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* sQ = smem + kQOff;
   uint8_t* sRing = smem + kRingOff;
-  float* sX = reinterpret_cast<float*>(smem + kXOff);
   Barriers* bar = reinterpret_cast<Barriers*>(smem + kBarOff);
   volatile int* abort_flag = &bar->abort;
 
-  const int warp = threadIdx.x >> 5;
+  // shuffled, so that the compiler knows it uniform over the warp
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
   const int lane = threadIdx.x & 31;
-  const int64_t slot = a.slots - 1 - blockIdx.x % a.slots;
-  const int hk = static_cast<int>((blockIdx.x / a.slots) % a.kv_heads);
-  const int split = static_cast<int>(blockIdx.x / (a.slots * a.kv_heads));
-  const Work w = find_work(a, slot, a.tile_tokens);
-  if (w.tokens == 0) return;
   const int G = a.group;
-  const int all = (row_limit(w, w.tokens - 1, a.causal) + kBlock - 1) / kBlock;
-  const int block0 = static_cast<int>(static_cast<int64_t>(all) * split / a.splits);
-  const int n = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / a.splits) - block0;
-  // The first block of this CTA that some row of the tile does not see whole.
-  const int masked_from = max(0, min(n, max(0, row_limit(w, 0, a.causal)) / kBlock - block0));
+  const int tt = a.tile_tokens;
 
   if (threadIdx.x == 0) {
     uint32_t dyn_bytes;
     asm("mov.u32 %0, %%dynamic_smem_size;" : "=r"(dyn_bytes));
     const bool fits = (smem - smem_raw) + kUsed <= static_cast<int>(dyn_bytes);
+    bar->abort = (prior_timeout(a.err_word) || !fits) ? 1 : 0;
+    if (!fits) atomicOr(a.err_word, kErrSmemLayout);
     mbar_init(&bar->q_full, 1);
-    for (int i = 0; i < kSBuffers; ++i) {
-      mbar_init(&bar->s_full[i], 1);
-      mbar_init(&bar->p_full[i], 128);
-      mbar_init(&bar->o_done[i], 1);
-    }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&bar->m_full[i], 128);
-      mbar_init(&bar->drain[i], 1);
-      mbar_init(&bar->masked_full[i], 1);
+    mbar_init(&bar->q_empty, 2);
+    for (int t = 0; t < 2; ++t) {
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(&bar->s_full[t][b], 1);
+        mbar_init(&bar->p_full[t][b], 128);
+      }
+      mbar_init(&bar->pv_done[t], 1);
+      mbar_init(&bar->o_full[t], 1);
+      mbar_init(&bar->o_empty[t], 128);
     }
     for (int s = 0; s < kSlots; ++s) {
       mbar_init(&bar->slot_full[s], 1);
-      mbar_init(&bar->slot_empty[s], 1);
+      mbar_init(&bar->slot_empty[s], 2);
     }
-    bar->exact_rows = 0;
-    bar->abort = (prior_timeout(a.err_word) || !fits) ? 1 : 0;
-    if (!fits) atomicOr(a.err_word, kErrSmemLayout);
+    for (int i = 0; i < kMaskedRing; ++i) mbar_init(&bar->masked_full[i], 1);
+    for (int i = 0; i < kWorkRing; ++i) {
+      mbar_init(&bar->work_full[i], 1);
+      mbar_init(&bar->work_empty[i], kWorkReaders);
+    }
+    mbar_init(&bar->nearly_done, 1);
+    mbar_init(&bar->next_full, 1);
+    for (int t = 0; t < 2; ++t) mbar_init(&bar->drain[t], 1);
     fence_mbar_init();
   }
   __syncthreads();
@@ -118,40 +201,126 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = bar->tmem_base;
 
-  // Load sequence: K0, then K_{j+1}, V_j for every j.
-  auto seq_k = [](int j) { return j == 0 ? 0 : 2 * j - 1; };
-  auto seq_v = [n](int j) { return j + 1 < n ? 2 * j + 2 : 2 * j + 1; };
+  // Item number i of this CTA, or null (no more, or aborting).
+  auto item_at = [&](int i) -> Item* {
+    const int r = i % kWorkRing;
+    if (!mbar_wait(&bar->work_full[r], (i / kWorkRing) & 1, abort_flag, a.err_word)) return nullptr;
+    Item* it = &bar->item[r];
+    return it->w.tokens < 0 ? nullptr : it;
+  };
+  auto done_with = [&](int i) { mbar_arrive(&bar->work_empty[i % kWorkRing]); };
+  // First block of the item that some row of tile t does not see whole.
+  auto masked_from = [&](const Work& w, int t) { return row_limit(w, t * tt, a.causal) / kBlock; };
 
-  if (warp == kProducerWarp) {
-    // ------------------------------------------------------------ producer
-    if (lane == 0 && n > 0) {
-      uint32_t armed = 0, armed_phase = 0;
-      int masked = 0;            // masked V blocks loaded
-      bool ok = true;
-      auto load = [&](const CUtensorMap* tm, int seq, int j, bool is_v) {
-        const int s = seq % kSlots;
-        const uint32_t ph = (seq / kSlots) & 1;
-        if (!mbar_wait(&bar->slot_empty[s], ph ^ 1, abort_flag, a.err_word)) return false;
-        uint8_t* dst = sRing + s * kSlotBytes;
-        uint64_t* full = &bar->slot_full[s];
-        if (is_v && j >= masked_from) {
-          full = &bar->masked_full[masked++];     // at most two: the limits of a tile's rows
-                                                  // span at most 127 keys
-          armed &= ~(1u << s);   // an earlier load of this slot has long been consumed
-        } else {
-          armed |= 1u << s;
-          armed_phase = (armed_phase & ~(1u << s)) | (ph << s);
+  // Blocks of 128 keys of an item: both tiles'.
+  auto item_blocks = [&](const Item* it) { return (max(it->n[0], it->n[1]) + 1) / 2; };
+
+  if (warp >= kSoftWarps) {
+   if (warp == kSchedWarp) {
+    // ------------------------------------------------------------ scheduler
+    // The next item is asked for when the loads of the one at work come to
+    // their last blocks: asked for earlier, an item waits here while other CTAs
+    // run out of work.
+    int64_t cta = blockIdx.x;
+    uint32_t answers = 0;
+    for (int i = 0;;) {
+      Item it{};
+      it.w.tokens = -1;
+      if (cta >= 0) {
+        // late slots first; a key head's items next to each other
+        it.hk = static_cast<int>(cta % a.kv_heads);
+        const int64_t rest = cta / a.kv_heads;
+        it.w = find_work(a, a.slots - 1 - rest % a.slots, 2 * tt);
+        if constexpr (kSplit) {
+          it.part = static_cast<int>(rest / a.slots);
+          take_part(it.w, it.part, a);
         }
-        const int row = static_cast<int>(w.k0 + static_cast<int64_t>(block0 + j) * kBlock);
-        mbar_arrive_expect_tx(full, kSlotBytes);
-        tma_load_3d(dst, tm, full, 0, hk, row);
-        tma_load_3d(dst + kPanel, tm, full, 64, hk, row);
-        return true;
-      };
-      ok = load(&tm_k, 0, 0, false);
-      for (int j = 0; ok && j < n; ++j) {
-        if (j + 1 < n) ok = load(&tm_k, seq_k(j + 1), j + 1, false);
-        if (ok) ok = load(&tm_v, seq_v(j), j, true);
+      }
+      if (it.w.tokens != 0) {
+        for (int t = 0; t < 2; ++t) {
+          const int last = min(it.w.tokens, (t + 1) * tt) - 1;
+          it.n[t] = last < t * tt ? 0 : (row_limit(it.w, last, a.causal) + kSub - 1) / kSub;
+        }
+        bool ok = true;
+        if (lane == 0) {
+          const int r = i % kWorkRing;
+          ok = mbar_wait(&bar->work_empty[r], ((i / kWorkRing) & 1) ^ 1, abort_flag, a.err_word);
+          if (ok) {
+            bar->item[r] = it;
+            mbar_arrive(&bar->work_full[r]);
+            if (cta >= 0) ok = mbar_wait(&bar->nearly_done, i & 1, abort_flag, a.err_word);
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        ++i;
+        if (cta < 0 || !ok) break;
+      }
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&bar->next_full, 16);
+        request_next(&bar->next, &bar->next_full);
+      }
+      if (!mbar_wait(&bar->next_full, answers & 1, abort_flag, a.err_word)) {
+        int never = 0;   // an answer is on its way into shared memory
+        mbar_wait(&bar->next_full, answers & 1, &never, a.err_word);
+        break;
+      }
+      ++answers;
+      cta = answered_next(&bar->next);
+      fence_proxy_async_smem();   // the answer is read before the next one is asked for
+      __syncwarp();
+    }
+   } else if (warp == kProducerWarp) {
+    // ------------------------------------------------------------ producer
+    if (lane == 0) {
+      uint32_t armed = 0, armed_phase = 0;
+      int seq = 0, masked = 0, loads = 0;      // of K/V, of masked V, of Q
+      bool ok = true;
+      for (int i = 0; ok; ++i) {
+        const Item* it = item_at(i);
+        if (it == nullptr) break;
+        const Work w = it->w;
+        const int hk = it->hk;
+        const int n = item_blocks(it);
+        done_with(i);
+        const int from = masked_from(w, 0);
+        auto load = [&](const CUtensorMap* tm, int j, bool is_v) {
+          const int s = seq % kSlots;
+          const uint32_t ph = (seq / kSlots) & 1;
+          if (!mbar_wait(&bar->slot_empty[s], ph ^ 1, abort_flag, a.err_word)) return false;
+          uint8_t* dst = sRing + s * kSlotBytes;
+          uint64_t* full = &bar->slot_full[s];
+          if (is_v && j >= from) {
+            full = &bar->masked_full[masked++ % kMaskedRing];
+            armed &= ~(1u << s);   // an earlier load of this slot has long been consumed
+          } else {
+            armed |= 1u << s;
+            armed_phase = (armed_phase & ~(1u << s)) | (ph << s);
+          }
+          const int row = static_cast<int>(w.k0 + static_cast<int64_t>(j) * kBlock);
+          mbar_arrive_expect_tx(full, kSlotBytes);
+          tma_load_3d(dst, tm, full, 0, hk, row);
+          tma_load_3d(dst + kPanel, tm, full, 64, hk, row);
+          ++seq;
+          return true;
+        };
+        if (n <= kLate) mbar_arrive(&bar->nearly_done);
+        if (n == 0) continue;
+        ok = load(&tm_k, 0, false);
+        if (ok) ok = mbar_wait(&bar->q_empty, (loads & 1) ^ 1, abort_flag, a.err_word);
+        if (!ok) break;
+        // Rows past tt * G keep whatever the shared memory held: a row of
+        // garbage reaches only its own row of S and O, which is not stored.
+        mbar_arrive_expect_tx(&bar->q_full, static_cast<uint32_t>(tt * G) * 512u);
+        for (int t = 0; t < 2; ++t)
+          for (int p = 0; p < 2; ++p)
+            tma_load_3d(sQ + t * kSlotBytes + p * kPanel, &tm_q, &bar->q_full, p * 64, hk * G,
+                        static_cast<int>(w.q0) + t * tt);
+        ++loads;
+        for (int j = 0; ok && j < n; ++j) {
+          if (n > kLate && j == n - kLate) mbar_arrive(&bar->nearly_done);
+          if (j + 1 < n) ok = load(&tm_k, j + 1, false);
+          if (ok) ok = load(&tm_v, j, true);
+        }
       }
       // Never leave a copy in flight into shared memory.
       int never = 0;
@@ -159,205 +328,329 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int s = 0; s < kSlots; ++s)
         if (armed & (1u << s))
           mbar_wait(&bar->slot_full[s], (armed_phase >> s) & 1u, &never, a.err_word);
-      for (int i = 0; i < masked; ++i) mbar_wait(&bar->masked_full[i], 0, &never, a.err_word);
+      for (int j = max(0, masked - kMaskedRing); j < masked; ++j)
+        mbar_wait(&bar->masked_full[j % kMaskedRing], (j / kMaskedRing) & 1, &never, a.err_word);
+      if (loads) mbar_wait(&bar->q_full, (loads - 1) & 1, &never, a.err_word);
     }
-  } else if (warp == kMmaWarp) {
-    if (lane == 0 && n > 0) {
-      const uint32_t idesc = idesc_bf16_f32(128, kBlock, false);
+   } else if (warp == kMmaWarp || warp == kMmaWarp + 1) {
+    // ------------------------------------------------------------ MMA issuers
+    {
+      const int t = warp - kMmaWarp;
+      const uint32_t idesc_s = idesc_bf16_f32(128, kSub, false);
+      const uint32_t idesc_o = idesc_bf16_f32(128, kHeadDim, true);
       const uint64_t kdesc0 = sdesc_sw128(smem_u32(sRing), 16, 1024);
-      const uint64_t qdesc0 = sdesc_sw128(smem_u32(sQ), 16, 1024);
-      // Rows past tile_tokens * G keep whatever the shared memory held: a row
-      // of garbage reaches only its own row of S and O, which is not stored.
-      mbar_arrive_expect_tx(&bar->q_full, static_cast<uint32_t>(a.tile_tokens * G) * 256u);
-      tma_load_3d(sQ, &tm_q, &bar->q_full, 0, hk * G, static_cast<int>(w.q0));
-      tma_load_3d(sQ + 16384, &tm_q, &bar->q_full, 64, hk * G, static_cast<int>(w.q0));
-      int never = 0;
-      bool ok = mbar_wait(&bar->q_full, 0, &never, a.err_word);
-      for (int j = 0; ok && j < n; ++j) {
-        const int sq = seq_k(j);
-        const int s = sq % kSlots;
-        ok = mbar_wait(&bar->slot_full[s], (sq / kSlots) & 1, abort_flag, a.err_word);
-        // S_j overwrites P_{j-3} (same TMEM buffer): PV_{j-3} must be done.
-        const int sb = j % kSBuffers;
-        if (ok && j >= kSBuffers)
-          ok = mbar_wait(&bar->o_done[sb], ((j - kSBuffers) / kSBuffers) & 1, abort_flag,
-                         a.err_word);
-        if (!ok) break;
-        tc_fence_after();
-        const uint64_t kd = kdesc0 + static_cast<uint64_t>((s * kSlotBytes) >> 4);
-#pragma unroll
-        for (int kk = 0; kk < kHeadDim / 16; ++kk) {
-          const uint64_t db = kd + static_cast<uint64_t>(((kk >> 2) * kPanel + (kk & 3) * 32) >> 4);
-          const uint64_t da = qdesc0 + static_cast<uint64_t>(((kk >> 2) * 16384 + (kk & 3) * 32) >> 4);
-          umma_bf16_ss(tmem + sb * 128, da, db, idesc, kk > 0 ? 1u : 0u);
-        }
-        umma_commit(&bar->s_full[sb]);
-        umma_commit(&bar->slot_empty[s]);
-      }
-      umma_commit(&bar->drain[0]);
-      mbar_wait(&bar->drain[0], 0, &never, a.err_word);
-    }
-  } else if (warp == kPvWarp) {
-    if (lane == 0 && n > 0) {
-      const uint32_t idesc = idesc_bf16_f32(128, kHeadDim, true);
       const uint64_t vdesc0 = sdesc_sw128(smem_u32(sRing), kPanel, 1024);
+      const uint64_t qdesc = sdesc_sw128(smem_u32(sQ + t * kSlotBytes), 16, 1024);
+      const uint32_t s_tmem = tmem + t * 128, o_tmem = tmem + 256 + t * 128;
+      int slot = 0, loads = 0;
+      uint32_t ring_phase = 0;
+      uint32_t scored = 0, used = 0, outs = 0;   // S issued, P consumed, O finished
       bool ok = true;
-      for (int j = 0; ok && j < n; ++j) {
-        const int sq = seq_v(j);
-        const int s = sq % kSlots;
-        ok = mbar_wait(&bar->slot_full[s], (sq / kSlots) & 1, abort_flag, a.err_word);
-        const int sb = j % kSBuffers;
-        if (ok) ok = mbar_wait(&bar->p_full[sb], (j / kSBuffers) & 1, abort_flag, a.err_word);
-        if (!ok) break;
-        tc_fence_after();
-        const uint64_t vd = vdesc0 + static_cast<uint64_t>((s * kSlotBytes) >> 4);
+      // The whole warp goes through the loop, so that the descriptors stay in
+      // uniform registers; one elected lane issues.
+      auto wait = [&](uint64_t* b, uint32_t parity) {
+        return __all_sync(0xffffffffu, mbar_wait(b, parity, abort_flag, a.err_word)) != 0;
+      };
+      auto commit = [&](uint64_t* b) {
+        if (elect_one()) umma_commit(b);
+      };
+      // Next slot of the ring, once it is full.
+      auto next_slot = [&]() -> int {
+        const int s = slot;
+        ok = wait(&bar->slot_full[s], ring_phase);
+        if (++slot == kSlots) slot = 0, ring_phase ^= 1;
+        return s;
+      };
+      // S of keys 64 half .. of the K block in slot s, into the next buffer.
+      auto issue_s = [&](int s, int half) {
+        const uint64_t kd = kdesc0 + static_cast<uint64_t>((s * kSlotBytes + half * kSub * 128) >> 4);
+        const uint32_t b = scored & 1;
+        if (elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < kBlock / 16; ++kk)
-          umma_bf16_ts(tmem + kTmemO, tmem + sb * 128 + kk * 8,
-                       vd + static_cast<uint64_t>((kk * 16 * 128) >> 4), idesc,
-                       (j > 0 || kk > 0) ? 1u : 0u);
-        umma_commit(&bar->o_done[sb]);
-        umma_commit(&bar->slot_empty[s]);
+          for (int kk = 0; kk < kHeadDim / 16; ++kk) {
+            const uint64_t off = static_cast<uint64_t>(((kk >> 2) * kPanel + (kk & 3) * 32) >> 4);
+            umma_bf16_ss(s_tmem + b * kSub, qdesc + off, kd + off, idesc_s, kk > 0 ? 1u : 0u);
+          }
+          umma_commit(&bar->s_full[t][b]);
+        }
+        __syncwarp();
+        ++scored;
+      };
+      for (int i = 0; ok; ++i) {
+        const Item* it = item_at(i);
+        if (!__all_sync(0xffffffffu, it != nullptr)) break;
+        const int mine = __shfl_sync(0xffffffffu, it->n[t], 0);         // sub-blocks
+        const int n = __shfl_sync(0xffffffffu, item_blocks(it), 0);
+        __syncwarp();
+        if (elect_one()) done_with(i);
+        if (n == 0) continue;
+        // Blocks past this tile's last are only passed on (the other tile reads
+        // them): the slot is given back once it is full.
+        int sk = next_slot();
+        if (!ok || !(ok = wait(&bar->q_full, loads & 1))) break;
+        ++loads;
+        tc_fence_after();
+        if (mine > 0) issue_s(sk, 0);
+        if (mine > 1) issue_s(sk, 1);
+        commit(&bar->slot_empty[sk]);
+        if (mine <= 2) commit(&bar->q_empty);
+        for (int j = 0; ok && j < n; ++j) {
+          if (j + 1 < n) {
+            sk = next_slot();
+            if (!ok) break;
+          }
+          const int sv = next_slot();
+          if (!ok) break;
+          const uint64_t vd = vdesc0 + static_cast<uint64_t>((sv * kSlotBytes) >> 4);
+#pragma unroll 1
+          for (int half = 0; half < 2; ++half) {
+            const int u = 2 * j + half;
+            if (u >= mine) break;
+            // the first PV of an item overwrites the O that the softmax group stores
+            if (u == 0 && !(ok = wait(&bar->o_empty[t], (outs & 1) ^ 1))) break;
+            const uint32_t b = used & 1;
+            if (!(ok = wait(&bar->p_full[t][b], (used >> 1) & 1))) break;
+            tc_fence_after();
+            if (elect_one()) {
+#pragma unroll
+              for (int kk = 0; kk < kSub / 16; ++kk)
+                umma_bf16_ts(o_tmem, s_tmem + b * kSub + kk * 8,
+                             vd + static_cast<uint64_t>(((half * kSub + kk * 16) * 128) >> 4), idesc_o,
+                             (u > 0 || kk > 0) ? 1u : 0u);
+              umma_commit(&bar->pv_done[t]);
+            }
+            __syncwarp();
+            ++used;
+            if (u + 1 == mine) {
+              commit(&bar->o_full[t]);
+              ++outs;
+            }
+            if (u + 2 < mine) issue_s(sk, half);
+            if (u + 3 == mine) commit(&bar->q_empty);
+          }
+          if (!ok) break;
+          commit(&bar->slot_empty[sv]);
+          if (j + 1 < n) commit(&bar->slot_empty[sk]);
+        }
       }
       int never = 0;
-      umma_commit(&bar->drain[1]);
-      mbar_wait(&bar->drain[1], 0, &never, a.err_word);
+      commit(&bar->drain[t]);
+      mbar_wait(&bar->drain[t], 0, &never, a.err_word);
     }
-  } else if (warp == kCheckWarp) {
+   } else if (warp == kCheckWarp) {
     // ------------------------------------------------------ masked V blocks
-    for (int j = masked_from; j < n; ++j) {
-      const bool ok = mbar_wait(&bar->masked_full[j - masked_from], 0, abort_flag, a.err_word);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      const int s = seq_v(j) % kSlots;
-      const int key0 = (block0 + j) * kBlock;
-      if (clean_masked_values(sRing + s * kSlotBytes, max(0, row_limit(w, 0, a.causal) - key0),
-                              min(kBlock, w.keys - key0)) &&
-          lane == 0)
-        *reinterpret_cast<volatile int*>(&bar->exact_rows) = 1;
+    int seq = 0, masked = 0;
+    for (int i = 0;; ++i) {
+      Item* it = item_at(i);
+      if (!__all_sync(0xffffffffu, it != nullptr)) break;
+      const Work w = it->w;
+      const int n = item_blocks(it);
+      bool ok = true;
+      for (int j = masked_from(w, 0); ok && j < n; ++j) {
+        ok = mbar_wait(&bar->masked_full[masked % kMaskedRing], (masked / kMaskedRing) & 1, abort_flag,
+                       a.err_word);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        ++masked;
+        const int s = (seq + (j + 1 < n ? 2 * j + 2 : 2 * j + 1)) % kSlots;
+        const int key0 = j * kBlock;
+        if (clean_masked_values(sRing + s * kSlotBytes, max(0, row_limit(w, 0, a.causal) - key0),
+                                min(kBlock, w.keys - key0)) &&
+            lane == 0)
+          *reinterpret_cast<volatile int*>(&it->exact) = 1;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar->slot_full[s]);
+      }
+      if (!ok) break;
+      seq += 2 * n;
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bar->slot_full[s]);
+      if (lane == 0) done_with(i);
     }
+   }
   } else {
     // ------------------------------------------------------------ softmax
-    const int grp = warp >> 2;
+    const int t = warp >> 2;                   // this group's tile
     const int wq = warp & 3;
     const int row = wq * 32 + lane;
     const uint32_t lane_addr = static_cast<uint32_t>(wq * 32) << 16;
-    const uint32_t pair_barrier = 1 + wq;
-    const int token = row / G;
-    const bool row_valid = token < w.tokens;
-    const bool warp_active = wq * 32 < w.tokens * G;
-    const int limit = row_limit(w, token, a.causal);
-
-    float* m_buf = sX;
+    const uint32_t sbuf = tmem + lane_addr + t * 128;
+    const uint32_t obuf = tmem + lane_addr + 256 + t * 128;
+    const int token = t * tt + row / G;        // in the item
+    const int head_in_group = row - row / G * G;
     const float c = a.scale * kLog2e;
     const float2 c2 = make_float2(c, c);
-    float m_mine = -INFINITY;
-    float l = 0.f;
+    uint32_t seen = 0, outs = 0;               // sub-blocks, outputs
     bool ok = true;
-    for (int j = grp; ok && j < n; j += 2) {
-      const int sb = j % kSBuffers;
-      ok = mbar_wait(&bar->s_full[sb], (j / kSBuffers) & 1, abort_flag, a.err_word);
-      if (!ok) break;
-      tc_fence_after();
-      const uint32_t sbuf = tmem + lane_addr + sb * 128;
-      const bool partial = j >= masked_from;
-      const int64_t valid = limit - (block0 + j) * kBlock;
-      uint32_t keep[kKeptChunks<128>][32];
-      const float mrow = warp_active ? row_max<128>(sbuf, partial, valid, keep) * c : -INFINITY;
-      float m_prev = -INFINITY;
-      if (j > 0) {
-        ok = mbar_wait(&bar->m_full[(j - 1) & 1], ((j - 1) >> 1) & 1, abort_flag, a.err_word);
-        if (!ok) break;
-        m_prev = m_buf[((j - 1) & 1) * 128 + row];
-      }
-      const bool need = mrow > m_prev + kRescaleThreshold;
-      const float m_used = need ? mrow : m_prev;
-      m_buf[(j & 1) * 128 + row] = m_used;
-      mbar_arrive(&bar->m_full[j & 1]);
-      if (warp_active) {
-        // -inf stands for "no key yet": the sum is 0 and the row's exponents
-        // (all -inf) are taken against 0.
-        l = m_mine == -INFINITY ? 0.f : l * ex2_approx(m_mine - m_used);
-        m_mine = m_used;
-        const float neg = m_used == -INFINITY ? 0.f : -m_used;
-        const float2 rs =
-            row_exp<128, 0>(sbuf, partial, valid, c2, make_float2(neg, neg), keep);
-        l += rs.x + rs.y;
-      }
-      if (j > 0 && __any_sync(0xffffffffu, need)) {
-        ok = mbar_wait(&bar->o_done[(j - 1) % kSBuffers], ((j - 1) / kSBuffers) & 1, abort_flag,
-                       a.err_word);
-        if (!ok) break;
+    for (int i = 0; ok; ++i) {
+      Item* it = item_at(i);
+      if (!__all_sync(0xffffffffu, it != nullptr)) break;
+      const Work w = it->w;
+      const int n = t ? it->n[1] : it->n[0];
+      const int head = it->hk * G + head_in_group;
+      const int from = row_limit(w, t * tt, a.causal) / kSub;   // first sub-block not seen whole
+      // rows past the tile's tokens x heads (row / G >= tt) belong to no query
+      const int limit = row < tt * G ? row_limit(w, token, a.causal) : 0;
+      const bool warp_active = wq * 32 < min(tt, w.tokens - t * tt) * G;
+      float m = -INFINITY, l = 0.f;
+      for (int u = 0; u < n; ++u, ++seen) {
+        const uint32_t b = seen & 1;
+        ok = mbar_wait(&bar->s_full[t][b], (seen >> 1) & 1, abort_flag, a.err_word);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
         tc_fence_after();
         if (warp_active) {
-          const float p_scale = need ? ex2_approx(m_prev - m_used) : 1.f;
+          const uint32_t buf = sbuf + b * kSub;
+          uint32_t r[2][32];
+          tmem_ld_32x32b_x32(buf, r[0]);
+          tmem_ld_32x32b_x32(buf + 32, r[1]);
+          tmem_wait_ld();
+          reg_fence<32>(r[0]);
+          reg_fence<32>(r[1]);
+          if (u >= from) {
+            const int64_t valid = limit - u * kSub;
+            mask_chunk(r[0], 0, valid);
+            mask_chunk(r[1], 32, valid);
+          }
+          float m8[8];
+#pragma unroll
+          for (int q = 0; q < 8; ++q) m8[q] = -INFINITY;
+          max_chunk(m8, r[0]);
+          max_chunk(m8, r[1]);
+          const float mrow = fmax3(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], m8[5]),
+                                   fmaxf(m8[6], m8[7])) * c;
+          const bool need = mrow > m + kRescaleThreshold;
+          if (u > 0 && __any_sync(0xffffffffu, need)) {
+            // O_t holds the keys before these relative to m, once their PV is complete.
+            ok = mbar_wait(&bar->pv_done[t], (seen - 1) & 1, abort_flag, a.err_word);
+            if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+            tc_fence_after();
+            const float f = need ? ex2_approx(m - mrow) : 1.f;
+            l *= f;
 #pragma unroll 1
-          for (int cc = 0; cc < kHeadDim / 32; ++cc) {
-            uint32_t o[32];
-            const uint32_t addr = tmem + lane_addr + kTmemO + cc * 32;
-            tmem_ld_32x32b_x32(addr, o);
+            for (int cc = 0; cc < kHeadDim / 16; ++cc) {
+              uint32_t o[16];
+              tmem_ld_32x32b_x16(obuf + cc * 16, o);
+              tmem_wait_ld();
+              reg_fence<16>(o);
+#pragma unroll
+              for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+              tmem_st_32x32b_x16(obuf + cc * 16, o);
+            }
+          }
+          if (need) m = mrow;
+          // -inf stands for "no key yet": the exponents (all -inf) are taken against 0.
+          const float neg = m == -INFINITY ? 0.f : -m;
+          const float2 neg_m = make_float2(neg, neg);
+          float2 acc[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f),
+                           make_float2(0.f, 0.f)};
+          exp_chunk<kEmulated>(r[0], c2, neg_m, acc, buf);
+          exp_chunk<kEmulated>(r[1], c2, neg_m, acc, buf + 16);
+          const float2 sum = __fadd2_rn(__fadd2_rn(acc[0], acc[1]), __fadd2_rn(acc[2], acc[3]));
+          l += sum.x + sum.y;
+          tmem_wait_st();
+          tc_fence_before();
+        }
+        mbar_arrive(&bar->p_full[t][b]);
+      }
+      if (!ok) break;
+      // ---------------------------------------------------------- epilogue
+      if (n > 0) {
+        ok = mbar_wait(&bar->o_full[t], outs & 1, abort_flag, a.err_word);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        ++outs;
+        tc_fence_after();
+      }
+      if (n > 0 && *reinterpret_cast<volatile int*>(&it->exact)) {
+        const int rows = min(tt, w.tokens - t * tt) * G;
+        for (int r = wq; r < rows; r += 4) {
+          const int64_t q_row = w.q0 + t * tt + r / G;
+          const int h = it->hk * G + r % G;
+          float4 o;
+          const float2 ml = exact_row(a, a.q + q_row * a.q_stride_t + h * a.q_stride_h, w.k0, it->hk, 0,
+                                      row_limit(w, t * tt + r / G, a.causal), c, o);
+          if constexpr (kSplit) {
+            const int64_t p = (it->part * a.q_rows + q_row) * a.heads + h;
+            *reinterpret_cast<float4*>(a.part_o + p * kHeadDim + lane * 4) = o;
+            if (lane == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * p) = ml;
+            continue;
+          }
+          const float inv = ml.y != 0.f ? 1.f / ml.y : 0.f;
+          *reinterpret_cast<uint2*>(a.out + (q_row * a.heads + h) * kHeadDim + lane * 4) =
+              make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+        }
+        mbar_arrive(&bar->o_empty[t]);
+      } else if constexpr (kSplit) {
+        const int64_t p = (it->part * a.q_rows + w.q0 + token) * a.heads + head;
+        const bool row_valid = row < tt * G && token < w.tokens;
+#pragma unroll 1
+        for (int cc = 0; cc < kHeadDim / 32; ++cc) {
+          uint32_t o[32];
+          if (n > 0 && warp_active) {
+            tmem_ld_32x32b_x32(obuf + cc * 32, o);
             tmem_wait_ld();
             reg_fence<32>(o);
+          } else {
 #pragma unroll
-            for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * p_scale);
-            tmem_st_32x32b_x32(addr, o);
+            for (int x = 0; x < 32; ++x) o[x] = 0u;
+          }
+          if (row_valid) {
+            uint4* dst = reinterpret_cast<uint4*>(a.part_o + p * kHeadDim + cc * 32);
+#pragma unroll
+            for (int x = 0; x < 8; ++x) dst[x] = make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
           }
         }
-      }
-      tmem_wait_st();
-      tc_fence_before();
-      mbar_arrive(&bar->p_full[sb]);
-    }
-    // ---------------------------------------------------------- epilogue
-    float* xs = sX;
-    named_bar_sync(pair_barrier, 64);
-    xs[grp * 128 + row] = m_mine;
-    xs[256 + grp * 128 + row] = l;
-    named_bar_sync(pair_barrier, 64);
-    const float m0 = xs[row], m1 = xs[128 + row];
-    const float m_fin = fmaxf(m0, m1);
-    float l_row = 0.f;
-    if (m0 != -INFINITY) l_row += xs[256 + row] * ex2_approx(m0 - m_fin);
-    if (m1 != -INFINITY) l_row += xs[384 + row] * ex2_approx(m1 - m_fin);
-    if (ok && n > 0) {
-      ok = mbar_wait(&bar->drain[1], 0, abort_flag, a.err_word);
-      tc_fence_after();
-    }
-    const int head0 = hk * G;
-    if (ok && n > 0 && *reinterpret_cast<volatile int*>(&bar->exact_rows)) {
-      for (int r = warp; r < w.tokens * G; r += 8) {
-        const int t = r / G, h = head0 + r % G;
-        const int end = min(row_limit(w, t, a.causal), (block0 + n) * kBlock);
-        float4 o;
-        const float2 ml = exact_row(a, a.q + (w.q0 + t) * a.q_stride_t + h * a.q_stride_h, w.k0,
-                                    hk, block0 * kBlock, end, c, o);
-        const int64_t p = (split * a.q_rows + w.q0 + t) * a.heads + h;
-        *reinterpret_cast<float4*>(a.part_o + p * kHeadDim + lane * 4) = o;
-        if (lane == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * p) = ml;
-      }
-    } else if (warp_active) {
-      const int64_t p = (split * a.q_rows + w.q0 + token) * a.heads + head0 + (row - token * G);
-#pragma unroll 1
-      for (int cc = 0; cc < 2; ++cc) {
-        uint32_t o[32];
-        if (ok && n > 0) {
-          tmem_ld_32x32b_x32(tmem + lane_addr + kTmemO + grp * 64 + cc * 32, o);
-          tmem_wait_ld();
-          reg_fence<32>(o);
-        } else {
-#pragma unroll
-          for (int x = 0; x < 32; ++x) o[x] = 0u;
+        if (n > 0) {
+          tc_fence_before();
+          mbar_arrive(&bar->o_empty[t]);
         }
-        if (!row_valid) continue;
-        float4* dst = reinterpret_cast<float4*>(a.part_o + p * kHeadDim + grp * 64 + cc * 32);
+        if (row_valid) *reinterpret_cast<float2*>(a.part_ml + 2 * p) = make_float2(m, l);
+      } else {
+        // O goes out through shared memory: a thread owns a row, whose 16-byte
+        // pieces would each be a store of their own; staged, 8 lanes write 128
+        // bytes of a row.  (16 16-byte stores a thread took 9,000 cycles an item.)
+        const float inv_l = l != 0.f ? 1.f / l : 0.f;
+        const int64_t at = ((w.q0 + token) * a.heads + head) * kHeadDim;
+        const int rows = min(tt, w.tokens - t * tt) * G - wq * 32;   // of this warp
+        uint8_t* stage = smem + kStageOff + warp * kStageBytes;
 #pragma unroll
-        for (int x = 0; x < 8; ++x)
-          dst[x] = make_float4(__uint_as_float(o[4 * x]), __uint_as_float(o[4 * x + 1]),
-                               __uint_as_float(o[4 * x + 2]), __uint_as_float(o[4 * x + 3]));
+        for (int half = 0; half < 2; ++half) {
+          uint32_t o[2][32];
+          if (n > 0 && warp_active) {
+            tmem_ld_32x32b_x32(obuf + half * 64, o[0]);
+            tmem_ld_32x32b_x32(obuf + half * 64 + 32, o[1]);
+            tmem_wait_ld();
+            reg_fence<32>(o[0]);
+            reg_fence<32>(o[1]);
+          } else {
+#pragma unroll
+            for (int x = 0; x < 32; ++x) o[0][x] = o[1][x] = 0u;
+          }
+          if (half == 1 && n > 0) {
+            tc_fence_before();
+            mbar_arrive(&bar->o_empty[t]);     // O_t is in registers: its buffer is free
+          }
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            const uint32_t* v = &o[x >> 2][(x & 3) * 8];
+            *reinterpret_cast<uint4*>(stage + sw128_offset(lane, x)) = make_uint4(
+                pack_bf16x2(__uint_as_float(v[0]) * inv_l, __uint_as_float(v[1]) * inv_l),
+                pack_bf16x2(__uint_as_float(v[2]) * inv_l, __uint_as_float(v[3]) * inv_l),
+                pack_bf16x2(__uint_as_float(v[4]) * inv_l, __uint_as_float(v[5]) * inv_l),
+                pack_bf16x2(__uint_as_float(v[6]) * inv_l, __uint_as_float(v[7]) * inv_l));
+          }
+          __syncwarp();
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            const int r = x * 4 + (lane >> 3);
+            const int64_t dst = __shfl_sync(0xffffffffu, at, r);
+            if (r < rows)
+              *reinterpret_cast<uint4*>(a.out + dst + half * 64 + (lane & 7) * 8) =
+                  *reinterpret_cast<const uint4*>(stage + sw128_offset(r, lane & 7));
+          }
+          __syncwarp();
+        }
       }
-      if (row_valid && grp == 0)
-        *reinterpret_cast<float2*>(a.part_ml + 2 * p) = make_float2(m_fin, l_row);
+      __syncwarp();
+      if (lane == 0) done_with(i);
     }
   }
   tc_fence_before();
@@ -368,26 +661,39 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Joins the parts of a split row: out = sum_p 2^(m_p - m) O_p / sum_p 2^(m_p -
-// m) l_p, parts in order.  One warp a (query row, head).
+// Joins the parts of a row: out = sum_p 2^(m_p - m) O_p / sum_p 2^(m_p - m)
+// l_p, parts in order.  One warp a (query row, head).
 __global__ void __launch_bounds__(256) combine_kernel(const PackedArgs a) {
-  const int64_t row = blockIdx.x * 8ll + (threadIdx.x >> 5);
   const int64_t rows = a.q_rows * a.heads;
+  const int64_t row = blockIdx.x * 8ll + (threadIdx.x >> 5);
   if (row >= rows) return;
   const int lane = threadIdx.x & 31;
+  const int tt = 2 * a.tile_tokens;
+  const int64_t q = row / a.heads;
+  const int s = request_of_row(a.q_starts, a.requests, q);
+  if (s < 0) return;                             // reported by the main kernel
+  const int64_t begin = __ldg(a.q_starts + s);
+  const Work w = find_work(a, begin / tt + s + (q - begin) / tt, tt);
+  if (w.tokens == 0) return;
+  const int parts = parts_of(item_blocks(w, a.causal), a.splits);
+  const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + row;
+  const float4* po = reinterpret_cast<const float4*>(a.part_o + row * kHeadDim) + lane;
   float m = -INFINITY;
-  for (int p = 0; p < a.splits; ++p) {
-    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * (p * rows + row));
-    if (ml.y != 0.f) m = fmaxf(m, ml.x);
+  for (int p = lane; p < parts; p += 32) {
+    const float2 x = __ldg(ml + p * rows);
+    if (x.y != 0.f) m = fmaxf(m, x.x);
   }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
   float l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int p = 0; p < a.splits; ++p) {
-    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * (p * rows + row));
-    if (ml.y == 0.f) continue;
-    const float f = ex2_approx(ml.x - m);
-    const float4 v = *reinterpret_cast<const float4*>(a.part_o + (p * rows + row) * kHeadDim + lane * 4);
-    l += ml.y * f;
+#pragma unroll 8
+  for (int p = 0; p < parts; ++p) {
+    const float2 x = __ldg(ml + p * rows);
+    const float4 v = __ldg(po + p * rows * (kHeadDim / 4));
+    const float f = x.y != 0.f ? ex2_approx(x.x - m) : 0.f;
+    // a part without a key holds zeros
+    l = fmaf(x.y, f, l);
     o.x = fmaf(v.x, f, o.x);
     o.y = fmaf(v.y, f, o.y);
     o.z = fmaf(v.z, f, o.z);
@@ -398,7 +704,8 @@ __global__ void __launch_bounds__(256) combine_kernel(const PackedArgs a) {
       make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
 }
 
-cudaError_t launch_parts(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
+template <bool kSplit>
+cudaError_t launch_tiles(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                          const PackedArgs& a, cudaStream_t stream) {
   static std::atomic<int> smem_bytes[64] = {};
   int dev = 0;
@@ -411,33 +718,35 @@ cudaError_t launch_parts(const CUtensorMap& tq, const CUtensorMap& tk, const CUt
     if (e != cudaSuccess) return e;
     bytes = optin < kUsed + 1024 ? optin : kUsed + 1024;
     if (bytes < kUsed) return cudaErrorInvalidConfiguration;
-    e = cudaFuncSetAttribute(packed_attention_split_kernel,
+    e = cudaFuncSetAttribute(packed_attention_tiles_kernel<kSplit>,
                              cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64) smem_bytes[dev].store(bytes, std::memory_order_release);
   }
-  const int64_t grid = a.slots * a.kv_heads * a.splits;
-  packed_attention_split_kernel<<<static_cast<unsigned>(grid), kThreads, bytes, stream>>>(tq, tk, tv, a);
+  packed_attention_tiles_kernel<kSplit>
+      <<<static_cast<unsigned>(a.slots * a.kv_heads * a.splits), kThreads, bytes, stream>>>(tq, tk, tv, a);
   return cudaGetLastError();
 }
 
 }  // namespace
 
-// Parts of a tile's keys: one where the tiles alone give every SM two CTAs;
-// otherwise enough for four a SM, of 512 keys at least on the average request.
+// Parts of an item's keys: one where the items alone give every SM two;
+// otherwise parts of 4 blocks of 128 keys on the average request, up to sixteen
+// parts an SM (a part costs about a microsecond beyond its loads).
 int32_t packed_splits(int64_t q_rows, int64_t k_rows, int32_t requests, int32_t heads,
                       int32_t kv_heads, int num_sms) {
-  const int64_t ctas = (q_rows / (128 / (heads / kv_heads)) + requests) * kv_heads;
-  if (ctas >= 2 * num_sms) return 1;
-  const int64_t splits = std::min((4 * num_sms + ctas - 1) / ctas, k_rows / requests / 512);
+  const int64_t items = (q_rows / (2 * (128 / (heads / kv_heads))) + requests) * kv_heads;
+  if (items >= 2 * num_sms) return 1;
+  const int64_t splits = std::min<int64_t>((16 * num_sms + items - 1) / items,
+                                           k_rows / requests / (4 * kBlock));
   return static_cast<int32_t>(std::max<int64_t>(1, splits));
 }
 
 cudaError_t launch_packed_attention(const CUtensorMap& tq, const CUtensorMap& tk,
                                     const CUtensorMap& tv, const PackedArgs& a,
                                     cudaStream_t stream) {
-  if (a.splits == 1) return launch_packed_tiles(tq, tk, tv, a, stream);
-  const cudaError_t e = launch_parts(tq, tk, tv, a, stream);
+  if (a.splits == 1) return launch_tiles<false>(tq, tk, tv, a, stream);
+  const cudaError_t e = launch_tiles<true>(tq, tk, tv, a, stream);
   if (e != cudaSuccess) return e;
   const int64_t rows = a.q_rows * a.heads;
   combine_kernel<<<static_cast<unsigned>((rows + 7) / 8), 256, 0, stream>>>(a);

@@ -1,6 +1,5 @@
-// What the two packed attention kernels share: finding a tile's request, the
-// keys each of its rows sees, and the key-by-key way out for values that are
-// not finite.
+// Parts of packed_attention.cu: finding an item's request, the keys each of its
+// rows sees, and the key-by-key way out for values that are not finite.
 #pragma once
 
 #include "attention_softmax.cuh"
@@ -61,6 +60,30 @@ __device__ __forceinline__ Work find_work(const PackedArgs& a, int64_t slot, int
   // int: q_rows, k_rows < 2^31 - 256
   w.first_limit = a.causal ? static_cast<int>(w.q0 - qb + 1 + (ke - kb) - (qe - qb)) : w.keys;
   return w;
+}
+
+// Key blocks that the item sees.
+__device__ __forceinline__ int item_blocks(const Work& w, bool causal) {
+  return (row_limit(w, w.tokens - 1, causal) + kBlock - 1) / kBlock;
+}
+// Parts of an item of `blocks` key blocks, four blocks at least to a part.
+__device__ __forceinline__ int parts_of(int blocks, int splits) {
+  return max(1, min(splits, blocks / 4));
+}
+// Narrows `w` to one part of its keys (tokens = 0: there is no such part).
+__device__ __forceinline__ void take_part(Work& w, int part, const PackedArgs& a) {
+  if (w.tokens == 0) return;
+  const int blocks = item_blocks(w, a.causal);
+  const int parts = parts_of(blocks, a.splits);
+  if (part >= parts) {
+    w.tokens = 0;
+    return;
+  }
+  const int b0 = static_cast<int>(static_cast<int64_t>(blocks) * part / parts);
+  const int b1 = static_cast<int>(static_cast<int64_t>(blocks) * (part + 1) / parts);
+  w.k0 += static_cast<int64_t>(b0) * kBlock;
+  w.first_limit -= b0 * kBlock;
+  w.keys = min(w.keys - b0 * kBlock, (b1 - b0) * kBlock);
 }
 
 // The masked end of a block of V in shared memory (a warp): rows [real, 128)
