@@ -608,7 +608,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         // pieces would each be a store of their own; staged, 8 lanes write 128
         // bytes of a row.  (16 16-byte stores a thread took 9,000 cycles an item.)
         const float inv_l = l != 0.f ? 1.f / l : 0.f;
-        const int64_t at = ((w.q0 + token) * a.heads + head) * kHeadDim;
+        // this lane's rows of the stage (4 x + lane / 8): their offsets from the
+        // item's first output
+        const int own = ((token - t * tt) * a.heads + head_in_group) * kHeadDim;
+        int at[8];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) at[x] = __shfl_sync(0xffffffffu, own, x * 4 + (lane >> 3));
+        __nv_bfloat16* out = a.out + ((w.q0 + t * tt) * a.heads + it->hk * G) * kHeadDim + (lane & 7) * 8;
+        const float2 inv2 = make_float2(inv_l, inv_l);
         const int rows = min(tt, w.tokens - t * tt) * G - wq * 32;   // of this warp
         uint8_t* stage = smem + kStageOff + warp * kStageBytes;
 #pragma unroll
@@ -631,21 +638,22 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int x = 0; x < 8; ++x) {
             const uint32_t* v = &o[x >> 2][(x & 3) * 8];
-            *reinterpret_cast<uint4*>(stage + sw128_offset(lane, x)) = make_uint4(
-                pack_bf16x2(__uint_as_float(v[0]) * inv_l, __uint_as_float(v[1]) * inv_l),
-                pack_bf16x2(__uint_as_float(v[2]) * inv_l, __uint_as_float(v[3]) * inv_l),
-                pack_bf16x2(__uint_as_float(v[4]) * inv_l, __uint_as_float(v[5]) * inv_l),
-                pack_bf16x2(__uint_as_float(v[6]) * inv_l, __uint_as_float(v[7]) * inv_l));
+            uint32_t pk[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float2 y = __fmul2_rn(make_float2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), inv2);
+              pk[e] = pack_bf16x2(y.x, y.y);
+            }
+            *reinterpret_cast<uint4*>(stage + sw128_offset(lane, x)) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
           }
           __syncwarp();
+          uint4 line[8];
 #pragma unroll
-          for (int x = 0; x < 8; ++x) {
-            const int r = x * 4 + (lane >> 3);
-            const int64_t dst = __shfl_sync(0xffffffffu, at, r);
-            if (r < rows)
-              *reinterpret_cast<uint4*>(a.out + dst + half * 64 + (lane & 7) * 8) =
-                  *reinterpret_cast<const uint4*>(stage + sw128_offset(r, lane & 7));
-          }
+          for (int x = 0; x < 8; ++x)
+            line[x] = *reinterpret_cast<const uint4*>(stage + sw128_offset(x * 4 + (lane >> 3), lane & 7));
+#pragma unroll
+          for (int x = 0; x < 8; ++x)
+            if (x * 4 + (lane >> 3) < rows) *reinterpret_cast<uint4*>(out + at[x] + half * 64) = line[x];
           __syncwarp();
         }
       }
