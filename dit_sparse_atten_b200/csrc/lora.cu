@@ -104,10 +104,18 @@ __device__ __forceinline__ void join_slices(const LoraArgs& a, const Tile& t, co
     if (row >= t.rows) break;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     if (c < pad) {
-      for (int s = 0; s < a.slices; ++s) {
-        const float* at = part + row * stride + c;
-        const float4 p = a.slices > 1 ? peer_float4(at, s) : *reinterpret_cast<const float4*>(at);
-        v.x += p.x; v.y += p.y; v.z += p.z; v.w += p.w;
+      const float* at = part + row * stride + c;
+      if (a.slices == 1) {
+        v = *reinterpret_cast<const float4*>(at);
+      } else {
+        float4 p[kMaxSlices];                    // all on their way at once
+#pragma unroll
+        for (int s = 0; s < kMaxSlices; ++s)
+          p[s] = s < a.slices ? peer_float4(at, s) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int s = 0; s < kMaxSlices; ++s) {
+          v.x += p[s].x; v.y += p[s].y; v.z += p[s].z; v.w += p[s].w;
+        }
       }
     }
     *reinterpret_cast<uint2*>(a.workspace + (t.row + row) * a.rank_pad + c) =
