@@ -13,6 +13,7 @@ Public surface:
   build_spatial_layout                  Morton layout (``spatial.py``)
   get_backend(name, **config)           registry: "dense", "flex_reuse"
   kernels                               torch wrappers of every C entry point
+  packed_model                          several requests through the Wan blocks
 """
 
 from __future__ import annotations
