@@ -39,8 +39,6 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, int bytes,
       : "memory");
 }
 
-// Eight consecutive values starting at p, of which the first `left` exist.
-// kVec: all eight exist and p is 16-byte aligned.
 __device__ __forceinline__ void widen2(uint32_t w, float& a, float& b, __nv_bfloat16) {
   a = __uint_as_float(w << 16);
   b = __uint_as_float(w & 0xffff0000u);
@@ -64,11 +62,19 @@ __device__ __forceinline__ void narrow(float v, float* p) { *p = v; }
 __device__ __forceinline__ void narrow(float v, __nv_bfloat16* p) { *p = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void narrow(float v, __half* p) { *p = __float2half_rn(v); }
 
+// A thread's eight values of a chunk.  kVec: consecutive, all there, 16-byte
+// aligned.  Otherwise (a width that is not a multiple of 8, or rows off the
+// 16-byte grid) `es` apart, so that the block's threads read neighbouring
+// columns, and there where e * es < left (20,000 x 1,777 bf16 rows with three
+// modulations: 150 us, eight consecutive columns a thread 213).
 template <bool kVec, bool kStream, typename T>
-__device__ __forceinline__ void load8(const T* __restrict__ p, int left, float (&v)[8]) {
+__device__ __forceinline__ void load8(const T* __restrict__ p, int left, int es, float (&v)[8]) {
   if constexpr (!kVec) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = e < left ? widen(p[e]) : 0.f;
+    for (int e = 0; e < 8; ++e) {              // a column past the width reads the last one: no branches
+      const float t = widen(p[min(e * es, left - 1)]);
+      v[e] = e * es < left ? t : 0.f;
+    }
   } else if constexpr (sizeof(T) == 4) {
     const float4* q = reinterpret_cast<const float4*>(p);
     const float4 a = kStream ? __ldcs(q) : __ldg(q);
@@ -114,11 +120,11 @@ __device__ __forceinline__ void store_pairs(T* p, const float2 (&v)[4]) {
 }
 
 template <bool kVec, typename T>
-__device__ __forceinline__ void store8(T* __restrict__ p, int left, const float (&v)[8]) {
+__device__ __forceinline__ void store8(T* __restrict__ p, int left, int es, const float (&v)[8]) {
   if constexpr (!kVec) {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (e < left) narrow(v[e], p + e);
+      if (e * es < left) narrow(v[e], p + e * es);
   } else if constexpr (sizeof(T) == 4) {
     reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
     reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
@@ -131,14 +137,14 @@ __device__ __forceinline__ void store8(T* __restrict__ p, int left, const float 
 // A parameter vector of any of the three types (NormParam::dtype), the same
 // for the whole launch.
 template <bool kVec>
-__device__ __forceinline__ void load_param(const NormParam& p, int64_t offset, int left,
+__device__ __forceinline__ void load_param(const NormParam& p, int64_t offset, int left, int es,
                                            float (&v)[8]) {
   if (p.dtype == kDtypeF32)
-    load8<kVec, false>(static_cast<const float*>(p.ptr) + offset, left, v);
+    load8<kVec, false>(static_cast<const float*>(p.ptr) + offset, left, es, v);
   else if (p.dtype == kDtypeBf16)
-    load8<kVec, false>(static_cast<const __nv_bfloat16*>(p.ptr) + offset, left, v);
+    load8<kVec, false>(static_cast<const __nv_bfloat16*>(p.ptr) + offset, left, es, v);
   else
-    load8<kVec, false>(static_cast<const __half*>(p.ptr) + offset, left, v);
+    load8<kVec, false>(static_cast<const __half*>(p.ptr) + offset, left, es, v);
 }
 
 // Sum over the block, in a fixed order.  `slot` alternates between two arrays
@@ -163,7 +169,7 @@ __device__ __forceinline__ float block_sum(float v, float* slot) {
 
 // v -> norm(v) in place (columns past the width stay 0).
 template <int kChunks>
-__device__ __forceinline__ void normalise(float (&v)[kChunks][8], int first, int width, int kind,
+__device__ __forceinline__ void normalise(float (&v)[kChunks][8], int first, int es, int width, int kind,
                                           float eps, float (*slots)[32], int& turn) {
   const float inv_n = 1.f / static_cast<float>(width);
   const int stride = blockDim.x * 8;
@@ -182,7 +188,7 @@ __device__ __forceinline__ void normalise(float (&v)[kChunks][8], int first, int
     const int left = width - (first + c * stride);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      v[c][e] = e < left ? v[c][e] - mean : 0.f;
+      v[c][e] = e * es < left ? v[c][e] - mean : 0.f;
       s += v[c][e] * v[c][e];
     }
   }
@@ -195,7 +201,7 @@ __device__ __forceinline__ void normalise(float (&v)[kChunks][8], int first, int
 
 // v = v * weight + bias for the parameters that are there.
 template <bool kVec, int kChunks>
-__device__ __forceinline__ void affine(float (&v)[kChunks][8], int first, int width,
+__device__ __forceinline__ void affine(float (&v)[kChunks][8], int first, int es, int width,
                                        const NormParam& weight, const NormParam& bias) {
 #pragma unroll
   for (int c = 0; c < kChunks; ++c) {
@@ -203,12 +209,12 @@ __device__ __forceinline__ void affine(float (&v)[kChunks][8], int first, int wi
     if (col >= width) break;
     float w[8];
     if (weight.ptr != nullptr) {
-      load_param<kVec>(weight, col, width - col, w);
+      load_param<kVec>(weight, col, width - col, es, w);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[c][e] *= w[e];
     }
     if (bias.ptr != nullptr) {
-      load_param<kVec>(bias, col, width - col, w);
+      load_param<kVec>(bias, col, width - col, es, w);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[c][e] += w[e];
     }
@@ -222,7 +228,8 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_kernel(const NormAr
   __syncthreads();
   int turn = 0;
   const int64_t row = blockIdx.x;
-  const int first = threadIdx.x * 8;
+  const int first = kVec ? threadIdx.x * 8 : threadIdx.x;
+  const int es = kVec ? 1 : blockDim.x;
   const int stride = blockDim.x * 8;
   const TX* x = static_cast<const TX*>(a.x) + row * a.x_stride;
   const TY* y = static_cast<const TY*>(a.y) + row * a.y_stride;
@@ -233,8 +240,8 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_kernel(const NormAr
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[c][e] = p[c][e] = 0.f;
     if (col >= a.width) continue;
-    load8<kVec, true>(x + col, a.width - col, v[c]);
-    if (a.y != nullptr) load8<kVec, true>(y + col, a.width - col, p[c]);
+    load8<kVec, true>(x + col, a.width - col, es, v[c]);
+    if (a.y != nullptr) load8<kVec, true>(y + col, a.width - col, es, p[c]);
   }
   int64_t s = a.requests == 1 ? 0 : row;       // no row_starts: one request, or one for each row
   if (a.row_starts != nullptr) {
@@ -246,8 +253,8 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_kernel(const NormAr
   }
   if (a.y != nullptr) {
     if (a.post_kind != kNormNone) {
-      normalise<kChunks>(p, first, a.width, a.post_kind, a.eps, slots, turn);
-      affine<kVec, kChunks>(p, first, a.width, a.post_weight, a.post_bias);
+      normalise<kChunks>(p, first, es, a.width, a.post_kind, a.eps, slots, turn);
+      affine<kVec, kChunks>(p, first, es, a.width, a.post_weight, a.post_bias);
     }
     TX* r = static_cast<TX*>(a.residual) + row * a.width;
 #pragma unroll
@@ -255,14 +262,14 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_kernel(const NormAr
       const int col = first + c * stride;
       if (col >= a.width) break;
       float g[8] = {1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
-      if (a.gate.ptr != nullptr) load_param<kVec>(a.gate, s * a.gate_stride + col, a.width - col, g);
+      if (a.gate.ptr != nullptr) load_param<kVec>(a.gate, s * a.gate_stride + col, a.width - col, es, g);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[c][e] = fmaf(g[e], p[c][e], v[c][e]);
-      store8<kVec>(r + col, a.width - col, v[c]);
+      store8<kVec>(r + col, a.width - col, es, v[c]);
     }
   }
-  normalise<kChunks>(v, first, a.width, a.norm_kind, a.eps, slots, turn);
-  affine<kVec, kChunks>(v, first, a.width, a.weight, a.bias);
+  normalise<kChunks>(v, first, es, a.width, a.norm_kind, a.eps, slots, turn);
+  affine<kVec, kChunks>(v, first, es, a.width, a.weight, a.bias);
   TN* h = static_cast<TN*>(a.normed) + row * a.width;
 #pragma unroll
   for (int c = 0; c < kChunks; ++c) {
@@ -270,16 +277,16 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_kernel(const NormAr
     if (col >= a.width) break;
     float m[8];
     if (a.scale.ptr != nullptr) {
-      load_param<kVec>(a.scale, s * a.scale_stride + col, a.width - col, m);
+      load_param<kVec>(a.scale, s * a.scale_stride + col, a.width - col, es, m);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[c][e] = fmaf(v[c][e], m[e], v[c][e]);
     }
     if (a.shift.ptr != nullptr) {
-      load_param<kVec>(a.shift, s * a.shift_stride + col, a.width - col, m);
+      load_param<kVec>(a.shift, s * a.shift_stride + col, a.width - col, es, m);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[c][e] += m[e];
     }
-    store8<kVec>(h + col, a.width - col, v[c]);
+    store8<kVec>(h + col, a.width - col, es, v[c]);
   }
 }
 
@@ -288,7 +295,7 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_kernel(const NormAr
 __device__ __forceinline__ void param_pairs(const NormParam& p, int64_t offset, float absent,
                                             float2 (&v)[4]) {
   float t[8] = {absent, absent, absent, absent, absent, absent, absent, absent};
-  if (p.ptr != nullptr) load_param<true>(p, offset, 8, t);
+  if (p.ptr != nullptr) load_param<true>(p, offset, 8, 1, t);
 #pragma unroll
   for (int e = 0; e < 4; ++e) v[e] = make_float2(t[2 * e], t[2 * e + 1]);
 }
@@ -328,7 +335,8 @@ __device__ __forceinline__ float centre(float2 (&v)[kChunks][4], const bool (&mi
 
 // Many rows: a resident block takes rows blockIdx.x, + gridDim.x, ... (a run
 // of rows a block instead: 407 us for 57,600 x 5,120 bf16, against 367) and a
-// thread keeps its columns for all of them, so the modulation stays in registers, folded with the affine parameters into
+// thread keeps its columns for all of them, so the modulation stays in
+// registers, folded with the affine parameters into
 //   r = x + g * post_norm(y),   h = a * norm(r) + b,
 // and is loaded again only where the rows pass into another request.  x and y
 // rows come through a ring of bulk copies that run `stages` rows ahead.
@@ -515,8 +523,11 @@ cudaError_t launch_typed(const NormArgs& a, cudaStream_t stream, int num_sms) {
     }
   }
   // one CTA a row: few rows get a thread for every chunk, more rows fewer
-  // threads with more loads in flight each
-  int threads = a.rows <= 2 * num_sms && chunks <= 1024 ? std::max(128, round(chunks)) : 128;
+  // threads with more loads in flight each; odd widths no thread without a
+  // column (20,000 x 100: 21 us, with 128 threads 72)
+  int threads = a.rows <= 2 * num_sms && chunks <= 1024 ? std::max(128, round(chunks))
+                : kVec                                  ? 128
+                                                        : std::min(128, round(chunks));
   while (threads < 1024 && threads * (threads <= 256 ? 5 : 4) < chunks) threads *= 2;
   const int per = (chunks + threads - 1) / threads;
   if (per <= 1) start<TX, TY, TN, kVec, 1, 1024>(a, threads, stream);
