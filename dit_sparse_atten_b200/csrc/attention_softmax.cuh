@@ -41,12 +41,12 @@ __device__ __forceinline__ void max_chunk(float* m8, const uint32_t* r) {
 
 // p = 2^(s*c - m) for one chunk: packed FMA for the argument, MUFU (or, for
 // kEmulated of every 8 pairs, the FMA-pipe polynomial); the pairs are rounded
-// to bf16 (nearest even, one conversion per pair) into 16 words (exp_pack) or
-// 16 TMEM columns at pdst (exp_chunk), and summed in fp32 into four packed
-// accumulators.
+// to bf16 (nearest even, one conversion per pair) into 16 TMEM columns at
+// pdst, and summed in fp32 into four packed accumulators.
 template <int kEmulated>
-__device__ __forceinline__ void exp_pack(const uint32_t* r, float2 c2, float2 neg_m, float2* acc,
-                                         uint32_t* pk) {
+__device__ __forceinline__ void exp_chunk(const uint32_t* r, float2 c2, float2 neg_m,
+                                          float2* acc, uint32_t pdst) {
+  uint32_t pk[16];
 #pragma unroll
   for (int x = 0; x < 32; x += 2) {
     const float2 t =
@@ -61,12 +61,6 @@ __device__ __forceinline__ void exp_pack(const uint32_t* r, float2 c2, float2 ne
     acc[(x >> 1) & 3] = __fadd2_rn(acc[(x >> 1) & 3], p);
     pk[x >> 1] = pack_bf16x2(p.x, p.y);
   }
-}
-template <int kEmulated>
-__device__ __forceinline__ void exp_chunk(const uint32_t* r, float2 c2, float2 neg_m,
-                                          float2* acc, uint32_t pdst) {
-  uint32_t pk[16];
-  exp_pack<kEmulated>(r, c2, neg_m, acc, pk);
   tmem_st_32x32b_x16(pdst, pk);
 }
 

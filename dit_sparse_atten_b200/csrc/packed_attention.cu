@@ -63,10 +63,6 @@ constexpr int kMaxSlots = 5;
 template <bool kSplit>
 constexpr int kSlotsOf = kSplit ? 5 : 4;
 constexpr int kMaskedRing = 4;          // masked V blocks between the producer and warp 12
-#ifndef BSA_PACKED_EMULATED
-#define BSA_PACKED_EMULATED 0
-#endif
-constexpr int kEmulated = BSA_PACKED_EMULATED;
 constexpr int kWorkRing = 2;            // an item at work and the next
 constexpr int kWorkReaders = kSoftWarps + 4;   // and both issuers, producer, check
 constexpr int kQOff = 0;
@@ -542,8 +538,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float2 neg_m = make_float2(neg, neg);
           float2 acc[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f),
                            make_float2(0.f, 0.f)};
-          exp_chunk<kEmulated>(r[0], c2, neg_m, acc, buf);
-          exp_chunk<kEmulated>(r[1], c2, neg_m, acc, buf + 16);
+          exp_chunk<0>(r[0], c2, neg_m, acc, buf);
+          exp_chunk<0>(r[1], c2, neg_m, acc, buf + 16);
           const float2 sum = __fadd2_rn(__fadd2_rn(acc[0], acc[1]), __fadd2_rn(acc[2], acc[3]));
           l += sum.x + sum.y;
           tmem_wait_st();
