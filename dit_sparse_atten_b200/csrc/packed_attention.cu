@@ -50,13 +50,12 @@ using namespace attn;
 using namespace packed;
 
 constexpr int kSoftWarps = 8;
-constexpr int kThreads = 416;
+constexpr int kThreads = 384;
 constexpr int kMmaWarp = 8;             // and 9
 constexpr int kProducerWarp = 10;
-constexpr int kSchedWarp = 11;
-constexpr int kCheckWarp = 12;
+constexpr int kCheckWarp = 11;
+constexpr int kSub = 64;                // keys of S and of a P buffer
 constexpr int kLate = 2;                // key blocks left to load of an item when the next is asked for
-constexpr int kSub = 64;                // keys of an S buffer
 // Ring slots; parts of keys are bound by HBM and stage no output, which leaves
 // room for one more.
 constexpr int kMaxSlots = 5;
@@ -64,13 +63,12 @@ template <bool kSplit>
 constexpr int kSlotsOf = kSplit ? 5 : 4;
 constexpr int kMaskedRing = 4;          // masked V blocks between the producer and warp 12
 constexpr int kWorkRing = 2;            // an item at work and the next
-constexpr int kWorkReaders = kSoftWarps + 4;   // and both issuers, producer, check
+constexpr int kWorkReaders = kSoftWarps + 3;   // and both issuers, check
 constexpr int kQOff = 0;
 constexpr int kRingOff = 2 * kSlotBytes;
 constexpr int kStageOff = kRingOff + kSlotsOf<false> * kSlotBytes;
 constexpr int kStageBytes = 32 * 128;   // of each softmax warp: 64 features of its 32 rows
-constexpr int kBarOff = kStageOff + kSoftWarps * kStageBytes;
-static_assert(kBarOff == kRingOff + kSlotsOf<true> * kSlotBytes, "the fifth slot takes the stage's place");
+constexpr int kBarOff = std::max(kStageOff + kSoftWarps * kStageBytes, kRingOff + kSlotsOf<true> * kSlotBytes);
 
 // An item as the scheduler publishes it.
 struct Item {
@@ -83,13 +81,11 @@ struct Item {
 
 struct Barriers {
   uint64_t q_full, q_empty;
-  uint64_t s_full[2][2], p_full[2][2];  // [tile][S buffer]
-  uint64_t pv_done[2];
+  uint64_t s_full[2], s_empty[2], p_full[2][2], pv_done[2];   // [tile][P buffer]
   uint64_t o_full[2], o_empty[2];
   uint64_t slot_full[kMaxSlots], slot_empty[kMaxSlots];
   uint64_t masked_full[kMaskedRing];    // V of a masked block, before warp 12
   uint64_t work_full[kWorkRing], work_empty[kWorkRing];
-  uint64_t nearly_done;                 // the producer is at an item's last blocks
   uint64_t next_full;                   // answer of the cluster launch control
   uint64_t drain[2];
   uint32_t tmem_base;
@@ -167,10 +163,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&bar->q_full, 1);
     mbar_init(&bar->q_empty, 2);
     for (int t = 0; t < 2; ++t) {
-      for (int b = 0; b < 2; ++b) {
-        mbar_init(&bar->s_full[t][b], 1);
-        mbar_init(&bar->p_full[t][b], 128);
-      }
+      mbar_init(&bar->s_full[t], 1);
+      mbar_init(&bar->s_empty[t], 128);
+      for (int b = 0; b < 2; ++b) mbar_init(&bar->p_full[t][b], 128);
       mbar_init(&bar->pv_done[t], 1);
       mbar_init(&bar->o_full[t], 1);
       mbar_init(&bar->o_empty[t], 128);
@@ -184,7 +179,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&bar->work_full[i], 1);
       mbar_init(&bar->work_empty[i], kWorkReaders);
     }
-    mbar_init(&bar->nearly_done, 1);
     mbar_init(&bar->next_full, 1);
     for (int t = 0; t < 2; ++t) mbar_init(&bar->drain[t], 1);
     fence_mbar_init();
@@ -208,18 +202,20 @@ __global__ void __launch_bounds__(kThreads, 1)
   // First block of the item that some row of tile t does not see whole.
   auto masked_from = [&](const Work& w, int t) { return row_limit(w, t * tt, a.causal) / kBlock; };
 
-  // Blocks of 128 keys of an item: both tiles'.
+  // Key blocks of an item: both tiles'.
   auto item_blocks = [&](const Item* it) { return (max(it->n[0], it->n[1]) + 1) / 2; };
 
   if (warp >= kSoftWarps) {
-   if (warp == kSchedWarp) {
-    // ------------------------------------------------------------ scheduler
-    // The next item is asked for when the loads of the one at work come to
-    // their last blocks: asked for earlier, an item waits here while other CTAs
-    // run out of work.
+   if (warp == kProducerWarp) {
+    // ------------------------------------------------------------ producer
+    // The next item is asked for when an item's loads come to their last
+    // blocks: asked for earlier, it would wait here while other CTAs run out
+    // of work.
     int64_t cta = blockIdx.x;
-    uint32_t answers = 0;
-    for (int i = 0;;) {
+    uint32_t asked = 0, answers = 0, armed = 0, armed_phase = 0;
+    int seq = 0, masked = 0, loads = 0;        // of K/V, of masked V, of Q
+    bool ok = true;
+    for (int i = 0; ok;) {
       Item it{};
       it.w.tokens = -1;
       if (cta >= 0) {
@@ -232,53 +228,31 @@ __global__ void __launch_bounds__(kThreads, 1)
           take_part(it.w, it.part, a);
         }
       }
-      if (it.w.tokens != 0) {
+      const Work& w = it.w;
+      if (w.tokens != 0) {
         for (int t = 0; t < 2; ++t) {
-          const int last = min(it.w.tokens, (t + 1) * tt) - 1;
-          it.n[t] = last < t * tt ? 0 : (row_limit(it.w, last, a.causal) + kSub - 1) / kSub;
+          const int last = min(w.tokens, (t + 1) * tt) - 1;
+          it.n[t] = last < t * tt ? 0 : (row_limit(w, last, a.causal) + kSub - 1) / kSub;
         }
-        bool ok = true;
         if (lane == 0) {
           const int r = i % kWorkRing;
           ok = mbar_wait(&bar->work_empty[r], ((i / kWorkRing) & 1) ^ 1, abort_flag, a.err_word);
           if (ok) {
             bar->item[r] = it;
             mbar_arrive(&bar->work_full[r]);
-            if (cta >= 0) ok = mbar_wait(&bar->nearly_done, i & 1, abort_flag, a.err_word);
           }
         }
-        ok = __shfl_sync(0xffffffffu, ok, 0);
         ++i;
-        if (cta < 0 || !ok) break;
       }
-      if (lane == 0) {
-        mbar_arrive_expect_tx(&bar->next_full, 16);
-        request_next(&bar->next, &bar->next_full);
-      }
-      if (!mbar_wait(&bar->next_full, answers & 1, abort_flag, a.err_word)) {
-        int never = 0;   // an answer is on its way into shared memory
-        mbar_wait(&bar->next_full, answers & 1, &never, a.err_word);
-        break;
-      }
-      ++answers;
-      cta = answered_next(&bar->next);
-      fence_proxy_async_smem();   // the answer is read before the next one is asked for
-      __syncwarp();
-    }
-   } else if (warp == kProducerWarp) {
-    // ------------------------------------------------------------ producer
-    if (lane == 0) {
-      uint32_t armed = 0, armed_phase = 0;
-      int seq = 0, masked = 0, loads = 0;      // of K/V, of masked V, of Q
-      bool ok = true;
-      for (int i = 0; ok; ++i) {
-        const Item* it = item_at(i);
-        if (it == nullptr) break;
-        const Work w = it->w;
-        const int hk = it->hk;
-        const int n = item_blocks(it);
-        done_with(i);
+      if (cta < 0) break;
+      if (lane == 0 && ok) {
+        const int n = w.tokens == 0 ? 0 : item_blocks(&it);
         const int from = masked_from(w, 0);
+        auto ask = [&] {
+          mbar_arrive_expect_tx(&bar->next_full, 16);
+          request_next(&bar->next, &bar->next_full);
+          ++asked;
+        };
         auto load = [&](const CUtensorMap* tm, int j, bool is_v) {
           const int s = seq % kSlots;
           const uint32_t ph = (seq / kSlots) & 1;
@@ -294,31 +268,42 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           const int row = static_cast<int>(w.k0 + static_cast<int64_t>(j) * kBlock);
           mbar_arrive_expect_tx(full, kSlotBytes);
-          tma_load_3d(dst, tm, full, 0, hk, row);
-          tma_load_3d(dst + kPanel, tm, full, 64, hk, row);
+          tma_load_3d(dst, tm, full, 0, it.hk, row);
+          tma_load_3d(dst + kPanel, tm, full, 64, it.hk, row);
           ++seq;
           return true;
         };
-        if (n <= kLate) mbar_arrive(&bar->nearly_done);
-        if (n == 0) continue;
-        ok = load(&tm_k, 0, false);
-        if (ok) ok = mbar_wait(&bar->q_empty, (loads & 1) ^ 1, abort_flag, a.err_word);
-        if (!ok) break;
-        // Rows past tt * G keep whatever the shared memory held: a row of
-        // garbage reaches only its own row of S and O, which is not stored.
-        mbar_arrive_expect_tx(&bar->q_full, static_cast<uint32_t>(tt * G) * 512u);
-        for (int t = 0; t < 2; ++t)
-          for (int p = 0; p < 2; ++p)
-            tma_load_3d(sQ + t * kSlotBytes + p * kPanel, &tm_q, &bar->q_full, p * 64, hk * G,
-                        static_cast<int>(w.q0) + t * tt);
-        ++loads;
+        if (n <= kLate) ask();
+        if (n > 0) {
+          ok = load(&tm_k, 0, false);
+          if (ok) ok = mbar_wait(&bar->q_empty, (loads & 1) ^ 1, abort_flag, a.err_word);
+          if (ok) {
+            // Rows past tt * G keep whatever the shared memory held: a row of
+            // garbage reaches only its own row of S and O, which is not stored.
+            mbar_arrive_expect_tx(&bar->q_full, static_cast<uint32_t>(tt * G) * 512u);
+            for (int t = 0; t < 2; ++t)
+              for (int p = 0; p < 2; ++p)
+                tma_load_3d(sQ + t * kSlotBytes + p * kPanel, &tm_q, &bar->q_full, p * 64, it.hk * G,
+                            static_cast<int>(w.q0) + t * tt);
+            ++loads;
+          }
+        }
         for (int j = 0; ok && j < n; ++j) {
-          if (n > kLate && j == n - kLate) mbar_arrive(&bar->nearly_done);
-          if (j + 1 < n) ok = load(&tm_k, j + 1, false);
+          if (n > kLate && j == n - kLate) ask();
+          if (j > 0) ok = load(&tm_k, j, false);
           if (ok) ok = load(&tm_v, j, true);
         }
+        if (ok) ok = mbar_wait(&bar->next_full, answers & 1, abort_flag, a.err_word);
+        if (ok) ++answers;
       }
-      // Never leave a copy in flight into shared memory.
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      if (!ok) break;
+      cta = answered_next(&bar->next);
+      fence_proxy_async_smem();     // the answer is read before the next one is asked for
+      __syncwarp();
+    }
+    if (lane == 0) {
+      // Never leave a copy, or an answer, in flight into shared memory.
       int never = 0;
 #pragma unroll
       for (int s = 0; s < kSlots; ++s)
@@ -327,6 +312,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int j = max(0, masked - kMaskedRing); j < masked; ++j)
         mbar_wait(&bar->masked_full[j % kMaskedRing], (j / kMaskedRing) & 1, &never, a.err_word);
       if (loads) mbar_wait(&bar->q_full, (loads - 1) & 1, &never, a.err_word);
+      if (asked != answers) mbar_wait(&bar->next_full, answers & 1, &never, a.err_word);
     }
    } else if (warp == kMmaWarp || warp == kMmaWarp + 1) {
     // ------------------------------------------------------------ MMA issuers
@@ -357,20 +343,42 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (++slot == kSlots) slot = 0, ring_phase ^= 1;
         return s;
       };
-      // S of keys 64 half .. of the K block in slot s, into the next buffer.
+      // S of keys 64 half .. of the K block in slot s, once the softmax has read
+      // the S before.
       auto issue_s = [&](int s, int half) {
+        if (!(ok = wait(&bar->s_empty[t], (scored & 1) ^ 1))) return;
+        ++scored;
+        tc_fence_after();
         const uint64_t kd = kdesc0 + static_cast<uint64_t>((s * kSlotBytes + half * kSub * 128) >> 4);
-        const uint32_t b = scored & 1;
         if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < kHeadDim / 16; ++kk) {
             const uint64_t off = static_cast<uint64_t>(((kk >> 2) * kPanel + (kk & 3) * 32) >> 4);
-            umma_bf16_ss(s_tmem + b * kSub, qdesc + off, kd + off, idesc_s, kk > 0 ? 1u : 0u);
+            umma_bf16_ss(s_tmem, qdesc + off, kd + off, idesc_s, kk > 0 ? 1u : 0u);
           }
-          umma_commit(&bar->s_full[t][b]);
+          umma_commit(&bar->s_full[t]);
         }
         __syncwarp();
-        ++scored;
+      };
+      // O += P V for sub-block u, half of the V block in slot s.
+      auto issue_pv = [&](int s, int half, int u, bool last) {
+        // the first PV of an item overwrites the O that the softmax group stores
+        if (u == 0 && !(ok = wait(&bar->o_empty[t], (outs & 1) ^ 1))) return;
+        const uint32_t b = used & 1;
+        if (!(ok = wait(&bar->p_full[t][b], (used >> 1) & 1))) return;
+        ++used;
+        tc_fence_after();
+        const uint64_t vd = vdesc0 + static_cast<uint64_t>((s * kSlotBytes + half * kSub * 128) >> 4);
+        if (elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < kSub / 16; ++kk)
+            umma_bf16_ts(o_tmem, s_tmem + kSub + b * (kSub / 2) + kk * 8,
+                         vd + static_cast<uint64_t>((kk * 16 * 128) >> 4), idesc_o, (u > 0 || kk > 0) ? 1u : 0u);
+          umma_commit(&bar->pv_done[t]);
+          if (last) umma_commit(&bar->o_full[t]);
+        }
+        __syncwarp();
+        if (last) ++outs;
       };
       for (int i = 0; ok; ++i) {
         const Item* it = item_at(i);
@@ -387,46 +395,29 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++loads;
         tc_fence_after();
         if (mine > 0) issue_s(sk, 0);
-        if (mine > 1) issue_s(sk, 1);
-        commit(&bar->slot_empty[sk]);
-        if (mine <= 2) commit(&bar->q_empty);
-        for (int j = 0; ok && j < n; ++j) {
+        if (!ok) break;
+        if (mine <= 1) commit(&bar->q_empty);
+        for (int j = 0; j < n; ++j) {
+          // sub-block u's PV behind S of the next, whose softmax is first
+          const int u = 2 * j;
+          if (u + 1 < mine) issue_s(sk, 1);
+          if (!ok) break;
+          commit(&bar->slot_empty[sk]);
+          if (u + 2 == mine) commit(&bar->q_empty);
+          const int sv = next_slot();
+          if (!ok) break;
+          if (u < mine) issue_pv(sv, 0, u, u + 1 == mine);
+          if (!ok) break;
           if (j + 1 < n) {
             sk = next_slot();
             if (!ok) break;
-          }
-          const int sv = next_slot();
-          if (!ok) break;
-          const uint64_t vd = vdesc0 + static_cast<uint64_t>((sv * kSlotBytes) >> 4);
-#pragma unroll 1
-          for (int half = 0; half < 2; ++half) {
-            const int u = 2 * j + half;
-            if (u >= mine) break;
-            // the first PV of an item overwrites the O that the softmax group stores
-            if (u == 0 && !(ok = wait(&bar->o_empty[t], (outs & 1) ^ 1))) break;
-            const uint32_t b = used & 1;
-            if (!(ok = wait(&bar->p_full[t][b], (used >> 1) & 1))) break;
-            tc_fence_after();
-            if (elect_one()) {
-#pragma unroll
-              for (int kk = 0; kk < kSub / 16; ++kk)
-                umma_bf16_ts(o_tmem, s_tmem + b * kSub + kk * 8,
-                             vd + static_cast<uint64_t>(((half * kSub + kk * 16) * 128) >> 4), idesc_o,
-                             (u > 0 || kk > 0) ? 1u : 0u);
-              umma_commit(&bar->pv_done[t]);
-            }
-            __syncwarp();
-            ++used;
-            if (u + 1 == mine) {
-              commit(&bar->o_full[t]);
-              ++outs;
-            }
-            if (u + 2 < mine) issue_s(sk, half);
+            if (u + 2 < mine) issue_s(sk, 0);
+            if (!ok) break;
             if (u + 3 == mine) commit(&bar->q_empty);
           }
+          if (u + 1 < mine) issue_pv(sv, 1, u + 1, u + 2 == mine);
           if (!ok) break;
           commit(&bar->slot_empty[sv]);
-          if (j + 1 < n) commit(&bar->slot_empty[sk]);
         }
       }
       int never = 0;
@@ -448,7 +439,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         ++masked;
-        const int s = (seq + (j + 1 < n ? 2 * j + 2 : 2 * j + 1)) % kSlots;
+        const int s = (seq + 2 * j + 1) % kSlots;
         const int key0 = j * kBlock;
         if (clean_masked_values(sRing + s * kSlotBytes, max(0, row_limit(w, 0, a.causal) - key0),
                                 min(kBlock, w.keys - key0)) &&
@@ -489,33 +480,35 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool warp_active = wq * 32 < min(tt, w.tokens - t * tt) * G;
       float m = -INFINITY, l = 0.f;
       for (int u = 0; u < n; ++u, ++seen) {
-        const uint32_t b = seen & 1;
-        ok = mbar_wait(&bar->s_full[t][b], (seen >> 1) & 1, abort_flag, a.err_word);
+        ok = mbar_wait(&bar->s_full[t], seen & 1, abort_flag, a.err_word);
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
         tc_fence_after();
         if (warp_active) {
-          const uint32_t buf = sbuf + b * kSub;
-          uint32_t r[2][32];
-          tmem_ld_32x32b_x32(buf, r[0]);
-          tmem_ld_32x32b_x32(buf + 32, r[1]);
+          uint32_t r[kSub];
+          tmem_ld_32x32b_x32(sbuf, r);
+          tmem_ld_32x32b_x32(sbuf + 32, r + 32);
           tmem_wait_ld();
-          reg_fence<32>(r[0]);
-          reg_fence<32>(r[1]);
+          reg_fence<kSub>(r);
+          tc_fence_before();
+          mbar_arrive(&bar->s_empty[t]);
           if (u >= from) {
-            const int64_t valid = limit - u * kSub;
-            mask_chunk(r[0], 0, valid);
-            mask_chunk(r[1], 32, valid);
+            const int valid = limit - u * kSub;
+#pragma unroll
+            for (int x = 0; x < kSub; ++x)
+              if (x >= valid) r[x] = __float_as_uint(-INFINITY);
           }
           float m8[8];
 #pragma unroll
-          for (int q = 0; q < 8; ++q) m8[q] = -INFINITY;
-          max_chunk(m8, r[0]);
-          max_chunk(m8, r[1]);
+          for (int q = 0; q < 8; ++q) m8[q] = fmaxf(__uint_as_float(r[2 * q]), __uint_as_float(r[2 * q + 1]));
+#pragma unroll
+          for (int x = 16; x < kSub; x += 16)
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+              m8[q] = fmax3(m8[q], __uint_as_float(r[x + 2 * q]), __uint_as_float(r[x + 2 * q + 1]));
           const float mrow = fmax3(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], m8[5]),
                                    fmaxf(m8[6], m8[7])) * c;
           const bool need = mrow > m + kRescaleThreshold;
           if (u > 0 && __any_sync(0xffffffffu, need)) {
-            // O_t holds the keys before these relative to m, once their PV is complete.
             ok = mbar_wait(&bar->pv_done[t], (seen - 1) & 1, abort_flag, a.err_word);
             if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
             tc_fence_after();
@@ -538,14 +531,24 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float2 neg_m = make_float2(neg, neg);
           float2 acc[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f),
                            make_float2(0.f, 0.f)};
-          exp_chunk<0>(r[0], c2, neg_m, acc, buf);
-          exp_chunk<0>(r[1], c2, neg_m, acc, buf + 16);
+          uint32_t pk[kSub / 2];
+#pragma unroll
+          for (int x = 0; x < kSub; x += 2) {
+            const float2 e =
+                __ffma2_rn(make_float2(__uint_as_float(r[x]), __uint_as_float(r[x + 1])), c2, neg_m);
+            const float2 p = make_float2(ex2_approx(e.x), ex2_approx(e.y));
+            acc[(x >> 1) & 3] = __fadd2_rn(acc[(x >> 1) & 3], p);
+            pk[x >> 1] = pack_bf16x2(p.x, p.y);
+          }
+          tmem_st_32x32b_x32(sbuf + kSub + (seen & 1) * 32, pk);
           const float2 sum = __fadd2_rn(__fadd2_rn(acc[0], acc[1]), __fadd2_rn(acc[2], acc[3]));
           l += sum.x + sum.y;
           tmem_wait_st();
           tc_fence_before();
+        } else {
+          mbar_arrive(&bar->s_empty[t]);
         }
-        mbar_arrive(&bar->p_full[t][b]);
+        mbar_arrive(&bar->p_full[t][seen & 1]);
       }
       if (!ok) break;
       // ---------------------------------------------------------- epilogue
