@@ -1050,7 +1050,7 @@ int bsa_lora_add(const void* y, int64_t y_stride, const void* x, int64_t x_strid
 namespace {
 
 int64_t packed_workspace(int64_t q_rows, int32_t heads, int32_t splits) {
-  return splits > 1 ? q_rows * heads * splits * (128 + 2) * 4 : 0;
+  return splits > 1 ? q_rows * heads * 2 * splits * (128 + 2) * 4 : 0;
 }
 
 // Map over [rows, heads, 128] with element strides; box: 64 features x
@@ -1077,7 +1077,7 @@ int64_t bsa_packed_attention_workspace_bytes(int64_t q_rows, int64_t k_rows, int
       heads % kv_heads != 0 || heads / kv_heads > 128)
     return 0;
   return packed_workspace(
-      q_rows, heads, bsa::packed_splits(q_rows, k_rows, requests, heads, kv_heads, sm_count()));
+      q_rows, heads, bsa::packed_plan(q_rows, k_rows, requests, heads, kv_heads, sm_count()).splits);
 }
 
 int bsa_packed_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k,
@@ -1144,7 +1144,9 @@ int bsa_packed_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h, 
   a.group = heads / kv_heads;
   a.tile_tokens = 128 / a.group;
   a.slots = q_rows / (2 * a.tile_tokens) + requests;
-  a.splits = bsa::packed_splits(q_rows, k_rows, requests, heads, kv_heads, sm_count());
+  const bsa::PackedPlan plan = bsa::packed_plan(q_rows, k_rows, requests, heads, kv_heads, sm_count());
+  a.splits = plan.splits;
+  a.part_blocks = plan.part_blocks;
   a.causal = causal != 0;
   a.scale = scale;
   a.out = static_cast<__nv_bfloat16*>(out);
@@ -1153,7 +1155,7 @@ int bsa_packed_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h, 
     return fail(BSA_ERR_INVALID_ARGUMENT, "workspace of %lld bytes needed (got %lld)",
                 static_cast<long long>(need), static_cast<long long>(workspace_bytes));
   a.part_o = static_cast<float*>(workspace);
-  a.part_ml = need > 0 ? a.part_o + q_rows * heads * a.splits * 128 : nullptr;
+  a.part_ml = need > 0 ? a.part_o + q_rows * heads * 2 * a.splits * 128 : nullptr;
   a.err_word = err_word;
   if (a.slots * kv_heads * a.splits > 0x7fffffff)
     return fail(BSA_ERR_UNSUPPORTED, "too many query tiles");

@@ -276,16 +276,20 @@ struct PackedArgs {
   int32_t group;                // heads / kv_heads <= 128
   int32_t tile_tokens;          // 128 / group
   int64_t slots;                // q_rows / (2 tile_tokens) + requests
-  int32_t splits;
+  int32_t splits;               // parts of an item's keys, at most
+  int32_t part_blocks;          // 128-key blocks of a part, at least
   bool causal;
   float scale;
   __nv_bfloat16* out;           // [q_rows, heads, 128] contiguous
-  float* part_o;                // [splits, q_rows, heads, 128] (splits > 1)
-  float* part_ml;               // [splits, q_rows, heads, 2]: stabiliser (log2), sum
+  float* part_o;                // [2 splits, q_rows, heads, 128] (splits > 1)
+  float* part_ml;               // [2 splits, q_rows, heads, 2]: stabiliser (log2), sum
   int* err_word;
 };
-int32_t packed_splits(int64_t q_rows, int64_t k_rows, int32_t requests, int32_t heads,
-                      int32_t kv_heads, int num_sms);
+struct PackedPlan {
+  int32_t splits, part_blocks;  // as in PackedArgs
+};
+PackedPlan packed_plan(int64_t q_rows, int64_t k_rows, int32_t requests, int32_t heads,
+                       int32_t kv_heads, int num_sms);
 cudaError_t launch_packed_attention(const CUtensorMap& tm_q, const CUtensorMap& tm_k,
                                     const CUtensorMap& tm_v, const PackedArgs& args,
                                     cudaStream_t stream);

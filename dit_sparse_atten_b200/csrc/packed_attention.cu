@@ -16,24 +16,43 @@
 // keys.
 //   warps 0-3, 4-7   softmax of tile 0, 1: 64 keys at a time, one row a thread,
 //               log2 domain, a stabiliser that moves only past 2^8 (then O_t is
-//               rescaled in TMEM), P as bf16 into the first half of S's columns
-//   warps 8, 9  MMA issuers, one thread for each tile t: for each 64 keys u,
-//               O_t += P_t(u) V(u), then S_t(u + 2) = Q_t K(u + 2)^T; warp 8
+//               rescaled in TMEM); P is rounded to bf16, the tensor cores'
+//               operand, its row sum is taken before the rounding
+//   warps 8, 9  MMA issuers, one warp for each tile t: for each 64 keys u,
+//               S_t(u + 1) = Q_t K(u + 1)^T, then O_t += P_t(u) V(u); warp 8
 //               owns TMEM.  A tile has its own issuer so that it never waits
 //               for the other's softmax.
-//   warp 10     TMA producer: Q; K/V blocks of 128 keys into a ring of 32 KB
-//               slots (K0, K1, V0, K2, V1, ...)
-//   warp 11     scheduler: cancels a pending CTA, looks its item up, publishes
-//   warp 12     cleans V of the masked blocks (clean_masked_values)
-// TMEM: tile t's two S buffers of 64 columns at 128 t, O_t at 256 + 128 t.
-// Two buffers of 64 keys, not one of 128: P lives in S's columns, so S of the
-// next keys waits for PV, and with one buffer the softmax waited for both (1,300
-// of 3,700 cycles a block); with two it runs while the other's PV and S do.
-// (S of 64 keys reads Q from shared memory twice as often: 1.5 times the time
-// of one product of 128, still under the softmax's.)
+//   warp 10     producer: asks for the next item, looks it up and publishes it;
+//               loads Q, and K/V blocks of 128 keys into a ring of 32 KB slots
+//               (K0, V0, K1, V1, ...)
+//   warp 11     cleans V of the masked blocks (clean_masked_values)
+// TMEM: tile t's S (64 columns) at 128 t, its two P buffers (32 columns each)
+// behind it, O_t at 256 + 128 t.  P does not lie over S, so S(u + 1) is asked
+// for as soon as the softmax has S(u) in registers, and the PV of the keys
+// before has the time of a whole softmax; S of more than 64 keys leaves no room
+// for two P.  Twelve warps leave a softmax thread 168 registers (thirteen: 128).
+//
+// Bound: the softmax warps.  64 keys of both tiles take 1,800 cycles: 1,024 of
+// exponentials, the rest the latency of loading S, the row maxima and the
+// hand-overs, which two warps a scheduler hide only in part; the products take
+// 1,250 of tensor pipe (S of 64 keys 390 where 256 would be the full rate: Q is
+// read from shared memory for every 64 keys).  Measured: 16,380 causal tokens,
+// 16 / 4 heads, 840 us, 1,310 TFLOP/s; 22,000 tokens x 40 heads against prompts
+// of up to 512, 184 us; 16 causal prompts of 4,951 tokens, 69 us.  Earlier
+// forms: P over S's own columns with two S buffers of 64 keys 940 / 200 / 71 us,
+// one S of 128 keys 957 / 240 / 108, one issuer for both tiles 1,082 / 282; with
+// the next block's S loaded ahead into registers the softmax spills (1,630 us);
+// 16 softmax warps, tiles taking turns at the exponentials, and exponentials on
+// the FMA pipe were slower too.
+//
+// Few items: the keys are cut into parts (kSplit), whose O, stabiliser and sum
+// combine_kernel joins.  An item of at most one tile's tokens is `paired`:
+// both tiles hold its queries and take alternate key blocks, each with a part of
+// its own, since one tile's softmax is slower than the loads.  Measured: 16
+// requests of one token over 250,000 keys, 40 / 8 heads, 180 us, 5.05 TB/s.
 //
 // A value of V that is not finite at a key which part of the item must not see
-// (causal) cannot be kept out of those rows by P = 0; warp 12 looks for one
+// (causal) cannot be kept out of those rows by P = 0; warp 11 looks for one
 // and, if there is, the item's rows are computed again key by key in float32.
 //
 // Every mbarrier wait is bounded (bsa::mbar_wait); on a timeout the CTA sets
@@ -61,7 +80,7 @@ constexpr int kLate = 2;                // key blocks left to load of an item wh
 constexpr int kMaxSlots = 5;
 template <bool kSplit>
 constexpr int kSlotsOf = kSplit ? 5 : 4;
-constexpr int kMaskedRing = 4;          // masked V blocks between the producer and warp 12
+constexpr int kMaskedRing = 4;          // masked V blocks between the producer and warp 11
 constexpr int kWorkRing = 2;            // an item at work and the next
 constexpr int kWorkReaders = kSoftWarps + 3;   // and both issuers, check
 constexpr int kQOff = 0;
@@ -75,8 +94,10 @@ struct Item {
   Work w;              // w.tokens < 0: no more items
   int hk;              // key head
   int n[2];            // 64-key sub-blocks of each tile
+  int blocks;          // key blocks of the item
+  int paired;          // the tiles hold the same queries, tile t key blocks t, t + 2, ...
   int part;            // of the keys
-  int exact;           // set by warp 12
+  int exact;           // set by warp 11
 };
 
 struct Barriers {
@@ -84,7 +105,7 @@ struct Barriers {
   uint64_t s_full[2], s_empty[2], p_full[2][2], pv_done[2];   // [tile][P buffer]
   uint64_t o_full[2], o_empty[2];
   uint64_t slot_full[kMaxSlots], slot_empty[kMaxSlots];
-  uint64_t masked_full[kMaskedRing];    // V of a masked block, before warp 12
+  uint64_t masked_full[kMaskedRing];    // V of a masked block, before warp 11
   uint64_t work_full[kWorkRing], work_empty[kWorkRing];
   uint64_t next_full;                   // answer of the cluster launch control
   uint64_t drain[2];
@@ -131,7 +152,7 @@ __device__ __forceinline__ int64_t answered_next(const uint4* answer) {
   return ok ? static_cast<int64_t>(x) : -1;
 }
 
-// kSplit: items are parts of the keys (find_part); O (relative to its
+// kSplit: items are parts of the keys (take_part); O (relative to its
 // stabiliser), the stabiliser and the sum go to the workspace for
 // combine_kernel.
 template <bool kSplit>
@@ -203,7 +224,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto masked_from = [&](const Work& w, int t) { return row_limit(w, t * tt, a.causal) / kBlock; };
 
   // Key blocks of an item: both tiles'.
-  auto item_blocks = [&](const Item* it) { return (max(it->n[0], it->n[1]) + 1) / 2; };
+  auto item_blocks = [&](const Item* it) { return it->blocks; };
 
   if (warp >= kSoftWarps) {
    if (warp == kProducerWarp) {
@@ -230,9 +251,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       const Work& w = it.w;
       if (w.tokens != 0) {
+        it.blocks = packed::item_blocks(w, a.causal);
+        it.paired = kSplit && w.tokens > 0 && w.tokens <= tt;
         for (int t = 0; t < 2; ++t) {
-          const int last = min(w.tokens, (t + 1) * tt) - 1;
-          it.n[t] = last < t * tt ? 0 : (row_limit(w, last, a.causal) + kSub - 1) / kSub;
+          const int last = min(w.tokens, it.paired ? tt : (t + 1) * tt) - 1;
+          const int keys = row_limit(w, last, a.causal);
+          if (!it.paired) {
+            it.n[t] = last < t * tt ? 0 : (keys + kSub - 1) / kSub;
+          } else {
+            const int before = (it.blocks - t - 1) / 2;       // blocks before this tile's last
+            it.n[t] = it.blocks <= t ? 0 : 2 * before + min(2, (keys - (2 * before + t) * kBlock + kSub - 1) / kSub);
+          }
         }
         if (lane == 0) {
           const int r = i % kWorkRing;
@@ -284,7 +313,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int t = 0; t < 2; ++t)
               for (int p = 0; p < 2; ++p)
                 tma_load_3d(sQ + t * kSlotBytes + p * kPanel, &tm_q, &bar->q_full, p * 64, it.hk * G,
-                            static_cast<int>(w.q0) + t * tt);
+                            static_cast<int>(w.q0) + (it.paired ? 0 : t * tt));
             ++loads;
           }
         }
@@ -385,6 +414,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!__all_sync(0xffffffffu, it != nullptr)) break;
         const int mine = __shfl_sync(0xffffffffu, it->n[t], 0);         // sub-blocks
         const int n = __shfl_sync(0xffffffffu, item_blocks(it), 0);
+        const bool paired = __shfl_sync(0xffffffffu, it->paired, 0) != 0;
         __syncwarp();
         if (elect_one()) done_with(i);
         if (n == 0) continue;
@@ -394,30 +424,40 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok || !(ok = wait(&bar->q_full, loads & 1))) break;
         ++loads;
         tc_fence_after();
-        if (mine > 0) issue_s(sk, 0);
+        int u = 0;                             // this tile's next sub-block
+        bool own = !paired || t == 0;          // block j is this tile's
+        if (own && mine > 0) issue_s(sk, 0);
         if (!ok) break;
-        if (mine <= 1) commit(&bar->q_empty);
+        if (mine == 0 || (own && mine == 1)) commit(&bar->q_empty);
         for (int j = 0; j < n; ++j) {
           // sub-block u's PV behind S of the next, whose softmax is first
-          const int u = 2 * j;
-          if (u + 1 < mine) issue_s(sk, 1);
+          if (own && u + 1 < mine) issue_s(sk, 1);
           if (!ok) break;
           commit(&bar->slot_empty[sk]);
-          if (u + 2 == mine) commit(&bar->q_empty);
+          if (own && u + 2 == mine) commit(&bar->q_empty);
           const int sv = next_slot();
           if (!ok) break;
-          if (u < mine) issue_pv(sv, 0, u, u + 1 == mine);
+          if (own && u < mine) issue_pv(sv, 0, u, u + 1 == mine);
           if (!ok) break;
-          if (j + 1 < n) {
+          if (!paired && j + 1 < n) {
             sk = next_slot();
             if (!ok) break;
             if (u + 2 < mine) issue_s(sk, 0);
             if (!ok) break;
             if (u + 3 == mine) commit(&bar->q_empty);
           }
-          if (u + 1 < mine) issue_pv(sv, 1, u + 1, u + 2 == mine);
+          if (own && u + 1 < mine) issue_pv(sv, 1, u + 1, u + 2 == mine);
           if (!ok) break;
           commit(&bar->slot_empty[sv]);
+          if (own) u += 2;
+          if (paired && j + 1 < n) {
+            own = ((j + 1) & 1) == t;
+            sk = next_slot();
+            if (!ok) break;
+            if (own && u < mine) issue_s(sk, 0);
+            if (!ok) break;
+            if (own && u + 1 == mine) commit(&bar->q_empty);
+          }
         }
       }
       int never = 0;
@@ -462,7 +502,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lane_addr = static_cast<uint32_t>(wq * 32) << 16;
     const uint32_t sbuf = tmem + lane_addr + t * 128;
     const uint32_t obuf = tmem + lane_addr + 256 + t * 128;
-    const int token = t * tt + row / G;        // in the item
     const int head_in_group = row - row / G * G;
     const float c = a.scale * kLog2e;
     const float2 c2 = make_float2(c, c);
@@ -474,10 +513,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Work w = it->w;
       const int n = t ? it->n[1] : it->n[0];
       const int head = it->hk * G + head_in_group;
-      const int from = row_limit(w, t * tt, a.causal) / kSub;   // first sub-block not seen whole
+      const int paired = kSplit ? it->paired : 0;
+      const int t0 = paired ? 0 : t * tt;        // first query of the tile
+      const int token = t0 + row / G;            // in the item
+      const int from = row_limit(w, t0, a.causal);   // keys that every row sees
       // rows past the tile's tokens x heads (row / G >= tt) belong to no query
       const int limit = row < tt * G ? row_limit(w, token, a.causal) : 0;
-      const bool warp_active = wq * 32 < min(tt, w.tokens - t * tt) * G;
+      const bool warp_active = wq * 32 < min(tt, w.tokens - t0) * G;
       float m = -INFINITY, l = 0.f;
       for (int u = 0; u < n; ++u, ++seen) {
         ok = mbar_wait(&bar->s_full[t], seen & 1, abort_flag, a.err_word);
@@ -491,8 +533,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           reg_fence<kSub>(r);
           tc_fence_before();
           mbar_arrive(&bar->s_empty[t]);
-          if (u >= from) {
-            const int valid = limit - u * kSub;
+          const int key0 = paired ? (u & ~1) * kBlock + t * kBlock + (u & 1) * kSub : u * kSub;
+          if (key0 + kSub > from) {
+            const int valid = limit - key0;
 #pragma unroll
             for (int x = 0; x < kSub; ++x)
               if (x >= valid) r[x] = __float_as_uint(-INFINITY);
@@ -559,15 +602,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
       }
       if (n > 0 && *reinterpret_cast<volatile int*>(&it->exact)) {
-        const int rows = min(tt, w.tokens - t * tt) * G;
+        const int rows = min(tt, w.tokens - t0) * G;
         for (int r = wq; r < rows; r += 4) {
-          const int64_t q_row = w.q0 + t * tt + r / G;
+          const int64_t q_row = w.q0 + t0 + r / G;
           const int h = it->hk * G + r % G;
           float4 o;
           const float2 ml = exact_row(a, a.q + q_row * a.q_stride_t + h * a.q_stride_h, w.k0, it->hk, 0,
-                                      row_limit(w, t * tt + r / G, a.causal), c, o);
+                                      paired && t ? 0 : row_limit(w, t0 + r / G, a.causal), c, o);
           if constexpr (kSplit) {
-            const int64_t p = (it->part * a.q_rows + q_row) * a.heads + h;
+            const int64_t p = ((it->part + paired * (it->part + t)) * a.q_rows + q_row) * a.heads + h;
             *reinterpret_cast<float4*>(a.part_o + p * kHeadDim + lane * 4) = o;
             if (lane == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * p) = ml;
             continue;
@@ -578,7 +621,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         mbar_arrive(&bar->o_empty[t]);
       } else if constexpr (kSplit) {
-        const int64_t p = (it->part * a.q_rows + w.q0 + token) * a.heads + head;
+        const int64_t p = ((it->part + paired * (it->part + t)) * a.q_rows + w.q0 + token) * a.heads + head;
         const bool row_valid = row < tt * G && token < w.tokens;
 #pragma unroll 1
         for (int cc = 0; cc < kHeadDim / 32; ++cc) {
@@ -682,7 +725,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const PackedArgs a) {
   const int64_t begin = __ldg(a.q_starts + s);
   const Work w = find_work(a, begin / tt + s + (q - begin) / tt, tt);
   if (w.tokens == 0) return;
-  const int parts = parts_of(item_blocks(w, a.causal), a.splits);
+  const int parts = parts_of(item_blocks(w, a.causal), a) * (w.tokens <= a.tile_tokens ? 2 : 1);
   const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + row;
   const float4* po = reinterpret_cast<const float4*>(a.part_o + row * kHeadDim) + lane;
   float m = -INFINITY;
@@ -737,16 +780,27 @@ cudaError_t launch_tiles(const CUtensorMap& tq, const CUtensorMap& tk, const CUt
 
 }  // namespace
 
-// Parts of an item's keys: one where the items alone give every SM two;
-// otherwise parts of 4 blocks of 128 keys on the average request, up to sixteen
-// parts an SM (a part costs about a microsecond beyond its loads).
-int32_t packed_splits(int64_t q_rows, int64_t k_rows, int32_t requests, int32_t heads,
-                      int32_t kv_heads, int num_sms) {
-  const int64_t items = (q_rows / (2 * (128 / (heads / kv_heads))) + requests) * kv_heads;
-  if (items >= 2 * num_sms) return 1;
-  const int64_t splits = std::min<int64_t>((16 * num_sms + items - 1) / items,
-                                           k_rows / requests / (4 * kBlock));
-  return static_cast<int32_t>(std::max<int64_t>(1, splits));
+// Parts of an item's keys: one where the items alone give every SM two, or an
+// average request has less than 1,024 keys; otherwise parts of part_blocks on
+// the average request, up to sixteen parts an SM (a part costs about a
+// microsecond beyond its loads).  Requests of a few tokens share a part between
+// both tiles and take parts of twice the keys (16 requests of one token over
+// 250,000 keys: 180 us, with parts of 4 blocks 187; one request of one token
+// over 16,384 keys: 33 us against 39), unless that leaves more than half of the
+// SMs without one (25 tokens of 4 requests over 33,700 keys: 45 us, with parts
+// of 4 blocks 33).
+PackedPlan packed_plan(int64_t q_rows, int64_t k_rows, int32_t requests, int32_t heads,
+                       int32_t kv_heads, int num_sms) {
+  const int32_t tile_tokens = 128 / (heads / kv_heads);
+  const int64_t items = (q_rows / (2 * tile_tokens) + requests) * kv_heads;
+  const int64_t keys = requests > 0 ? k_rows / requests : 0;
+  PackedPlan p{1, 4};
+  if (items >= 2 * num_sms || keys < 8 * kBlock) return p;
+  if (q_rows <= static_cast<int64_t>(requests) * tile_tokens && 2 * items * (keys / (8 * kBlock)) >= num_sms)
+    p.part_blocks = 8;
+  p.splits = static_cast<int32_t>(std::max<int64_t>(
+      2, std::min((16 * num_sms + items - 1) / items, keys / (p.part_blocks * kBlock))));
+  return p;
 }
 
 cudaError_t launch_packed_attention(const CUtensorMap& tq, const CUtensorMap& tk,

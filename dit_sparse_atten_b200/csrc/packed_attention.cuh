@@ -66,15 +66,15 @@ __device__ __forceinline__ Work find_work(const PackedArgs& a, int64_t slot, int
 __device__ __forceinline__ int item_blocks(const Work& w, bool causal) {
   return (row_limit(w, w.tokens - 1, causal) + kBlock - 1) / kBlock;
 }
-// Parts of an item of `blocks` key blocks, four blocks at least to a part.
-__device__ __forceinline__ int parts_of(int blocks, int splits) {
-  return max(1, min(splits, blocks / 4));
+// Parts of an item of `blocks` key blocks.
+__device__ __forceinline__ int parts_of(int blocks, const PackedArgs& a) {
+  return max(1, min(a.splits, blocks / a.part_blocks));
 }
 // Narrows `w` to one part of its keys (tokens = 0: there is no such part).
 __device__ __forceinline__ void take_part(Work& w, int part, const PackedArgs& a) {
   if (w.tokens == 0) return;
   const int blocks = item_blocks(w, a.causal);
-  const int parts = parts_of(blocks, a.splits);
+  const int parts = parts_of(blocks, a);
   if (part >= parts) {
     w.tokens = 0;
     return;
