@@ -37,8 +37,8 @@
 // hand-overs, which two warps a scheduler hide only in part; the products take
 // 1,250 of tensor pipe (S of 64 keys 390 where 256 would be the full rate: Q is
 // read from shared memory for every 64 keys).  Measured: 16,380 causal tokens,
-// 16 / 4 heads, 840 us, 1,310 TFLOP/s; 22,000 tokens x 40 heads against prompts
-// of up to 512, 184 us; 16 causal prompts of 4,951 tokens, 69 us.  Earlier
+// 16 / 4 heads, 840 us, 1,310 TFLOP/s; 21,967 tokens x 40 heads against prompts
+// of up to 512, 184 us; 16 causal prompts of 4,931 tokens, 69 us.  Earlier
 // forms: P over S's own columns with two S buffers of 64 keys 940 / 200 / 71 us,
 // one S of 128 keys 957 / 240 / 108, one issuer for both tiles 1,082 / 282; with
 // the next block's S loaded ahead into registers the softmax spills (1,630 us);
