@@ -97,7 +97,7 @@ struct Item {
   int blocks;          // key blocks of the item
   int paired;          // the tiles hold the same queries, tile t key blocks t, t + 2, ...
   int part;            // of the keys
-  int exact;           // set by warp 11
+  int exact[2];        // of each tile; set by warp 11
 };
 
 struct Barriers {
@@ -484,7 +484,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (clean_masked_values(sRing + s * kSlotBytes, max(0, row_limit(w, 0, a.causal) - key0),
                                 min(kBlock, w.keys - key0)) &&
             lane == 0)
-          *reinterpret_cast<volatile int*>(&it->exact) = 1;
+          for (int t = 0; t < 2; ++t)           // the tiles that read this block
+            if (it->paired ? (j & 1) == t : 2 * j < it->n[t])
+              *reinterpret_cast<volatile int*>(&it->exact[t]) = 1;
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar->slot_full[s]);
       }
@@ -601,14 +603,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++outs;
         tc_fence_after();
       }
-      if (n > 0 && *reinterpret_cast<volatile int*>(&it->exact)) {
+      if (n > 0 && *reinterpret_cast<volatile int*>(&it->exact[t])) {
         const int rows = min(tt, w.tokens - t0) * G;
         for (int r = wq; r < rows; r += 4) {
           const int64_t q_row = w.q0 + t0 + r / G;
           const int h = it->hk * G + r % G;
           float4 o;
-          const float2 ml = exact_row(a, a.q + q_row * a.q_stride_t + h * a.q_stride_h, w.k0, it->hk, 0,
-                                      paired && t ? 0 : row_limit(w, t0 + r / G, a.causal), c, o);
+          const float2 ml = exact_row(a, a.q + q_row * a.q_stride_t + h * a.q_stride_h, w.k0, it->hk,
+                                      paired ? t : -1, row_limit(w, t0 + r / G, a.causal), c, o);
           if constexpr (kSplit) {
             const int64_t p = ((it->part + paired * (it->part + t)) * a.q_rows + q_row) * a.heads + h;
             *reinterpret_cast<float4*>(a.part_o + p * kHeadDim + lane * 4) = o;

@@ -114,17 +114,19 @@ __device__ __forceinline__ bool clean_masked_values(uint8_t* tile, int open, int
 }
 
 // One query row key by key in float32 (a warp; lane owns 4 features): the way
-// out when V holds non-finite values at masked keys.  Returns the row's
-// stabiliser (log2 domain) and sum; o is relative to the stabiliser.
+// out when V holds non-finite values at masked keys.  Keys [0, end), of which
+// `own` >= 0 takes blocks own, own + 2, ... only.  Returns the row's stabiliser
+// (log2 domain) and sum; o is relative to the stabiliser.
 static __device__ __noinline__ float2 exact_row(const PackedArgs& a, const __nv_bfloat16* q,
-                                                int64_t k0, int head, int begin, int end, float c,
+                                                int64_t k0, int head, int own, int end, float c,
                                                 float4& o) {
   const int lane = threadIdx.x & 31;
   float qf[4], m = -INFINITY, l = 0.f;
   o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
   for (int e = 0; e < 4; ++e) qf[e] = __bfloat162float(q[lane * 4 + e]);
-  for (int j = begin; j < end; ++j) {
+  for (int j = 0; j < end; ++j) {
+    if (own >= 0 && (j / kBlock & 1) != own) continue;
     const int64_t row = k0 + j;
     const __nv_bfloat16* k = a.k + row * a.k_stride_t + head * a.k_stride_h + lane * 4;
     const __nv_bfloat16* v = a.v + row * a.v_stride_t + head * a.v_stride_h + lane * 4;
