@@ -96,11 +96,14 @@ __device__ __forceinline__ float4 peer_float4(const float* p, int rank) {
   return v;
 }
 
-// Joins the slices' partial tiles `part` (rows of pad floats, `stride` apart, in
+// Joins the slices' partial tiles `part` (rows `stride` floats apart, in
 // the shared memory of each CTA of the cluster): this CTA takes every slices-th
-// row, adds the slices in order, scales, rounds and writes u.
+// row, adds the slices in order, scales, rounds and writes u.  Columns past the
+// rank are 0, not what the padded products left there: that is 0 times x and
+// the scale, NaN where one of them is not finite, and would reach the whole row
+// through the expand's 0 columns of B.
 __device__ __forceinline__ void join_slices(const LoraArgs& a, const Tile& t, const float* part,
-                                            int pad, int stride, float scale) {
+                                            int stride, float scale) {
   if (a.slices > 1) cluster_sync(); else __syncthreads();
   const int per_row = a.rank_pad / 4;
   const int mine = static_cast<int>(blockIdx.y);
@@ -108,7 +111,7 @@ __device__ __forceinline__ void join_slices(const LoraArgs& a, const Tile& t, co
     const int row = mine + i / per_row * a.slices, c = i % per_row * 4;
     if (row >= t.rows) break;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (c < pad) {
+    if (c < a.rank) {                            // rank % 8 == 0
       const float* at = part + row * stride + c;
       if (a.slices == 1) {
         v = *reinterpret_cast<const float4*>(at);
@@ -122,9 +125,10 @@ __device__ __forceinline__ void join_slices(const LoraArgs& a, const Tile& t, co
           v.x += p[s].x; v.y += p[s].y; v.z += p[s].z; v.w += p[s].w;
         }
       }
+      v = make_float4(v.x * scale, v.y * scale, v.z * scale, v.w * scale);
     }
     *reinterpret_cast<uint2*>(a.workspace + (t.row + row) * a.rank_pad + c) =
-        make_uint2(pack_bf16x2(v.x * scale, v.y * scale), pack_bf16x2(v.z * scale, v.w * scale));
+        make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
   }
   __syncwarp();
   if (a.slices > 1) cluster_sync();   // peers may still read this CTA's tile
@@ -185,7 +189,7 @@ __global__ void __launch_bounds__(kWarps * 32) lora_shrink_few_kernel(const Lora
     for (int w = 0; w < kWarps; ++w) sum += (&part[w][0][0])[i];
     (&part[0][0][0])[i] = sum;
   }
-  join_slices(a, t, &part[0][0][0], kPad, kPad, adapter_scale(a, t.adapter));
+  join_slices(a, t, &part[0][0][0], kPad, adapter_scale(a, t.adapter));
 }
 
 // Shrink on the tensor cores (14,400 rows, K = 5,120, rank 32: 33 us for 148 MB,
@@ -321,7 +325,7 @@ __global__ void __launch_bounds__(kShrinkThreads)
     tc_fence_after();
     tmem_dealloc(tmem, kCols);
   }
-  join_slices(a, t, part, kPad, kPartStride, adapter_scale(a, t.adapter));
+  join_slices(a, t, part, kPartStride, adapter_scale(a, t.adapter));
 }
 
 // Expand for requests of few rows: out = y + u B^T for 16 rows of one request

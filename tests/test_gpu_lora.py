@@ -132,6 +132,28 @@ def test_poison_stays_in_its_request():
     assert out[40:65].isnan().all()
 
 
+@pytest.mark.parametrize("rank", [8, 24, 40, 72])
+@pytest.mark.parametrize("lengths", [[3, 2, 1], [40, 25, 130]])
+@pytest.mark.parametrize("where", ["x", "scales"])
+def test_infinities_keep_their_sign_at_padded_ranks(rank, lengths, where):
+    """Positive factors and an infinity in x, or as a scale: every result of
+    those rows is +inf, also where the kernels pad the rank."""
+    t = make(lengths, 72, 136, rank, 2, [0, 1, -1], seed=rank)
+    t["x"], t["a"], t["b"] = t["x"].abs() + 0.1, t["a"].abs() + 0.01, t["b"].abs() + 0.01
+    clean = call(t)
+    if where == "x":
+        t["x"][0, 5] = float("inf")
+        bad = slice(0, 1)
+    else:
+        t["scales"][1] = float("inf")
+        bad = slice(lengths[0], lengths[0] + lengths[1])
+    out = call(t)
+    assert torch.isposinf(out[bad]).all()
+    keep = torch.ones(sum(lengths), dtype=torch.bool)
+    keep[bad] = False
+    assert torch.equal(out[keep], clean[keep])
+
+
 def test_runs_are_identical_and_streams_agree():
     t = make([513, 100, 1], 1024, 768, 64, 3, [2, 0, 1], seed=12)
     want = call(t)
