@@ -673,13 +673,23 @@ def _call_on(device: torch.device, name: str, *args) -> None:
         _native.call(name, *args, _native.err_word(device).data_ptr(), _stream(device))
 
 
+def _saturated_i32(t: torch.Tensor, device: torch.device) -> torch.Tensor:
+    """Integers as contiguous int32 on ``device``.  int64 values that int32 does not hold
+    become its ends, which the kernels report as out of range; a plain conversion
+    would wrap them onto other rows or adapters."""
+    if t.dtype == torch.int64:
+        ends = torch.iinfo(torch.int32)
+        t = t.clamp(ends.min, ends.max)
+    return t.to(device=device, dtype=torch.int32).contiguous()
+
+
 def _starts_i32(starts: torch.Tensor, name: str, device: torch.device) -> torch.Tensor:
     """Request offsets as contiguous int32 on ``device`` (``[requests + 1]``)."""
     if starts.dim() != 1 or starts.numel() < 1:
         raise ValueError(f"{name} must be one-dimensional with requests + 1 entries")
     if starts.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"{name} must be integers")
-    return starts.to(device=device, dtype=torch.int32).contiguous()
+    return _saturated_i32(starts, device)
 
 
 def _rows_2d(t: torch.Tensor) -> torch.Tensor:
@@ -829,7 +839,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, lora_a: torch.Tensor, lora_b: tor
     requests = row_starts.numel() - 1
     if tuple(adapters.shape) != (requests,) or adapters.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"adapters must be integers [requests] = [{requests}]")
-    adapters = adapters.to(device=device, dtype=torch.int32).contiguous()
+    adapters = _saturated_i32(adapters, device)
     if scales is not None:
         if tuple(scales.shape) != (count,):
             raise ValueError(f"scales must be [count] = [{count}]")

@@ -182,6 +182,16 @@ def test_bad_offsets_and_ids_are_reported():
             call(b)
 
 
+def test_wide_ids_and_offsets_are_reported():
+    """int64 values that an int32 would wrap onto a valid adapter or row."""
+    t = make([40, 25], 64, 64, 8, 2, [0, 1], seed=14)
+    for key, bad in [("ids", [2 ** 32, 1]), ("ids", [0, -2 ** 32 + 1]), ("starts", [0, 2 ** 32 + 40, 65]),
+                     ("starts", [0, 40, 2 ** 32 + 65]), ("starts", [-2 ** 32, 40, 65])]:
+        b = dict(t, **{key: torch.tensor(bad, dtype=torch.int64, device=DEV)})
+        with pytest.raises(RuntimeError, match="out of range"):
+            call(b)
+
+
 def test_empty():
     t = make([0, 0], 64, 64, 8, 2, [0, 1])
     assert call(t).shape == (0, 64)

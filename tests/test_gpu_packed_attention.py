@@ -254,6 +254,15 @@ def test_bad_offsets_are_reported():
             call(dict(t, **{key: torch.tensor(bad, dtype=torch.int32, device=DEV)}))
 
 
+def test_wide_offsets_are_reported():
+    """int64 offsets that an int32 would wrap onto valid rows."""
+    t = make([40, 25], [40, 25], 2, 1, seed=17)
+    for key, bad in [("qs", [0, 2 ** 32 + 40, 65]), ("qs", [0, 40, 2 ** 32 + 65]), ("ks", [0, 2 ** 32 + 40, 65]),
+                     ("ks", [-2 ** 32, 40, 65])]:
+        with pytest.raises(RuntimeError, match="out of range"):
+            call(dict(t, **{key: torch.tensor(bad, dtype=torch.int64, device=DEV)}))
+
+
 def test_refusals():
     t = make([4], [4], 4, 2)
     with pytest.raises(RuntimeError, match="CUDA"):

@@ -139,3 +139,14 @@ def test_definitions():
     assert np.allclose(out[:, 0, 0], [2.0, 4.0])     # the first of two queries sees two of three keys
     out = opacked.packed_attention(q, np.zeros((1, 1, 1)), v[:1], [0, 2], [0, 1], True)
     assert np.allclose(out[:, 0, 0], [0.0, 1.0])     # no key: 0
+
+
+def test_wide_integers_do_not_wrap():
+    """int64 offsets and ids beyond int32 stay beyond every table, at its ends."""
+    import torch
+    from dit_sparse_atten_b200 import kernels
+    wide = torch.tensor([0, 7, 2 ** 32 + 4, 2 ** 31, -2 ** 32, -2 ** 31 - 1], dtype=torch.int64)
+    want = [0, 7, 2 ** 31 - 1, 2 ** 31 - 1, -2 ** 31, -2 ** 31]
+    for t in (wide, torch.stack([wide, wide], 1)[:, 1]):
+        got = kernels._starts_i32(t, "row_starts", torch.device("cpu"))
+        assert got.dtype == torch.int32 and got.is_contiguous() and got.tolist() == want
