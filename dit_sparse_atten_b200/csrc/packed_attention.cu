@@ -52,8 +52,10 @@
 // requests of one token over 250,000 keys, 40 / 8 heads, 180 us, 5.05 TB/s.
 //
 // A value of V that is not finite at a key which part of the item must not see
-// (causal) cannot be kept out of those rows by P = 0; warp 11 looks for one
-// and, if there is, the item's rows are computed again key by key in float32.
+// (causal) cannot be kept out of those rows by P = 0; warp 11 zeroes such values
+// and notes their keys, fewer than 256 an item, and the softmax warps add them
+// to the results of the rows that see them (add_not_finite).  The cost does not
+// grow with the keys' number.
 //
 // Every mbarrier wait is bounded (bsa::mbar_wait); on a timeout the CTA sets
 // kErrWaitTimeout, drains its copies and MMAs, frees TMEM and exits.
@@ -97,7 +99,7 @@ struct Item {
   int blocks;          // key blocks of the item
   int paired;          // the tiles hold the same queries, tile t key blocks t, t + 2, ...
   int part;            // of the keys
-  int exact[2];        // of each tile; set by warp 11
+  uint32_t odd[kHiddenWords];   // hidden keys with values that are not finite; set by warp 11
 };
 
 struct Barriers {
@@ -481,12 +483,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++masked;
         const int s = (seq + 2 * j + 1) % kSlots;
         const int key0 = j * kBlock;
-        if (clean_masked_values(sRing + s * kSlotBytes, max(0, row_limit(w, 0, a.causal) - key0),
-                                min(kBlock, w.keys - key0)) &&
-            lane == 0)
-          for (int t = 0; t < 2; ++t)           // the tiles that read this block
-            if (it->paired ? (j & 1) == t : 2 * j < it->n[t])
-              *reinterpret_cast<volatile int*>(&it->exact[t]) = 1;
+        clean_masked_values(sRing + s * kSlotBytes, row_limit(w, 0, a.causal) - key0,
+                            min(kBlock, w.keys - key0), it->odd);
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar->slot_full[s]);
       }
@@ -603,26 +601,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++outs;
         tc_fence_after();
       }
-      if (n > 0 && *reinterpret_cast<volatile int*>(&it->exact[t])) {
-        const int rows = min(tt, w.tokens - t0) * G;
-        for (int r = wq; r < rows; r += 4) {
-          const int64_t q_row = w.q0 + t0 + r / G;
-          const int h = it->hk * G + r % G;
-          float4 o;
-          const float2 ml = exact_row(a, a.q + q_row * a.q_stride_t + h * a.q_stride_h, w.k0, it->hk,
-                                      paired ? t : -1, row_limit(w, t0 + r / G, a.causal), c, o);
-          if constexpr (kSplit) {
-            const int64_t p = ((it->part + paired * (it->part + t)) * a.q_rows + q_row) * a.heads + h;
-            *reinterpret_cast<float4*>(a.part_o + p * kHeadDim + lane * 4) = o;
-            if (lane == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * p) = ml;
-            continue;
-          }
-          const float inv = ml.y != 0.f ? 1.f / ml.y : 0.f;
-          *reinterpret_cast<uint2*>(a.out + (q_row * a.heads + h) * kHeadDim + lane * 4) =
-              make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
-        }
-        mbar_arrive(&bar->o_empty[t]);
-      } else if constexpr (kSplit) {
+      if constexpr (kSplit) {
         const int64_t p = ((it->part + paired * (it->part + t)) * a.q_rows + w.q0 + token) * a.heads + head;
         const bool row_valid = row < tt * G && token < w.tokens;
 #pragma unroll 1
@@ -702,6 +681,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       __syncwarp();
+      if (a.causal && n > 0) {
+        const uint32_t odd = lane < kHiddenWords ? *reinterpret_cast<volatile uint32_t*>(&it->odd[lane]) : 0u;
+        if (__any_sync(0xffffffffu, odd != 0)) {
+          float* part = nullptr;
+          if constexpr (kSplit)
+            part = a.part_o + (it->part + paired * (it->part + t)) * a.q_rows * a.heads * kHeadDim;
+          add_not_finite(a, odd, w.q0 + t0, w.k0, it->hk, wq * 32, paired ? t : -1,
+                         row_limit(w, 0, a.causal), limit, m, kSplit ? 1.f : l != 0.f ? 1.f / l : 0.f, part);
+          __syncwarp();
+        }
+      }
       if (lane == 0) done_with(i);
     }
   }

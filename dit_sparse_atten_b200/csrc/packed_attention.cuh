@@ -1,5 +1,5 @@
 // Parts of packed_attention.cu: finding an item's request, the keys each of its
-// rows sees, and the key-by-key way out for values that are not finite.
+// rows sees, and values that are not finite at keys that only some rows see.
 #pragma once
 
 #include "attention_softmax.cuh"
@@ -86,67 +86,106 @@ __device__ __forceinline__ void take_part(Work& w, int part, const PackedArgs& a
   w.keys = min(w.keys - b0 * kBlock, (b1 - b0) * kBlock);
 }
 
+// Keys of an item that some of its queries see and some do not: fewer than its
+// queries, at most 256.  A bit each, from the first query's limit on.
+constexpr int kHiddenWords = 8;
+
 // The masked end of a block of V in shared memory (a warp): rows [real, 128)
 // lie past the request's end and are zeroed (0 * whatever another request
-// holds there would reach O); rows [open, real) are hidden from part of the
-// tile, and true is returned if one of them holds a value that is not finite.
-__device__ __forceinline__ bool clean_masked_values(uint8_t* tile, int open, int real) {
+// holds there would reach O).  Rows [first, real) are hidden from part of the
+// item, `first` being the first query's limit: their elements that are not
+// finite are zeroed too, and bit row - first of `odd` says that a row had one.
+__device__ __forceinline__ void clean_masked_values(uint8_t* tile, int first, int real, uint32_t* odd) {
   const int lane = threadIdx.x & 31;
   // a row is 8 chunks of 16 bytes in each panel; which of them is which (the
-  // swizzle) does not matter for zeroing or scanning a whole row
+  // swizzle) does not matter for a whole row
   for (int i = lane + real * 8; i < kBlock * 8; i += 32) {
     *reinterpret_cast<uint4*>(tile + i * 16) = make_uint4(0u, 0u, 0u, 0u);
     *reinterpret_cast<uint4*>(tile + kPanel + i * 16) = make_uint4(0u, 0u, 0u, 0u);
   }
-  bool found = false;
-  for (int i = lane + open * 8; i < real * 8; i += 32) {
-#pragma unroll
-    for (int panel = 0; panel < 2; ++panel) {
-      const uint4 x = *reinterpret_cast<const uint4*>(tile + panel * kPanel + i * 16);
-      const uint32_t words[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-      for (int p = 0; p < 4; ++p)
-        found |= (words[p] & 0x7f80u) == 0x7f80u || (words[p] & 0x7f800000u) == 0x7f800000u;
+  // First a look, without a branch (with one a word: 16 causal prompts 80 us
+  // instead of 68).  An exponent of ones, and only that, carries into the
+  // sign's place when its lowest bit is added.
+  const auto carries = [](uint32_t w) { return (w & 0x7f807f80u) + 0x00800080u; };
+  uint32_t found = 0;
+#pragma unroll 4
+  for (int i = lane + max(0, first) * 8; i < real * 8; i += 32) {
+    const uint4 x = *reinterpret_cast<const uint4*>(tile + i * 16);
+    const uint4 y = *reinterpret_cast<const uint4*>(tile + kPanel + i * 16);
+    found |= carries(x.x) | carries(x.y) | carries(x.z) | carries(x.w) | carries(y.x) | carries(y.y) |
+             carries(y.z) | carries(y.w);
+  }
+  if (__any_sync(0xffffffffu, (found & 0x80008000u) != 0)) {
+    for (int i = lane + max(0, first) * 8; i < real * 8; i += 32) {
+      bool here = false;
+      for (int p = 0; p < 8; ++p) {
+        uint32_t* at = reinterpret_cast<uint32_t*>(tile + (p & 4 ? kPanel : 0) + i * 16) + (p & 3);
+        const uint32_t bad = carries(*at) & 0x80008000u;
+        if (bad == 0) continue;
+        here = true;
+        *at &= ~(bad | (bad - (bad >> 15)));     // 0xffff for each half that carries
+      }
+      const int h = i / 8 - first;
+      if (here && h < 32 * kHiddenWords) atomicOr(odd + h / 32, 1u << (h & 31));   // past them: hidden from all
     }
   }
   fence_proxy_async_smem();
-  return __any_sync(0xffffffffu, found);
 }
 
-// One query row key by key in float32 (a warp; lane owns 4 features): the way
-// out when V holds non-finite values at masked keys.  Keys [0, end), of which
-// `own` >= 0 takes blocks own, own + 2, ... only.  Returns the row's stabiliser
-// (log2 domain) and sum; o is relative to the stabiliser.
-static __device__ __noinline__ float2 exact_row(const PackedArgs& a, const __nv_bfloat16* q,
-                                                int64_t k0, int head, int own, int end, float c,
-                                                float4& o) {
+// The zeroed elements' part of the results: a warp adds p_j v_j of the keys j in
+// `odd` (word w in lane w) to its 32 rows (a row's query sees keys [0, limit);
+// the row's limit, stabiliser m and the factor of its results are in the lane of
+// its number), for the elements that are not finite; the others went through
+// the tensor cores.  A row that sees none of those keys is not touched.  `own`
+// >= 0: keys of blocks own, own + 2, ... only.  The rows' results (float32
+// `part`, or bf16 a.out) have been written by this warp; lane owns 4 features.
+static __device__ __noinline__ void add_not_finite(const PackedArgs& a, uint32_t odd, int64_t q0,
+                                                   int64_t k0, int head, int row0, int own, int first,
+                                                   int limit, float m, float factor, float* part) {
   const int lane = threadIdx.x & 31;
-  float qf[4], m = -INFINITY, l = 0.f;
-  o = make_float4(0.f, 0.f, 0.f, 0.f);
+  const float c = a.scale * attn::kLog2e;
+  for (int x = 0; x < 32; ++x) {
+    const int end = __shfl_sync(0xffffffffu, limit, x);
+    const float m_row = __shfl_sync(0xffffffffu, m, x), f = __shfl_sync(0xffffffffu, factor, x);
+    if (end <= first) continue;
+    const int64_t q_row = q0 + (row0 + x) / a.group;
+    const int h = head * a.group + (row0 + x) % a.group;
+    const __nv_bfloat16* q = a.q + q_row * a.q_stride_t + h * a.q_stride_h + lane * 4;
+    float add[4] = {0.f, 0.f, 0.f, 0.f};
+    bool open = true;                              // an element that is not NaN yet
+    for (int w = 0; w < kHiddenWords && open; ++w) {
+      for (uint32_t bits = __shfl_sync(0xffffffffu, odd, w); bits != 0 && open; bits &= bits - 1) {
+        const int j = first + w * 32 + __ffs(bits) - 1;
+        if (j >= end) break;
+        if (own >= 0 && (j / kBlock & 1) != own) continue;
+        const __nv_bfloat16* k = a.k + (k0 + j) * a.k_stride_t + head * a.k_stride_h + lane * 4;
+        const __nv_bfloat16* v = a.v + (k0 + j) * a.v_stride_t + head * a.v_stride_h + lane * 4;
+        float s = 0.f;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) qf[e] = __bfloat162float(q[lane * 4 + e]);
-  for (int j = 0; j < end; ++j) {
-    if (own >= 0 && (j / kBlock & 1) != own) continue;
-    const int64_t row = k0 + j;
-    const __nv_bfloat16* k = a.k + row * a.k_stride_t + head * a.k_stride_h + lane * 4;
-    const __nv_bfloat16* v = a.v + row * a.v_stride_t + head * a.v_stride_h + lane * 4;
-    float s = 0.f;
+        for (int e = 0; e < 4; ++e) s = fmaf(__bfloat162float(q[e]), __bfloat162float(k[e]), s);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s = fmaf(qf[e], __bfloat162float(k[e]), s);
+        for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+        const float p = ex2_approx(fmaf(s, c, m_row == -INFINITY ? 0.f : -m_row));
+        bool nan = true;
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-    s *= c;
-    const float m_new = fmaxf(m, s);
-    const float keep = m == -INFINITY ? 0.f : ex2_approx(m - m_new);
-    const float p = m_new == -INFINITY && s == -INFINITY ? 0.f : ex2_approx(s - m_new);
-    l = l * keep + p;
-    o.x = fmaf(p, __bfloat162float(v[0]), m == -INFINITY ? 0.f : o.x * keep);
-    o.y = fmaf(p, __bfloat162float(v[1]), m == -INFINITY ? 0.f : o.y * keep);
-    o.z = fmaf(p, __bfloat162float(v[2]), m == -INFINITY ? 0.f : o.z * keep);
-    o.w = fmaf(p, __bfloat162float(v[3]), m == -INFINITY ? 0.f : o.w * keep);
-    m = m_new;
+        for (int e = 0; e < 4; ++e) {
+          const float t = __bfloat162float(v[e]);
+          if (!(fabsf(t) < INFINITY)) add[e] = fmaf(p, t, add[e]);
+          nan = nan && add[e] != add[e];
+        }
+        open = __any_sync(0xffffffffu, !nan);
+      }
+    }
+    const int64_t at = (q_row * a.heads + h) * kHeadDim + lane * 4;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (fabsf(add[e]) < INFINITY) continue;      // nothing was added
+      if (part != nullptr)
+        part[at + e] += add[e] * f;
+      else
+        a.out[at + e] = __float2bfloat16_rn(__bfloat162float(a.out[at + e]) + add[e] * f);
+    }
   }
-  return make_float2(m, l);
 }
 
 }  // namespace packed
