@@ -190,7 +190,8 @@ PyObject* lora_add(PyObject*, PyObject* const* args, Py_ssize_t n) {
       Py_RETURN_NONE;
     const int64_t rows = y->size(0), cols = y->size(1), k = x->size(1);
     if (la->dim() != 3 || !la->is_contiguous() || la->size(2) != k || lb->dim() != 3 ||
-        !lb->is_contiguous())
+        !lb->is_contiguous() || reinterpret_cast<uintptr_t>(la->data_ptr()) % 16 != 0 ||
+        reinterpret_cast<uintptr_t>(lb->data_ptr()) % 16 != 0)
       Py_RETURN_NONE;
     const int64_t count = la->size(0), rank = la->size(1);
     if (lb->size(0) != count || lb->size(1) != cols || lb->size(2) != rank || count > INT32_MAX ||

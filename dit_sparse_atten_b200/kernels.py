@@ -848,7 +848,12 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, lora_a: torch.Tensor, lora_b: tor
     def rows_8(t):
         t = _rows_2d(t)
         ok = t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0
-        return t if ok else t.contiguous().clone() if t.data_ptr() % 16 else t.contiguous()
+        # contiguous() keeps the stride of a single row, whatever it is
+        return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+    def factors(t):
+        t = t.contiguous()
+        return t if t.data_ptr() % 16 == 0 else t.clone()
 
     if out is None:
         out = torch.empty(y.shape, dtype=y.dtype, device=device)
@@ -864,14 +869,15 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, lora_a: torch.Tensor, lora_b: tor
         yr = o if out is y else rows_8(y)
     xr = rows_8(x)
     rows = xr.shape[0]
+    y_stride, out_stride = (yr.stride(0), o.stride(0)) if rows > 1 else (N, N)
     if rows and N:
-        lora_a, lora_b = lora_a.contiguous(), lora_b.contiguous()
+        lora_a, lora_b = factors(lora_a), factors(lora_b)
         nbytes = _native.load_library().bsa_lora_add_workspace_bytes(rows, requests, K, R)
         work = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        _call_on(device, "bsa_lora_add", yr.data_ptr(), yr.stride(0), xr.data_ptr(), xr.stride(0),
+        _call_on(device, "bsa_lora_add", yr.data_ptr(), y_stride, xr.data_ptr(), xr.stride(0),
                  lora_a.data_ptr(), lora_b.data_ptr(), _native.ptr(scales),
                  row_starts.data_ptr(), adapters.data_ptr(), rows, requests, count, K, N, R,
-                 work.data_ptr(), nbytes, o.data_ptr(), o.stride(0))
+                 work.data_ptr(), nbytes, o.data_ptr(), out_stride)
     return out
 
 

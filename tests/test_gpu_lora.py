@@ -122,6 +122,34 @@ def test_strided_inputs():
     check(call(t), t)
 
 
+@pytest.mark.parametrize("rows", [1, 2, 40])
+def test_slices_of_odd_widths(rows):
+    """Rows, and a single row, cut out of wider tensors of odd widths."""
+    t = make([rows], 256, 264, 16, 1, [0], seed=20)
+    want = call(t)
+    wide = {k: torch.zeros((rows, t[k].shape[1] + 11), dtype=torch.bfloat16, device=DEV) for k in "xy"}
+    for shift in (0, 3, 8):
+        views = {k: wide[k][:, shift:shift + t[k].shape[1]] for k in "xy"}
+        for k in "xy":
+            views[k].copy_(t[k])
+        assert torch.equal(call(dict(t, **views)), want)
+        if rows == 1 and shift != 3:
+            into = torch.zeros((1, 275), dtype=torch.bfloat16, device=DEV)[:, shift:shift + 264]
+            assert torch.equal(call(dict(t, **views), out=into), want) and torch.equal(into, want)
+            assert torch.equal(call(dict(t, **views), out=views["y"]), want)
+            assert torch.equal(views["y"], want)
+
+
+def test_factors_off_the_16_byte_grid():
+    t = make([33, 90], 256, 264, 16, 2, [1, 0], seed=21)
+    want = call(t)
+
+    def shifted(f):
+        return torch.cat([f.new_zeros(3), f.flatten()])[3:].view(f.shape)
+    for keys in ("a", "b", "ab"):
+        assert torch.equal(call(dict(t, **{k: shifted(t[k]) for k in keys})), want)
+
+
 def test_poison_stays_in_its_request():
     t = make([40, 25, 3], 320, 264, 32, 2, [0, 1, 0], seed=10)
     clean = call(t)
