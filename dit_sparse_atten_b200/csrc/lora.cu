@@ -265,21 +265,19 @@ __global__ void __launch_bounds__(kShrinkThreads)
   const uint32_t tmem = bar->tmem_base;
   if (warp == 0) {
     if (lane == 0) {
-      bool ok = true;
-      int i = 0;
-      for (; i < n; ++i) {
-        const int s = i % kStages;
-        ok = mbar_wait(&bar->empty[s], ((i / kStages) & 1) ^ 1, abort_flag, a.err_word);
-        if (!ok) break;
+      LoadRing<kStages> loads;
+      for (int i = 0; i < n; ++i) {
+        const int s = loads.slot();
+        if (!mbar_wait(&bar->empty[s], loads.empty_parity(), abort_flag, a.err_word)) break;
         uint8_t* dst = ring + s * kStage;
         mbar_arrive_expect_tx(&bar->full[s], kStage);
         tma_load_2d(dst, &tm_x, &bar->full[s], (s0 + i) * 64, static_cast<int>(t.row));
         tma_load_3d(dst + kXBytes, &tm_a, &bar->full[s], (s0 + i) * 64, 0, t.adapter);
+        loads.arm();
       }
       // Never leave a copy in flight into shared memory.
       int never = 0;
-      for (int j = i > kStages ? i - kStages : 0; j < i; ++j)
-        mbar_wait(&bar->full[j % kStages], (j / kStages) & 1, &never, a.err_word);
+      loads.for_each_open([&](int s, uint32_t parity) { mbar_wait(&bar->full[s], parity, &never, a.err_word); });
     }
   } else if (warp == 1) {
     if (lane == 0) {
@@ -547,15 +545,16 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
   bool changed;
   if (warp == 0) {
     // -------------------------------------------------------------- producer
-    int i = 0, u = 0;           // tiles and row tiles (with an adapter) loaded
+    LoadRing<L::kStages> tiles;
+    LoadRing<L::kUBuffers> us;      // u of row tiles with an adapter
     bool ok = true, waited = false;
-    for (int c; ok && (c = walk.next(a, changed)) >= 0; ++i) {
+    for (int c; ok && (c = walk.next(a, changed)) >= 0;) {
       const bool has = walk.tile.adapter >= 0;
-      const int s = i % L::kStages;
+      const int s = tiles.slot();
       uint8_t* dst = smem + s * L::kStage;
       const int row = static_cast<int>(walk.tile.row);
       if (lane == 0) {
-        ok = mbar_wait(&bar->empty[s], ((i / L::kStages) & 1) ^ 1, abort_flag, a.err_word);
+        ok = mbar_wait(&bar->empty[s], tiles.empty_parity(), abort_flag, a.err_word);
         if (ok) {
           mbar_arrive_expect_tx(&bar->full[s], L::kYBytes + (has ? L::kBBytes : 0));
           tma_load_2d(dst, &tm_y, &bar->full[s], c * 128, row);
@@ -568,12 +567,13 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
         }
       }
       ok = __shfl_sync(0xffffffffu, ok, 0);
+      if (ok) tiles.arm();
       if (ok && changed && has) {
         if (!waited) pdl_wait();               // u comes from the shrink
         waited = true;
-        const int ub = u % L::kUBuffers;
+        const int ub = us.slot();
         if (lane == 0) {
-          ok = mbar_wait(&bar->u_empty[ub], ((u / L::kUBuffers) & 1) ^ 1, abort_flag, a.err_word);
+          ok = mbar_wait(&bar->u_empty[ub], us.empty_parity(), abort_flag, a.err_word);
           if (ok) {
             mbar_arrive_expect_tx(&bar->u_full[ub], L::kUBytes);
 #pragma unroll
@@ -582,19 +582,16 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
           }
         }
         ok = __shfl_sync(0xffffffffu, ok, 0);
-        if (ok) ++u;
+        if (ok) us.arm();
       }
-      if (!ok) ++i;
     }
     if (!waited) pdl_wait();    // never end before the shrink has
-    // Never leave a copy in flight into shared memory (loads whose stage was
-    // not armed have a completed phase of this parity, or run out).
-    if (lane == 0 && *abort_flag) {
+    // Never leave a copy in flight into shared memory: the readers may have
+    // given up, or give up after this.
+    if (lane == 0) {
       int never = 0;
-      for (int j = i > L::kStages ? i - L::kStages : 0; j < i; ++j)
-        mbar_wait(&bar->full[j % L::kStages], (j / L::kStages) & 1, &never, a.err_word);
-      for (int j = u > L::kUBuffers ? u - L::kUBuffers : 0; j < u; ++j)
-        mbar_wait(&bar->u_full[j % L::kUBuffers], (j / L::kUBuffers) & 1, &never, a.err_word);
+      tiles.for_each_open([&](int s, uint32_t parity) { mbar_wait(&bar->full[s], parity, &never, a.err_word); });
+      us.for_each_open([&](int s, uint32_t parity) { mbar_wait(&bar->u_full[s], parity, &never, a.err_word); });
     }
   } else if (warp == 1) {
     // -------------------------------------------------------------- MMA issuer

@@ -42,6 +42,27 @@ __device__ __forceinline__ int request_of_row(const int32_t* __restrict__ starts
   return s;
 }
 
+// A producer's ring of kSlots shared-memory slots.  Load j goes to slot j %
+// kSlots and completes phase j / kSlots of the slot's "full" barrier.  `armed`
+// counts the loads that have been issued: arm() stands behind each, and nowhere
+// else, so that a producer which gives up knows what is still on its way.
+template <int kSlots>
+struct LoadRing {
+  int armed = 0;
+  __host__ __device__ int slot() const { return armed % kSlots; }
+  // parity of the slot's "empty" barrier to wait for before the next load
+  __host__ __device__ uint32_t empty_parity() const {
+    return static_cast<uint32_t>(((armed / kSlots) & 1) ^ 1);
+  }
+  __host__ __device__ void arm() { ++armed; }
+  // f(slot, parity of its "full" barrier) for the loads that may be in flight
+  template <typename F>
+  __host__ __device__ void for_each_open(F f) const {
+    for (int j = armed > kSlots ? armed - kSlots : 0; j < armed; ++j)
+      f(j % kSlots, static_cast<uint32_t>((j / kSlots) & 1));
+  }
+};
+
 // Programmatic dependent launch: wait until the kernels this one depends on
 // have completed and their writes are visible (returns at once when the
 // launch carries no such dependency); let the next kernel's blocks start.

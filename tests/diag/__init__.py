@@ -1,7 +1,7 @@
 """Test-only diagnostic kernels (``libbsa_diag.so``, built from ``diag.cu`` by
-``build.py``): the softmax kernels' two exponential paths and one bounded
-mbarrier wait that is made to time out.  Nothing in the package loads this
-library."""
+``build.py``): the softmax kernels' two exponential paths, one bounded
+mbarrier wait that is made to time out, and the producers' ring of loads on the
+host.  Nothing in the package loads this library."""
 
 from __future__ import annotations
 
@@ -26,6 +26,8 @@ def load():
         lib.bsa_diag_unarmed_wait.argtypes = [ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p,
                                               ctypes.c_void_p]
         lib.bsa_diag_unarmed_wait.restype = ctypes.c_int32
+        lib.bsa_diag_load_ring.argtypes = [ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p]
+        lib.bsa_diag_load_ring.restype = ctypes.c_int32
         _lib = lib
     return _lib
 
@@ -55,3 +57,14 @@ def unarmed_wait(timeout_ns: int, err_word: torch.Tensor):
         raise RuntimeError(f"bsa_diag_unarmed_wait failed ({rc})")
     torch.cuda.synchronize(err_word.device)
     return tuple(int(x) for x in result.cpu())
+
+
+def load_ring(slots: int, loads: int):
+    """``LoadRing<slots>`` on the host: ``(slot, empty parity)`` of each load and
+    ``(slot, full parity)`` of those that may be in flight after the last."""
+    out = (ctypes.c_int32 * (2 * (loads + slots)))()
+    n = load().bsa_diag_load_ring(slots, loads, out)
+    if n < 0:
+        raise RuntimeError(f"bsa_diag_load_ring failed ({n})")
+    pairs = [(out[2 * i], out[2 * i + 1]) for i in range(loads + n)]
+    return pairs[:loads], pairs[loads:]

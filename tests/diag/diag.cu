@@ -6,12 +6,33 @@
 //   * bsa_diag_unarmed_wait: one bounded mbarrier wait on a barrier that
 //     nothing arrives on, with a caller-chosen short limit, so a test can see
 //     the timeout path report kErrWaitTimeout and return (no trap, no fault,
-//     no unbounded wait).
+//     no unbounded wait);
+//   * bsa_diag_load_ring: the host's run of LoadRing (packed_common.cuh), what a
+//     producer of the packed operators' kernels waits for before it gives up.
 #include <stdint.h>
 
 #include "bsa_common.cuh"
+#include "packed_common.cuh"
 
 namespace {
+
+// (slot, empty parity) of each of `loads` loads, then (slot, full parity) of
+// those that may be in flight after them; returns the number of the latter.
+template <int kSlots>
+int load_ring(int loads, int32_t* out) {
+  bsa::LoadRing<kSlots> ring;
+  for (int j = 0; j < loads; ++j, ring.arm()) {
+    *out++ = ring.slot();
+    *out++ = static_cast<int32_t>(ring.empty_parity());
+  }
+  int open = 0;
+  ring.for_each_open([&](int slot, uint32_t parity) {
+    *out++ = slot;
+    *out++ = static_cast<int32_t>(parity);
+    ++open;
+  });
+  return open;
+}
 
 __global__ void exp2_kernel(const float* __restrict__ x, float* __restrict__ y, int64_t n,
                             int mode) {
@@ -66,6 +87,19 @@ __attribute__((visibility("default"))) int bsa_diag_exp2(const float* x, float* 
   exp2_kernel<<<static_cast<unsigned>((pairs + 255) / 256), 256, 0,
                 static_cast<cudaStream_t>(stream)>>>(x, y, n, mode);
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
+}
+
+// On the host; out holds 2 * (loads + slots) values.
+__attribute__((visibility("default"))) int bsa_diag_load_ring(int32_t slots, int32_t loads, int32_t* out) {
+  if (out == nullptr || loads < 0) return -1;
+  switch (slots) {
+    case 1: return load_ring<1>(loads, out);
+    case 2: return load_ring<2>(loads, out);
+    case 3: return load_ring<3>(loads, out);
+    case 4: return load_ring<4>(loads, out);
+    case 8: return load_ring<8>(loads, out);
+    default: return -1;
+  }
 }
 
 // timeout_ns must lie in (0, 1 s]: the wait always runs to its limit.

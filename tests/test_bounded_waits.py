@@ -24,3 +24,33 @@ def test_no_wait_without_a_limit(name):
     text = code(name)
     assert not re.search(r"\bbar\.sync|\bbarrier\.sync|named_bar_sync|\btry_wait|\btest_wait", text)
     assert text.count("bar.red") == (name == "lora.cu")
+
+
+def test_producers_count_their_loads_in_one_place():
+    """lora.cu's producers wait, when they give up, for the loads that their ring
+    has counted, and a ring counts behind an issued load only."""
+    text = code("lora.cu")
+    assert len(re.findall(r"LoadRing<", text)) == 3 == len(re.findall(r"\.arm\(\)", text))
+    assert len(re.findall(r"for_each_open\(", text)) == 3
+    assert not re.search(r"for \(int j = [^;]*>", text)      # no window of its own
+    assert not re.search(r"\*abort_flag\) *{", text)         # whoever gives up, and whenever
+
+
+@pytest.mark.parametrize("slots", [1, 2, 3, 4, 8])
+@pytest.mark.parametrize("loads", range(0, 27))
+def test_ring_of_loads(slots, loads):
+    """Against barriers that complete phase after phase: a load waits for the
+    phase that its slot's last reader completes, and after the last load exactly
+    the last one of each slot is waited for, at its own phase."""
+    import diag
+    taken, open_ = diag.load_ring(slots, loads)
+    phases = [0] * slots                    # loads of each slot so far
+    for j, (slot, parity) in enumerate(taken):
+        assert slot == j % slots
+        # phase k of "empty" completes when load k of the slot has been read; the
+        # wait before load k is for phase k - 1, and passes at once for k = 0
+        assert parity == (phases[slot] - 1) % 2
+        phases[slot] += 1
+    assert sorted(s for s, _ in open_) == [s for s in range(slots) if phases[s]]
+    for slot, parity in open_:
+        assert parity == (phases[slot] - 1) % 2
