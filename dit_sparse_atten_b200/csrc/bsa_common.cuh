@@ -120,6 +120,18 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity,
   return mbar_wait_for(bar, parity, abort_flag, err_word, kWaitTimeoutNs);
 }
 
+// The wait for what a kernel has in flight (copies into its shared memory, MMAs)
+// before it ends.  mbar_wait would give up after a few polls where another CTA
+// has timed out, or this one is aborting, and the work would outlive the CTA:
+// here only the wait's own limit counts.  `late` (starting at 0) is set when one
+// runs out, which is reported; later waits with it only look.
+__device__ __forceinline__ bool mbar_drain(uint64_t* bar, uint32_t parity, int* late, int* err_word,
+                                           uint64_t timeout_ns = kWaitTimeoutNs) {
+  if (mbar_wait_for(bar, parity, late, nullptr, timeout_ns)) return true;
+  if (err_word) atomicOr(err_word, kErrWaitTimeout);
+  return false;
+}
+
 // True when an earlier timeout was recorded in the error word: kernels then
 // skip their work so a systemic failure ends quickly instead of timing out
 // CTA by CTA.  Cleared by the host when it reads the word.

@@ -276,8 +276,8 @@ __global__ void __launch_bounds__(kShrinkThreads)
         loads.arm();
       }
       // Never leave a copy in flight into shared memory.
-      int never = 0;
-      loads.for_each_open([&](int s, uint32_t parity) { mbar_wait(&bar->full[s], parity, &never, a.err_word); });
+      int late = 0;
+      loads.for_each_open([&](int s, uint32_t parity) { mbar_drain(&bar->full[s], parity, &late, a.err_word); });
     }
   } else if (warp == 1) {
     if (lane == 0) {
@@ -294,9 +294,9 @@ __global__ void __launch_bounds__(kShrinkThreads)
           umma_bf16_ss(tmem, xd + kk * 2, ad + kk * 2, idesc, (i > 0 || kk > 0) ? 1u : 0u);
         umma_commit(&bar->empty[s]);
       }
-      int never = 0;
+      int late = 0;
       umma_commit(&bar->done);
-      mbar_wait(&bar->done, 0, &never, a.err_word);
+      mbar_drain(&bar->done, 0, &late, a.err_word);
     }
   }
   __syncthreads();
@@ -589,9 +589,9 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
     // Never leave a copy in flight into shared memory: the readers may have
     // given up, or give up after this.
     if (lane == 0) {
-      int never = 0;
-      tiles.for_each_open([&](int s, uint32_t parity) { mbar_wait(&bar->full[s], parity, &never, a.err_word); });
-      us.for_each_open([&](int s, uint32_t parity) { mbar_wait(&bar->u_full[s], parity, &never, a.err_word); });
+      int late = 0;
+      tiles.for_each_open([&](int s, uint32_t parity) { mbar_drain(&bar->full[s], parity, &late, a.err_word); });
+      us.for_each_open([&](int s, uint32_t parity) { mbar_drain(&bar->u_full[s], parity, &late, a.err_word); });
     }
   } else if (warp == 1) {
     // -------------------------------------------------------------- MMA issuer
@@ -629,9 +629,9 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
       if (changed) open = has;
     }
     if (lane == 0) {
-      int never = 0;
+      int late = 0;
       umma_commit(&bar->drain);
-      mbar_wait(&bar->drain, 0, &never, a.err_word);
+      mbar_drain(&bar->drain, 0, &late, a.err_word);
     }
   } else {
     // -------------------------------------------------------------- epilogue

@@ -335,15 +335,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (lane == 0) {
       // Never leave a copy, or an answer, in flight into shared memory.
-      int never = 0;
+      int late = 0;
 #pragma unroll
       for (int s = 0; s < kSlots; ++s)
         if (armed & (1u << s))
-          mbar_wait(&bar->slot_full[s], (armed_phase >> s) & 1u, &never, a.err_word);
+          mbar_drain(&bar->slot_full[s], (armed_phase >> s) & 1u, &late, a.err_word);
       for (int j = max(0, masked - kMaskedRing); j < masked; ++j)
-        mbar_wait(&bar->masked_full[j % kMaskedRing], (j / kMaskedRing) & 1, &never, a.err_word);
-      if (loads) mbar_wait(&bar->q_full, (loads - 1) & 1, &never, a.err_word);
-      if (asked != answers) mbar_wait(&bar->next_full, answers & 1, &never, a.err_word);
+        mbar_drain(&bar->masked_full[j % kMaskedRing], (j / kMaskedRing) & 1, &late, a.err_word);
+      if (loads) mbar_drain(&bar->q_full, (loads - 1) & 1, &late, a.err_word);
+      if (asked != answers) mbar_drain(&bar->next_full, answers & 1, &late, a.err_word);
     }
    } else if (warp == kMmaWarp || warp == kMmaWarp + 1) {
     // ------------------------------------------------------------ MMA issuers
@@ -462,9 +462,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      int never = 0;
+      int late = 0;
       commit(&bar->drain[t]);
-      mbar_wait(&bar->drain[t], 0, &never, a.err_word);
+      mbar_drain(&bar->drain[t], 0, &late, a.err_word);
     }
    } else if (warp == kCheckWarp) {
     // ------------------------------------------------------ masked V blocks

@@ -418,10 +418,10 @@ __global__ void __launch_bounds__(kMaxThreads, kMinBlocks)
     }
     if (!mbar_wait(&full[stage], phase, &abort_flag, a.err_word)) {
       // Never leave a copy in flight into shared memory.
-      int never = 0;
+      int late = 0;
       if (threadIdx.x == 0)
         for (int i = 0; i < stages && row + i * step < a.rows; ++i)
-          mbar_wait(&full[(stage + i) % stages], stage + i < stages ? phase : phase ^ 1, &never,
+          mbar_drain(&full[(stage + i) % stages], stage + i < stages ? phase : phase ^ 1, &late,
                     a.err_word);
       break;
     }

@@ -23,8 +23,8 @@ def load():
         lib.bsa_diag_exp2.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64,
                                       ctypes.c_int32, ctypes.c_void_p]
         lib.bsa_diag_exp2.restype = ctypes.c_int32
-        lib.bsa_diag_unarmed_wait.argtypes = [ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p,
-                                              ctypes.c_void_p]
+        lib.bsa_diag_unarmed_wait.argtypes = [ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p,
+                                              ctypes.c_void_p, ctypes.c_void_p]
         lib.bsa_diag_unarmed_wait.restype = ctypes.c_int32
         lib.bsa_diag_load_ring.argtypes = [ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p]
         lib.bsa_diag_load_ring.restype = ctypes.c_int32
@@ -47,11 +47,12 @@ def exp2(x: torch.Tensor, mode: str = "poly") -> torch.Tensor:
     return y
 
 
-def unarmed_wait(timeout_ns: int, err_word: torch.Tensor):
-    """Run one bounded wait on a barrier nobody arrives on; returns the device
-    result ``(completed, elapsed_ns, abort_flag)`` after synchronising."""
+def unarmed_wait(timeout_ns: int, err_word: torch.Tensor, drain: bool = False):
+    """Run one bounded wait (``drain``: the kernels' last one) on a barrier nobody
+    arrives on; returns the device result ``(completed, elapsed_ns, abort_flag)``
+    after synchronising."""
     result = torch.full((3,), -1, dtype=torch.int64, device=err_word.device)
-    rc = load().bsa_diag_unarmed_wait(int(timeout_ns), err_word.data_ptr(), result.data_ptr(),
+    rc = load().bsa_diag_unarmed_wait(int(timeout_ns), int(drain), err_word.data_ptr(), result.data_ptr(),
                                       _stream(err_word.device))
     if rc != 0:
         raise RuntimeError(f"bsa_diag_unarmed_wait failed ({rc})")

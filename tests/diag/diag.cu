@@ -54,7 +54,9 @@ __global__ void exp2_kernel(const float* __restrict__ x, float* __restrict__ y, 
 // never comes, and waits on phase 0 with the product's bounded wait.  The
 // result records whether the wait returned true, the nanoseconds it took and
 // the CTA's abort flag afterwards.
-__global__ void unarmed_wait_kernel(uint64_t timeout_ns, int* err_word,
+// `drain`: the same with mbar_drain, whose limit an earlier timeout in the error
+// word must not cut short; the flag is then its `late`.
+__global__ void unarmed_wait_kernel(uint64_t timeout_ns, int drain, int* err_word,
                                     long long* result) {
   __shared__ __align__(8) uint64_t bar;
   __shared__ int abort_flag;
@@ -66,7 +68,8 @@ __global__ void unarmed_wait_kernel(uint64_t timeout_ns, int* err_word,
   __syncwarp();
   if (threadIdx.x == 0) {
     const uint64_t t0 = bsa::global_timer_ns();
-    const bool done = bsa::mbar_wait_for(&bar, 0, &abort_flag, err_word, timeout_ns);
+    const bool done = drain ? bsa::mbar_drain(&bar, 0, &abort_flag, err_word, timeout_ns)
+                            : bsa::mbar_wait_for(&bar, 0, &abort_flag, err_word, timeout_ns);
     const uint64_t t1 = bsa::global_timer_ns();
     result[0] = done ? 1 : 0;
     result[1] = static_cast<long long>(t1 - t0);
@@ -103,14 +106,14 @@ __attribute__((visibility("default"))) int bsa_diag_load_ring(int32_t slots, int
 }
 
 // timeout_ns must lie in (0, 1 s]: the wait always runs to its limit.
-__attribute__((visibility("default"))) int bsa_diag_unarmed_wait(int64_t timeout_ns,
+__attribute__((visibility("default"))) int bsa_diag_unarmed_wait(int64_t timeout_ns, int32_t drain,
                                                                  int32_t* err_word,
                                                                  long long* result,
                                                                  void* stream) {
   if (err_word == nullptr || result == nullptr) return -1;
   if (timeout_ns <= 0 || timeout_ns > 1000ll * 1000ll * 1000ll) return -1;
   unarmed_wait_kernel<<<1, 32, 0, static_cast<cudaStream_t>(stream)>>>(
-      static_cast<uint64_t>(timeout_ns), err_word, result);
+      static_cast<uint64_t>(timeout_ns), drain, err_word, result);
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
 }
 

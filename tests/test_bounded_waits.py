@@ -54,3 +54,12 @@ def test_ring_of_loads(slots, loads):
     assert sorted(s for s, _ in open_) == [s for s in range(slots) if phases[s]]
     for slot, parity in open_:
         assert parity == (phases[slot] - 1) % 2
+
+
+@pytest.mark.parametrize("name", PACKED)
+def test_last_waits_have_their_own_limit(name):
+    """A wait that must outlast an abort does not go by the abort flag's rules."""
+    text = code(name)
+    for call in re.findall(r"mbar_wait\([^;]*;", text):
+        assert re.search(r",\s*(abort_flag|&abort_flag)\s*,", call), call
+    assert len(re.findall(r"int late = 0;", text)) <= len(re.findall(r"mbar_drain\(", text))
