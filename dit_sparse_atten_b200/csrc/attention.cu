@@ -234,10 +234,10 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         if (ok) ok = load(&tm_v, block_id(j));
       }
       // Never leave a copy in flight into shared memory.
-      int never = 0;
+      int late = 0;
 #pragma unroll
       for (int s = 0; s < L::kSlots; ++s)
-        if (armed & (1u << s)) mbar_wait(&bar->slot_full[s], (armed_phase >> s) & 1u, &never, a.err_word);
+        if (armed & (1u << s)) mbar_drain(&bar->slot_full[s], (armed_phase >> s) & 1u, &late, a.err_word);
     }
    } else if (warp == kMmaWarp || warp == kPvWarp) {
     // ------------------------------------------------------------ MMA issuers
@@ -276,9 +276,9 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         umma_commit(&bar->s_full[sb]);
         umma_commit(&bar->slot_empty[s]);
       }
-      int never = 0;
+      int late = 0;
       umma_commit(&bar->drain[0]);
-      mbar_wait(&bar->drain[0], 0, &never, a.err_word);
+      mbar_drain(&bar->drain[0], 0, &late, a.err_word);
     } else if (warp == kPvWarp && lane == 0 && n > 0) {
       const uint32_t idesc_o = idesc_bf16_f32(128, kHeadDim, true);
       const uint64_t vdesc0 = sdesc_sw128(ring_addr, L::kSlotPanel, 1024);
@@ -301,9 +301,9 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         umma_commit(&bar->o_done[sb]);
         umma_commit(&bar->slot_empty[s]);
       }
-      int never = 0;
+      int late = 0;
       umma_commit(&bar->drain[1]);
-      mbar_wait(&bar->drain[1], 0, &never, a.err_word);
+      mbar_drain(&bar->drain[1], 0, &late, a.err_word);
     }
    }
   } else {

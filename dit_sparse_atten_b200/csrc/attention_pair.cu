@@ -352,11 +352,11 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         prev_kb = kb;
       }
       // Never leave a copy in flight into shared memory.
-      int never = 0;
+      int late = 0;
 #pragma unroll
       for (int s = 0; s < kPairSlots; ++s)
         if (armed & (1u << s))
-          mbar_wait(&bar->slot_full[s], (armed_phase >> s) & 1u, &never, a.err_word);
+          mbar_drain(&bar->slot_full[s], (armed_phase >> s) & 1u, &late, a.err_word);
     }
    } else if (warp == kPairMmaWarp) {
     // ------------------------------------------------------------ MMA issuer
@@ -445,9 +445,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         if (mask == 0) break;
         prev_mask = mask;
       }
-      int never = 0;
+      int late = 0;
       umma_commit(&bar->drain);
-      mbar_wait(&bar->drain, 0, &never, a.err_word);
+      mbar_drain(&bar->drain, 0, &late, a.err_word);
     }
    }
   } else {

@@ -334,11 +334,11 @@ __global__ void __launch_bounds__(MassShape<LOG2S>::kThreads, 1)
         armed |= 1u << s;
         armed_phase = (armed_phase & ~(1u << s)) | (ph << s);
       }
-      int never = 0;
-      mbar_wait(&bar->q_full, 0, &never, a.err_word);
+      int late = 0;
+      mbar_drain(&bar->q_full, 0, &late, a.err_word);
 #pragma unroll
       for (int s = 0; s < kRing; ++s)
-        if (armed & (1u << s)) mbar_wait(&bar->slot_full[s], (armed_phase >> s) & 1u, &never, a.err_word);
+        if (armed & (1u << s)) mbar_drain(&bar->slot_full[s], (armed_phase >> s) & 1u, &late, a.err_word);
     }
   } else if (warp == Shape::kMmaWarp) {
     if (lane == 0) {
@@ -361,9 +361,9 @@ __global__ void __launch_bounds__(MassShape<LOG2S>::kThreads, 1)
         umma_commit(&bar->s_full[i & 1]);
         umma_commit(&bar->slot_empty[s]);
       }
-      int never = 0;
+      int late = 0;
       umma_commit(&bar->drain);
-      mbar_wait(&bar->drain, 0, &never, a.err_word);
+      mbar_drain(&bar->drain, 0, &late, a.err_word);
     }
   } else {
     const int part = warp >> 2;

@@ -1,6 +1,6 @@
-"""Waits in the packed operators' kernels, by reading their sources: a warp that
-gives up after a timeout leaves its loop, so nothing may wait for it without a
-limit."""
+"""Waits in the kernels, by reading their sources: a warp that gives up after a
+timeout leaves its loop, so nothing may wait for it without a limit, and what
+is in flight is waited for all the same."""
 
 import re
 from pathlib import Path
@@ -56,7 +56,7 @@ def test_ring_of_loads(slots, loads):
         assert parity == (phases[slot] - 1) % 2
 
 
-@pytest.mark.parametrize("name", PACKED)
+@pytest.mark.parametrize("name", sorted(p.name for p in CSRC.glob("*.cu")))
 def test_last_waits_have_their_own_limit(name):
     """A wait that must outlast an abort does not go by the abort flag's rules."""
     text = code(name)
