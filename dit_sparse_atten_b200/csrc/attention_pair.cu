@@ -480,11 +480,11 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       int kb = 0;
       if (need_kb) {
         ok = mbar_wait(&bar->kb_full[t], j & 1, abort_flag, a.err_word);
-        if (!ok) break;
         kb = bar->kb_box[t];
       }
-      ok = mbar_wait(&bar->s_full[t], j & 1, abort_flag, a.err_word);
-      if (!ok) break;
+      if (ok) ok = mbar_wait(&bar->s_full[t], j & 1, abort_flag, a.err_word);
+      ok = __all_sync(0xffffffffu, ok);
+      if (kHalves == 1 && !ok) break;
       tc_fence_after();
       const int64_t valid = a.tokens - static_cast<int64_t>(kb) * 128 - hf * kColsPerThread;
       const bool partial = kTail && valid < kColsPerThread;
@@ -492,9 +492,11 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       float mrow = row_max<kColsPerThread, kPairKept>(sbuf, partial, valid, keep) * c;
       if constexpr (kHalves == 2) {
         // Both halves' S columns are in registers now, so P may overwrite
-        // them after this barrier; the row max is the larger half's.
+        // them after this barrier; the row max is the larger half's.  A half
+        // whose waits ran out comes here too (with any S), and both leave.
         xmax[xidx(j & 1, hf)] = mrow;
-        named_bar_sync(pair_bar, 64);
+        ok = named_bar_and(pair_bar, 64, ok);
+        if (!ok) break;
         mrow = fmaxf(mrow, xmax[xidx(j & 1, hf ^ 1)]);
       }
       const bool need = mrow > m_run + kRescaleThreshold;

@@ -132,6 +132,22 @@ __device__ __forceinline__ bool mbar_drain(uint64_t* bar, uint32_t parity, int* 
   return false;
 }
 
+// Meeting of some of a CTA's warps (`threads` of them, named barrier `id`) where
+// they agree whether to go on: true if all came with `ok`.  A warp whose wait
+// ran out comes too; one that left alone would be waited for without a limit.
+__device__ __forceinline__ bool named_bar_and(uint32_t id, uint32_t threads, bool ok) {
+  uint32_t all;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %3, 0;\n\t"
+      "bar.red.and.pred q, %1, %2, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(all)
+      : "r"(id), "r"(threads), "r"(ok ? 1u : 0u)
+      : "memory");
+  return all != 0;
+}
+
 // True when an earlier timeout was recorded in the error word: kernels then
 // skip their work so a systemic failure ends quickly instead of timing out
 // CTA by CTA.  Cleared by the host when it reads the word.

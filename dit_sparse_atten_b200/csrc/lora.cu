@@ -445,20 +445,6 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void*
                : "memory");
 }
 
-// Meeting of 128 threads: whether all of them came with `ok`.
-__device__ __forceinline__ bool all_128(int barrier, bool ok) {
-  uint32_t all;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.u32 p, %2, 0;\n\t"
-      "bar.red.and.pred q, %1, 128, p;\n\t"
-      "selp.u32 %0, 1, 0, q;\n\t}"
-      : "=r"(all)
-      : "r"(barrier), "r"(ok ? 1u : 0u)
-      : "memory");
-  return all != 0;
-}
-
 // Walks this CTA's tiles; each warp has its own copy.  Items are runs of
 // `run` column tiles of one row tile; CTA b takes runs b, b + grid, ...
 struct ExpandWalk {
@@ -693,7 +679,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
       // A warp that has given up comes here too, and the group leaves together:
       // one that left alone would be waited for without a limit.  (An mbarrier
       // that only the leader waits on: 320 us for the 57,600 rows against 315.)
-      ok = all_128(1 + db, ok);
+      ok = named_bar_and(1 + db, 128, ok);
       if (!ok) break;
       if (leader) {
         if (whole) {

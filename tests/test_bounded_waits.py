@@ -20,10 +20,10 @@ def code(name):
 def test_no_wait_without_a_limit(name):
     """Whole-block and whole-cluster barriers, which every thread reaches, and
     mbar_wait; no wait of its own, and some of the warps meet only to agree
-    whether to go on (bar.red), in one place a file."""
+    whether to go on (named_bar_and)."""
     text = code(name)
     assert not re.search(r"\bbar\.sync|\bbarrier\.sync|named_bar_sync|\btry_wait|\btest_wait", text)
-    assert text.count("bar.red") == (name == "lora.cu")
+    assert "bar.red" not in text
 
 
 def test_producers_count_their_loads_in_one_place():
@@ -63,3 +63,12 @@ def test_last_waits_have_their_own_limit(name):
     for call in re.findall(r"mbar_wait\([^;]*;", text):
         assert re.search(r",\s*(abort_flag|&abort_flag)\s*,", call), call
     assert len(re.findall(r"int late = 0;", text)) <= len(re.findall(r"mbar_drain\(", text))
+
+
+def test_pair_kernel_leaves_its_loop_together():
+    """The halves of a row meet once a block inside the loop; no way out of the
+    loop lies before that meeting."""
+    text = code("attention_pair.cu")
+    loop = text[text.index("for (int j = 0; ok && j < n; ++j) {"):]
+    loop = loop[:loop.index("named_bar_and(pair_bar, 64, ok)")]
+    assert re.findall(r"[^\n]*break;", loop) == ["      if (kHalves == 1 && !ok) break;"]
