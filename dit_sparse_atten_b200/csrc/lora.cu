@@ -337,7 +337,10 @@ template <int KB, int kGroups>
 __global__ void __launch_bounds__(kWarps * 32) lora_expand_few_kernel(const LoraArgs a) {
   const int64_t slot = blockIdx.x / a.col_ctas;
   const Tile t = find_tile<kExpandRows>(a, slot);
-  if (t.rows == 0) return;
+  if (t.rows == 0) {
+    pdl_wait();     // no block ends before the shrink has: what follows may reuse its workspace
+    return;
+  }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, q = lane & 3;
   const bool has = t.adapter >= 0;
@@ -522,7 +525,10 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
     fence_mbar_init();
   }
   __syncthreads();
-  if (bar->abort) return;     // uniform
+  if (bar->abort) {           // uniform
+    pdl_wait();               // never end before the shrink has
+    return;
+  }
   if (warp == 1) tmem_alloc(&bar->tmem_base, 256);
   tc_fence_before();
   __syncthreads();

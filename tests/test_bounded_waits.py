@@ -72,3 +72,15 @@ def test_pair_kernel_leaves_its_loop_together():
     loop = text[text.index("for (int j = 0; ok && j < n; ++j) {"):]
     loop = loop[:loop.index("named_bar_and(pair_bar, 64, ok)")]
     assert re.findall(r"[^\n]*break;", loop) == ["      if (kHalves == 1 && !ok) break;"]
+
+
+@pytest.mark.parametrize("kernel", ["lora_expand_few_kernel", "lora_expand_tiles_kernel"])
+def test_dependent_kernels_outlast_the_one_before(kernel):
+    """A kernel that may start while the one before it runs waits for that one on
+    every way out: the caller frees the workspace, and the next kernel of the
+    stream starts, when this one ends."""
+    text = code("lora.cu")
+    body = re.search(kernel + r"\([^{]*\{\n(.*?)\n\}\n", text, re.S).group(1)
+    before = [body[:m.start()].rstrip() for m in re.finditer(r"\breturn;", body)]
+    assert before and all(b.endswith("pdl_wait();") for b in before)
+    assert len(re.findall(r"pdl_wait\(\);", body)) >= len(before) + 1      # and the ordinary way
