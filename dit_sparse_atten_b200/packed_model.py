@@ -70,12 +70,18 @@ class PackedWanTransformer:
         if adapters is not None and len(adapters.blocks) != self.cfg.layers:
             raise ValueError("adapters must have the model's number of blocks")
         self.lengths = [math.prod(g) for g in self.grids]
+        self.text_lengths = [int(n) for n in text_lengths]
+        if min(self.lengths + self.text_lengths, default=0) < 0:
+            raise ValueError("grids and text lengths must not be negative")
         self.starts = row_starts(self.lengths, device)
-        self.text_starts = row_starts(text_lengths, device)
+        self.text_starts = row_starts(self.text_lengths, device)
         self.adapters = adapters
-        ids = [-1] * len(self.grids) if adapter_ids is None else list(adapter_ids)
+        ids = [-1] * len(self.grids) if adapter_ids is None else [int(i) for i in adapter_ids]
         if len(ids) != len(self.grids):
             raise ValueError("one adapter id for each grid")
+        count = adapters.scales.numel() if adapters is not None else 0
+        if any(not -1 <= i < count for i in ids):
+            raise ValueError(f"adapter ids must be in [-1, {count})")
         self.adapter_ids = torch.tensor(ids, dtype=torch.int32, device=device)
         self.request_starts = row_starts([1] * len(ids), device)   # a row for each request
         tables = [rotary_tables(self.cfg, g) for g in self.grids]
@@ -103,6 +109,11 @@ class PackedWanTransformer:
         dtype, device = w.patch[0].dtype, patches.device
         if len(timesteps) != len(self.grids):
             raise ValueError("one timestep for each request")
+        rows, text_rows = sum(self.lengths), sum(self.text_lengths)
+        if tuple(patches.shape) != (rows, w.patch[0].shape[1]):
+            raise ValueError(f"patches must be {(rows, w.patch[0].shape[1])}, a row for each token")
+        if tuple(ctx.shape) != (text_rows, cfg.dim):
+            raise ValueError(f"ctx must be {(text_rows, cfg.dim)}, the context of the packed texts")
         emb = torch.cat([timestep_embedding(t, cfg.freq_dim) for t in timesteps]).to(device, dtype)
         temb = _linear(F.silu(_linear(emb, w.time_1)), w.time_2)         # [requests, dim]
         time_factors = self.adapters.time_proj if self.adapters is not None else None
