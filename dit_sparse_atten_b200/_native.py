@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes
 import importlib.util
 import os
+import re
 import threading
 from pathlib import Path
 
@@ -105,6 +106,14 @@ def load_library(path: Path | None = None) -> ctypes.CDLL:
         return lib
 
 
+def binding_torch_version(path: Path | None = None) -> str | None:
+    """The torch version that ``_binding.so`` was compiled against (read from the
+    file, which need not be loadable)."""
+    path = BINDING_PATH if path is None else path
+    found = re.search(rb"bsa-binding-torch=([^\0]*)\0", path.read_bytes()) if path.exists() else None
+    return found.group(1).decode() if found else None
+
+
 def load_binding():
     """The compiled calls of the packed operators (``_binding.so``, csrc/binding.cpp)."""
     global _binding
@@ -113,6 +122,11 @@ def load_binding():
         if not BINDING_PATH.exists():
             raise RuntimeError(
                 f"{BINDING_PATH} is missing: build it with `python -m dit_sparse_atten_b200.csrc.build`")
+        built_for = binding_torch_version()
+        if built_for != str(torch.__version__):  # it reads tensors through that version's layout
+            raise RuntimeError(
+                f"{BINDING_PATH} was built for torch {built_for}, this is {torch.__version__}: build it "
+                "again with `python -m dit_sparse_atten_b200.csrc.build`")
         spec = importlib.util.spec_from_file_location(__package__ + "._binding", BINDING_PATH)
         module = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(module)

@@ -17,6 +17,10 @@
 
 #include "../../include/bsa.h"
 
+// What _native.py compares with the running torch before it loads this file.
+extern "C" __attribute__((used, visibility("default"))) const char bsa_binding_torch[] =
+    "bsa-binding-torch=" BSA_TORCH_VERSION;
+
 namespace {
 
 constexpr int kDevices = 64;

@@ -76,8 +76,14 @@ def build(force: bool = False, verbose_ptxas: bool = False) -> Path:
 
 
 def binding_up_to_date() -> bool:
+    import torch
+
+    from .._native import binding_torch_version
+
+    if binding_torch_version(BINDING) != str(torch.__version__):
+        return False
     sources = [CSRC / "binding.cpp", REPO / "include" / "bsa.h", Path(__file__)]
-    return BINDING.exists() and all(p.stat().st_mtime <= BINDING.stat().st_mtime for p in sources)
+    return all(p.stat().st_mtime <= BINDING.stat().st_mtime for p in sources)
 
 
 def build_binding(force: bool = False) -> Path:
@@ -93,6 +99,7 @@ def build_binding(force: bool = False) -> Path:
     torch_lib = str(Path(torch.__file__).resolve().parent / "lib")
     tmp = BINDING.with_suffix(".so.tmp")
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f'-DBSA_TORCH_VERSION="{torch.__version__}"',
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            *[f"-I{p}" for p in includes], str(CSRC / "binding.cpp"), "-o", str(tmp),
            f"-L{torch_lib}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]

@@ -150,3 +150,16 @@ def test_wide_integers_do_not_wrap():
     for t in (wide, torch.stack([wide, wide], 1)[:, 1]):
         got = kernels._starts_i32(t, "row_starts", torch.device("cpu"))
         assert got.dtype == torch.int32 and got.is_contiguous() and got.tolist() == want
+
+
+def test_binding_of_another_torch_is_refused(monkeypatch):
+    """The compiled front goes through torch's C++ types: one that was built for
+    another version is not loaded, and not taken for up to date."""
+    import torch
+    from dit_sparse_atten_b200.csrc import build
+    assert _native.binding_torch_version() == torch.__version__ and build.binding_up_to_date()
+    monkeypatch.setattr(_native, "_binding", None)
+    monkeypatch.setattr(torch, "__version__", "0.0.1")
+    assert not build.binding_up_to_date()
+    with pytest.raises(RuntimeError, match="was built for torch"):
+        _native.load_binding()
