@@ -15,10 +15,11 @@
 // slices of a tile are one thread-block cluster, whose CTAs sum each other's
 // float32 partial tiles through distributed shared memory in a fixed order.
 //
-// Measured: 57,600 rows, K = N = 5,120, rank 32, 296 us, 5.98 TB/s; 10,007
-// ragged rows, N = 13,824, rank 64, 126 us; 1,859 rows of 8 prompts, K = 4,096,
-// rank 128, 33 us and 32 single rows, N = 30,720, rank 16, 19 us, which are the
-// latency of the two launches.
+// Measured over several runs: 57,600 rows, K = N = 5,120, rank 32, 312 to 320
+// us, 5.5 to 5.7 TB/s (the best: 296); 10,007 ragged rows, N = 13,824,
+// rank 64, 130 to 134 us (126); 1,859 rows of 8 prompts, K = 4,096, rank 128, 33
+// us and 32 single rows, N = 30,720, rank 16, 19 us, which are the latency of
+// the two launches.
 //
 // A row tile never spans two requests: tile slot g of M rows belongs to
 // request s = #{i >= 1: floor(starts[i] / M) + i <= g} (floor(e/M) - floor(b/M)

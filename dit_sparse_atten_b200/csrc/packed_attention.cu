@@ -37,10 +37,11 @@
 // hand-overs, which two warps a scheduler hide only in part; the products take
 // 1,250 of tensor pipe (S of 64 keys 390 where 256 would be the full rate: Q is
 // read from shared memory for every 64 keys).  Measured: 16,380 causal tokens,
-// 16 / 4 heads, 840 us, 1,310 TFLOP/s; 21,967 tokens x 40 heads against prompts
-// of up to 512, 184 us; 16 causal prompts of 4,931 tokens, 69 us.  Earlier
-// forms: P over S's own columns with two S buffers of 64 keys 940 / 200 / 71 us,
-// one S of 128 keys 957 / 240 / 108, one issuer for both tiles 1,082 / 282; with
+// 16 / 4 heads, 975 to 995 us over several runs, 1,105 to 1,127 TFLOP/s; 21,967
+// tokens x 40 heads against prompts of up to 512, 209 to 219 us; 16 causal
+// prompts of 4,931 tokens, 68 us.  Earlier forms, in one run where this one took
+// 840 / 184 / 69 us back to back: P over S's own columns with two S buffers of 64
+// keys 940 / 200 / 71 us, one S of 128 keys 957 / 240 / 108, one issuer for both tiles 1,082 / 282; with
 // the next block's S loaded ahead into registers the softmax spills (1,630 us);
 // 16 softmax warps, tiles taking turns at the exponentials, and exponentials on
 // the FMA pipe were slower too.
@@ -49,13 +50,16 @@
 // combine_kernel joins.  An item of at most one tile's tokens is `paired`:
 // both tiles hold its queries and take alternate key blocks, each with a part of
 // its own, since one tile's softmax is slower than the loads.  Measured: 16
-// requests of one token over 250,000 keys, 40 / 8 heads, 180 us, 5.05 TB/s.
+// requests of one token over 250,000 keys, 40 / 8 heads, 205 to 212 us over
+// several runs, 4.3 to 4.4 TB/s (the best: 180 us, 5.05 TB/s).
 //
 // A value of V that is not finite at a key which part of the item must not see
 // (causal) cannot be kept out of those rows by P = 0; warp 11 zeroes such values
 // and notes their keys, fewer than 256 an item, and the softmax warps add them
 // to the results of the rows that see them (add_not_finite).  The cost does not
-// grow with the keys' number.
+// grow with the keys' number: 8,192 causal tokens, 8 / 1 heads, 304 us; with one
+// NaN 352, half of the values NaN 433, half of them +inf 1,282 (recomputing the
+// item's rows key by key: 7,500 / 25,200 / 26,200).
 //
 // Every mbarrier wait is bounded (bsa::mbar_wait); on a timeout the CTA sets
 // kErrWaitTimeout, drains its copies and MMAs, frees TMEM and exits.
@@ -776,8 +780,8 @@ cudaError_t launch_tiles(const CUtensorMap& tq, const CUtensorMap& tk, const CUt
 // average request has less than 1,024 keys; otherwise parts of part_blocks on
 // the average request, up to sixteen parts an SM (a part costs about a
 // microsecond beyond its loads).  Requests of a few tokens share a part between
-// both tiles and take parts of twice the keys (16 requests of one token over
-// 250,000 keys: 180 us, with parts of 4 blocks 187; one request of one token
+// both tiles and take parts of twice the keys (in one run: 16
+// requests of one token over 250,000 keys 180 us, with parts of 4 blocks 187; one request of one token
 // over 16,384 keys: 33 us against 39), unless that leaves more than half of the
 // SMs without one (25 tokens of 4 requests over 33,700 keys: 45 us, with parts
 // of 4 blocks 33).

@@ -12,10 +12,11 @@
 // 16-byte chunk, kChunks chunks a thread), so x and y are read once and r and
 // h written once.  The variance is taken around the mean in a second register
 // pass, not as E[v^2] - mean^2, which loses the variance of rows with a large
-// mean.  Measured: 57,600 x 5,120 bf16 rows with y and three modulations in
-// 367 us, 6.43 TB/s, the rate of a plain copy; before the resident kernel the
-// float32 modulation rows went through L1 for every row and the sums' fixed
-// instructions (380 a warp and row) filled the issue slots.
+// mean.  Measured: 57,600 x 5,120 bf16 rows with y and three modulations in 402
+// to 415 us over several runs, 5.7 to 5.9 TB/s (the best: 367 us, 6.43 TB/s, the
+// rate of a plain copy; the other times in this file are from that run).  Before
+// the resident kernel the float32 modulation rows went through L1 for every row
+// and the sums' fixed instructions (380 a warp and row) filled the issue slots.
 #include <cuda_fp16.h>
 
 #include <algorithm>
